@@ -83,6 +83,9 @@ def build(force: bool = False) -> str:
     includes, defines, link = torch_flags()
     common = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
               "-Wno-unused-result"]
+    # Packed fp32 arithmetic stays off: the compiler forms v_pk_*_f32 out of ordinary float code
+    # by itself, and some of their operand forms have given wrong results on this hardware.
+    device = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     # Debug / sanitizer build (SURVEY.md §5 race-detection row):
     #   LSTM_TS_BUILD_MODE=debug -> -O1 -g + device asserts
     #   LSTM_TS_ASAN=1           -> host AddressSanitizer on the bindings
@@ -90,12 +93,12 @@ def build(force: bool = False) -> str:
         common = [f"--offload-arch={ARCH}", "-O1", "-g", "-std=c++17",
                   "-fPIC", "-Wno-unused-result", "-DLSTM_TS_DEBUG"]
     if os.environ.get("LSTM_TS_ASAN") == "1":
-        common += ["-fsanitize=address", "-shared-libasan"]
+        common += ["-Xarch_host", "-fsanitize=address", "-shared-libasan"]
         link += ["-fsanitize=address", "-shared-libasan"]
     objs = []
     for src in SOURCES:
         obj = os.path.join(BUILD, os.path.splitext(src)[0] + ".o")
-        cmd = [HIPCC, "-c", os.path.join(CSRC, src), "-o", obj] + common
+        cmd = [HIPCC, "-c", os.path.join(CSRC, src), "-o", obj] + common + device
         if src.endswith(".cpp"):
             cmd += includes + defines + ["-x", "hip"]
         run(cmd)
