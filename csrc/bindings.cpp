@@ -11,6 +11,8 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
+#include "lm_ops.h"
+
 #include <set>
 #include <vector>
 
@@ -676,5 +678,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("multi_tensor_clip_scale", &multi_tensor_clip_scale);
     m.def("fused_sgd", &fused_sgd);
     m.def("fused_adam", &fused_adam);
+    register_lm_ops(m);
     m.attr("BUILT_FOR") = "gfx950";
 }

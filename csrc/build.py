@@ -13,6 +13,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 CSRC = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(CSRC)
@@ -21,7 +22,8 @@ BUILD = os.path.join(CSRC, ".hip_build")
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
-SOURCES = ["lstm_kernels.hip", "bindings.cpp"]
+SOURCES = ["lstm_kernels.hip", "distill.hip", "bindings.cpp", "lm_ops.cpp"]
+HEADERS = ["lm_common.h", "lm_ops.h"]
 OUT_SO = os.path.join(PKG, "_lstm_hip.so")
 
 
@@ -52,7 +54,7 @@ def torch_flags():
 
 def digest() -> str:
     h = hashlib.sha256()
-    for s in SOURCES + ["build.py"]:
+    for s in SOURCES + HEADERS + ["build.py"]:
         with open(os.path.join(CSRC, s), "rb") as f:
             h.update(f.read())
     h.update(ARCH.encode())
@@ -95,14 +97,16 @@ def build(force: bool = False) -> str:
     if os.environ.get("LSTM_TS_ASAN") == "1":
         common += ["-Xarch_host", "-fsanitize=address", "-shared-libasan"]
         link += ["-fsanitize=address", "-shared-libasan"]
-    objs = []
+    objs, cmds = [], []
     for src in SOURCES:
         obj = os.path.join(BUILD, os.path.splitext(src)[0] + ".o")
         cmd = [HIPCC, "-c", os.path.join(CSRC, src), "-o", obj] + common + device
         if src.endswith(".cpp"):
             cmd += includes + defines + ["-x", "hip"]
-        run(cmd)
+        cmds.append(cmd)
         objs.append(obj)
+    with ThreadPoolExecutor(max_workers=4) as pool:     # one compiler a source
+        list(pool.map(run, cmds))
     run([HIPCC, "-shared", "-fPIC", "-o", OUT_SO] + objs + link)
     json.dump({"digest": dig, "arch": ARCH}, open(stamp, "w"))
     print(f"built {OUT_SO}")

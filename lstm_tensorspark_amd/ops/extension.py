@@ -69,3 +69,11 @@ def use_hip(device: torch.device | str,
     # GPU path: the extension is mandatory (fail loudly if missing).
     get_extension()
     return True
+
+
+def use_hip_lm(t: torch.Tensor) -> bool:
+    """Backend of the operators around the language-model head (distill,
+    adapters, logits): their kernels take bf16, fp16 and, where an operator
+    says so, fp32 on the GPU; the CPU and fp64 run the reference."""
+    return use_hip(t.device) and t.dtype in (
+        torch.bfloat16, torch.float16, torch.float32)
