@@ -19,6 +19,10 @@ void launch_distill_fwd(int, const void*, long, const void*, long, int, const vo
 void launch_distill_bwd(int, const void*, long, const void*, long, int, const void*, long, int,
                         const long*, int, const float*, const float*, const float*, void*, long,
                         int, float, float, hipStream_t);
+void launch_adjust(int, const void*, long, void*, const void*, long, int, int, const void*, int,
+                   const void*, int, const float*, float, const float*, float, const float*,
+                   float, const void*, long, int, const float*, long, int, const unsigned*, long,
+                   long, int, hipStream_t);
 }
 
 namespace {
@@ -140,6 +144,81 @@ Tensor distill_bwd(Tensor logits, Tensor index, Tensor teacher, OptTensor target
     return dz;
 }
 
+// ------------------------------------------------------------------ logits of a decode step
+// A per-request number as a (B,) tensor; the scalar beside it is used where there is none.
+Tensor per_row(const OptTensor& t, const Tensor& logits, const char* name) {
+    if (!t.has_value()) return Tensor();
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == logits.size(0), name, " must be (B,)");
+    check_on(*t, logits, name);
+    return t->to(at::kFloat).contiguous();
+}
+const float* float_ptr(const Tensor& t) { return t.defined() ? (const float*)t.data_ptr() : nullptr; }
+
+Tensor adjust(Tensor logits, OptTensor history, OptTensor lengths, OptTensor prompts,
+              OptTensor repetition, double repetition_all, OptTensor presence,
+              double presence_all, OptTensor frequency, double frequency_all,
+              OptTensor bias_index, OptTensor bias, OptTensor allowed) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be (B, V) on GPU");
+    const long B = logits.size(0), V = logits.size(1);
+    TORCH_CHECK(V <= (1 << 30), "logits: V must be at most 2^30");
+    const c10::DeviceGuard guard(logits.device());
+    const int type = type_of(logits, "logits");
+    const Tensor z = rows_of(logits);
+    Tensor h, len, pre, bi, bv, ok;
+    int h64 = 0, l64 = 0, p64 = 0, i64 = 0;
+    if (history.has_value()) {
+        TORCH_CHECK(history->dim() == 2 && history->size(0) == B &&
+                        history->size(1) <= (1 << 30),
+                    "history must be (B, L)");
+        check_on(*history, logits, "history");
+        h64 = wide_index(*history, "history");
+        h = rows_of(*history);
+        auto per_request = [&](const OptTensor& t, Tensor& to, int& wide, const char* name) {
+            if (!t.has_value()) return;
+            TORCH_CHECK(t->dim() == 1 && t->size(0) == B, name, " must be (B,)");
+            check_on(*t, logits, name);
+            wide = wide_index(*t, name);
+            to = t->contiguous();
+        };
+        per_request(lengths, len, l64, "lengths");
+        per_request(prompts, pre, p64, "prompt_lengths");
+    }
+    const Tensor rep = per_row(repetition, logits, "repetition"),
+                 pres = per_row(presence, logits, "presence"),
+                 freq = per_row(frequency, logits, "frequency");
+    if (bias_index.has_value()) {
+        TORCH_CHECK(bias.has_value() && bias_index->dim() == 2 && bias_index->size(0) == B &&
+                        bias->sizes() == bias_index->sizes() && bias->size(1) <= (1 << 30),
+                    "bias_index and bias must be (B, K)");
+        check_on(*bias_index, logits, "bias_index");
+        check_on(*bias, logits, "bias");
+        i64 = wide_index(*bias_index, "bias_index");
+        bi = rows_of(*bias_index);
+        bv = rows_of(bias->to(at::kFloat));
+    }
+    if (allowed.has_value()) {
+        TORCH_CHECK(allowed->dim() == 2 && allowed->size(0) == B &&
+                        allowed->size(1) == (V + 31) / 32 && allowed->scalar_type() == at::kInt,
+                    "allowed must be (B, ceil(V / 32)) int32");
+        check_on(*allowed, logits, "allowed");
+        ok = rows_of(*allowed);
+    }
+    auto out = at::empty({B, V}, logits.options());
+    if (B == 0 || V == 0) return out;
+    auto ptr = [](const Tensor& t) -> const void* { return t.defined() ? t.data_ptr() : nullptr; };
+    auto stride = [](const Tensor& t) { return t.defined() ? row_stride(t) : 0; };
+    // an empty list has no data: it is no list
+    const bool past = h.defined() && h.size(1) > 0, some = bi.defined() && bi.size(1) > 0;
+    launch_adjust(type, z.data_ptr(), row_stride(z), out.data_ptr(), past ? ptr(h) : nullptr,
+                  stride(h), past ? (int)h.size(1) : 0, h64, ptr(len), l64, ptr(pre), p64,
+                  float_ptr(rep), (float)repetition_all, float_ptr(pres), (float)presence_all,
+                  float_ptr(freq), (float)frequency_all, some ? ptr(bi) : nullptr, stride(bi),
+                  i64, some ? float_ptr(bv) : nullptr, stride(bv), some ? (int)bi.size(1) : 0,
+                  (const unsigned*)ptr(ok), stride(ok), B, (int)V, stream_of(logits));
+    check_launch("adjust_logits");
+    return out;
+}
+
 }  // namespace
 
 void register_lm_ops(pybind11::module_& m) {
@@ -150,4 +229,9 @@ void register_lm_ops(pybind11::module_& m) {
     m.def("distill_bwd", &distill_bwd, "gradient of distill_fwd", py::arg("logits"),
           py::arg("index"), py::arg("teacher"), py::arg("targets") = py::none(), py::arg("stats"),
           py::arg("inv"), py::arg("grad"), py::arg("alpha"), py::arg("tau"));
+    m.def("adjust_logits", &adjust, "penalties, biases and masks on decode logits",
+          py::arg("logits"), py::arg("history"), py::arg("lengths"), py::arg("prompt_lengths"),
+          py::arg("repetition"), py::arg("repetition_all"), py::arg("presence"),
+          py::arg("presence_all"), py::arg("frequency"), py::arg("frequency_all"),
+          py::arg("bias_index"), py::arg("bias"), py::arg("allowed"));
 }

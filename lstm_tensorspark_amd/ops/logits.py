@@ -1,0 +1,163 @@
+"""Penalties, biases and grammar masks on the logits of a decode step.
+
+For a row (one request) with history h, of which the first `prompt_lengths`
+tokens are the prompt and the rest was generated:
+
+    seen  = v stands in h;  count = times v stands in the generated part
+    z1 = seen ? (z > 0 ? z / repetition : z * repetition) : z
+    z2 = z1 - frequency * count - presence * (count > 0)
+    z3 = z2 + the sum of the row's biases for v
+    out = allowed ? z3 : -inf
+
+computed in fp32 and rounded once to the logits' type, in one launch
+(csrc/logits.hip) that keeps nothing between steps: a request may join,
+leave, or be rewound by handing in another history.  bf16, fp16 and fp32 run
+the kernel on the GPU, the CPU and fp64 the reference below.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Union
+
+import torch
+
+from . import extension
+from .functional import _acc_dtype
+
+PerRow = Union[float, torch.Tensor, None]
+
+
+def pack_allowed(allowed: torch.Tensor) -> torch.Tensor:
+    """(B, V) truth values -> (B, ceil(V / 32)) int32: token v is bit v % 32
+    of word v // 32."""
+    if allowed.dim() != 2 or allowed.dtype != torch.bool:
+        raise ValueError("allowed must be (B, V) bool")
+    B, V = allowed.shape
+    pad = torch.nn.functional.pad(allowed, (0, -V % 32)).view(B, -1, 32)
+    bit = 1 << torch.arange(32, device=allowed.device)
+    word = (pad.long() * bit).sum(dim=2)
+    return torch.where(word >= 2 ** 31, word - 2 ** 32, word).to(torch.int32)
+
+
+def _ref_adjust(logits, history, lengths, prompt_lengths, repetition,
+                presence, frequency, bias_index, bias, allowed):
+    B, V = logits.shape
+    dev = logits.device
+    z = logits.to(_acc_dtype(logits.dtype))
+
+    def column(x):
+        return x.to(z.dtype)[:, None] if isinstance(x, torch.Tensor) else x
+
+    if history is not None:
+        h = history.long()
+        at = torch.arange(h.shape[1], device=dev)
+        n = h.new_full((B,), h.shape[1]) if lengths is None else lengths
+        p = h.new_zeros(B) if prompt_lengths is None else prompt_lengths
+        inside = (at < n[:, None]) & (h >= 0) & (h < V)
+        h = torch.where(inside, h, 0)
+        zero = torch.zeros(B, V, dtype=torch.long, device=dev)
+        seen = zero.scatter_add(1, h, inside.long()) > 0
+        count = zero.scatter_add(1, h, (inside & (at >= p[:, None])).long())
+        rho = column(repetition)
+        z = torch.where(seen, torch.where(z > 0, z / rho, z * rho), z)
+        z = torch.where(count > 0, z - column(frequency) * count
+                        - column(presence), z)
+    if bias_index is not None:
+        i = bias_index.long()
+        inside = (i >= 0) & (i < V)
+        z = z + torch.zeros_like(z).scatter_add(
+            1, torch.where(inside, i, 0),
+            torch.where(inside, bias.to(z.dtype), 0.0))
+    if allowed is not None:
+        v = torch.arange(V, device=dev)
+        bit = (allowed[:, v // 32] >> (v % 32).to(torch.int32)) & 1
+        z = z.masked_fill(bit == 0, -math.inf)
+    return z.to(logits.dtype)
+
+
+def _per_row(x: PerRow, none: float, B: int, dev, name: str):
+    """-> (tensor or None, number used without one)."""
+    if x is None:
+        return None, none
+    if isinstance(x, torch.Tensor):
+        if x.shape != (B,) or not x.dtype.is_floating_point:
+            raise ValueError(f"{name} must be a number or (B={B},) floating")
+        if x.device != dev:
+            raise ValueError(f"all tensors must be on {dev}")
+        return x, none
+    x = float(x)
+    if not math.isfinite(x):
+        raise ValueError(f"{name} must be finite, got {x}")
+    return None, x
+
+
+@torch.no_grad()
+def adjust_logits(logits: torch.Tensor,
+                  history: Optional[torch.Tensor] = None,
+                  lengths: Optional[torch.Tensor] = None,
+                  prompt_lengths: Optional[torch.Tensor] = None, *,
+                  repetition: PerRow = None, presence: PerRow = None,
+                  frequency: PerRow = None,
+                  bias_index: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None,
+                  allowed: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Adjusted logits, a new (B, V) tensor of the logits' type.
+
+    logits: (B, V), rows of any stride.
+    history: (B, L) int32 / int64 tokens; row b counts its first lengths[b]
+    (all L without `lengths`, never more than L) and takes the first
+    prompt_lengths[b] of them as prompt (none without).  Tokens outside
+    [0, V) are no tokens.
+    repetition (> 0, 1 changes nothing), presence, frequency: a number for
+    all rows or a floating (B,) tensor; they need a history.
+    bias_index, bias: (B, K) tokens and what is added to them; an index
+    outside [0, V) is none, the same index twice adds both.
+    allowed: (B, ceil(V / 32)) int32 as `pack_allowed` makes it.  A row that
+    allows nothing comes back as -inf throughout; a masked NaN is -inf.
+    Not differentiable: this is the serving path.
+    """
+    if logits.dim() != 2 or not logits.dtype.is_floating_point:
+        raise ValueError(
+            f"logits must be (B, V) floating, got {tuple(logits.shape)}")
+    B, V = logits.shape
+    dev = logits.device
+    index = (torch.int32, torch.int64)
+    if history is None:
+        if any(x is not None for x in (lengths, prompt_lengths, repetition,
+                                       presence, frequency)):
+            raise ValueError("penalties and lengths need a history")
+    elif (history.dim() != 2 or history.shape[0] != B
+          or history.dtype not in index):
+        raise ValueError(f"history must be (B={B}, L) int32 or int64")
+    for t, name in ((lengths, "lengths"), (prompt_lengths, "prompt_lengths")):
+        if t is not None and (t.shape != (B,) or t.dtype not in index):
+            raise ValueError(f"{name} must be (B={B},) int32 or int64")
+    if (bias_index is None) != (bias is None):
+        raise ValueError("bias_index and bias come together")
+    if bias is not None and (
+            bias_index.dim() != 2 or bias_index.shape[0] != B
+            or bias.shape != bias_index.shape
+            or bias_index.dtype not in index
+            or not bias.dtype.is_floating_point):
+        raise ValueError(f"bias_index must be (B={B}, K) int32 or int64 and "
+                         "bias floating of the same shape")
+    if allowed is not None and (allowed.dtype != torch.int32 or allowed.shape
+                                != (B, (V + 31) // 32)):
+        raise ValueError(f"allowed must be (B={B}, {(V + 31) // 32}) int32")
+    for t in (history, lengths, prompt_lengths, bias_index, bias, allowed):
+        if t is not None and t.device != dev:
+            raise ValueError(f"all tensors must be on {dev}")
+    rep, rep_all = _per_row(repetition, 1.0, B, dev, "repetition")
+    if rep is None and rep_all <= 0.0:
+        raise ValueError(f"repetition must be positive, got {rep_all}")
+    pres, pres_all = _per_row(presence, 0.0, B, dev, "presence")
+    freq, freq_all = _per_row(frequency, 0.0, B, dev, "frequency")
+    if extension.use_hip_lm(logits):
+        return extension.get_extension().adjust_logits(
+            logits, history, lengths, prompt_lengths, rep, rep_all, pres,
+            pres_all, freq, freq_all, bias_index, bias, allowed)
+    return _ref_adjust(logits, history, lengths, prompt_lengths,
+                       rep_all if rep is None else rep,
+                       pres_all if pres is None else pres,
+                       freq_all if freq is None else freq, bias_index, bias,
+                       allowed)
