@@ -22,7 +22,7 @@ BUILD = os.path.join(CSRC, ".hip_build")
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
-SOURCES = ["lstm_kernels.hip", "distill.hip", "logits.hip", "bindings.cpp", "lm_ops.cpp"]
+SOURCES = ["lstm_kernels.hip", "distill.hip", "logits.hip", "adapters.hip", "bindings.cpp", "lm_ops.cpp"]
 HEADERS = ["lm_common.h", "lm_ops.h"]
 OUT_SO = os.path.join(PKG, "_lstm_hip.so")
 

@@ -8,6 +8,7 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <vector>
 
 extern "C" {
@@ -23,6 +24,17 @@ void launch_adjust(int, const void*, long, void*, const void*, long, int, int, c
                    const void*, int, const float*, float, const float*, float, const float*,
                    float, const void*, long, int, const float*, long, int, const unsigned*, long,
                    long, int, hipStream_t);
+int lowrank_rp(int R);
+int lowrank_splits(const long* counts, int S, long T, int K);
+int lowrank_outer_shift(const long* counts, int S, long T, int NP);
+int lowrank_outer_tiles(const long* counts, int S, long T, int shift);
+void launch_shrink(int, int, const void*, long, const void*, int, int, const int*, const int*,
+                   const int*, const long*, int, int, long, const float*, float, void*, float*,
+                   hipStream_t);
+void launch_expand(int, int, const void*, long, void*, long, const void*, const void*, int, int,
+                   const int*, const int*, const int*, const long*, int, int, long, hipStream_t);
+void launch_outer(int, int, const void*, long, int, const void*, float*, const int*, const int*,
+                  const int*, const long*, int, int, long, int, void*, int, int, hipStream_t);
 }
 
 namespace {
@@ -219,6 +231,146 @@ Tensor adjust(Tensor logits, OptTensor history, OptTensor lengths, OptTensor pro
     return out;
 }
 
+// ------------------------------------------------------------------ low-rank adapters
+// Rows grouped by adapter (ops/adapters.py: AdapterRows), and what every launch takes of them.
+struct Grouped {
+    Tensor order, segs, adapter, scale;
+    std::vector<long> counts;
+    int S, Bn, L, K, M, R, type;
+    long T, N;
+    float scale_all;
+
+    Grouped(const Tensor& x, const Tensor& y, const Tensor& a, const Tensor& b, Tensor order_,
+            Tensor segs_, Tensor adapter_, std::vector<int64_t> counts_, const OptTensor& scale_,
+            double all)
+        : order(order_), segs(segs_), adapter(adapter_), counts(counts_.begin(), counts_.end()),
+          scale_all((float)all) {
+        TORCH_CHECK(x.is_cuda() && x.dim() == 2 && y.dim() == 2 && x.size(0) == y.size(0),
+                    "lowrank: x (N, K) and y (N, M) on GPU");
+        TORCH_CHECK(a.dim() == 3 && b.dim() == 3 && a.size(0) == b.size(0) &&
+                        a.size(2) == b.size(1) && a.size(1) == x.size(1) &&
+                        b.size(2) == y.size(1),
+                    "lowrank: a (L, K, R), b (L, R, M)");
+        TORCH_CHECK(a.is_contiguous() && b.is_contiguous(), "lowrank: a and b contiguous");
+        for (const Tensor* t : {&y, &a, &b}) {
+            check_on(*t, x, "lowrank: every tensor");
+            TORCH_CHECK(t->scalar_type() == x.scalar_type(), "lowrank: one type for all");
+        }
+        for (const Tensor* t : {&order, &segs, &adapter}) {
+            check_on(*t, x, "lowrank: the grouped rows");
+            TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous(), "lowrank: rows int32");
+        }
+        type = type_of(x, "x");
+        TORCH_CHECK(type != 2, "lowrank: bf16 or fp16");
+        L = (int)a.size(0);
+        K = (int)a.size(1);
+        R = (int)a.size(2);
+        M = (int)b.size(2);
+        N = x.size(0);
+        Bn = (int)order.numel();
+        S = (int)counts.size();
+        TORCH_CHECK(R >= 1 && R <= 128 && K >= 1 && M >= 1 && K < (1 << 30) && M < (1 << 30),
+                    "lowrank: a rank of 1 to 128");
+        TORCH_CHECK(segs.numel() == 4l * S && adapter.numel() == Bn && Bn > 0 && N % Bn == 0,
+                    "lowrank: N rows of Bn columns");
+        T = N / Bn;
+        long sum = 0;
+        for (long c : counts) sum += c;
+        TORCH_CHECK(sum == Bn && N < (1l << 31) && N / 64 * ((std::max(K, M) + 127) / 128) <
+                        (1l << 31), "lowrank: too many rows");
+        if (scale_.has_value()) {
+            TORCH_CHECK(scale_->numel() == L && scale_->dim() == 1, "lowrank: scale (L,)");
+            check_on(*scale_, x, "scale");
+            scale = scale_->to(at::kFloat).contiguous();
+        }
+    }
+    const int* ip(const Tensor& t) const { return (const int*)t.data_ptr(); }
+
+    // v (N, RP) = s x W, W (L, K, R) or, contraction contiguous, (L, R, K)
+    Tensor shrink(const Tensor& x, const Tensor& w, bool kcont, hipStream_t st) const {
+        const int k = (int)x.size(1), splits = lowrank_splits(counts.data(), S, T, k);
+        auto v = at::empty({N, (long)lowrank_rp(R)}, x.options());
+        Tensor part;
+        if (splits > 1)
+            part = at::empty({(long)splits * N * lowrank_rp(R)}, x.options().dtype(at::kFloat));
+        launch_shrink(type, kcont, x.data_ptr(), row_stride(x), w.data_ptr(), k, R, ip(order),
+                      ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
+                      v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, st);
+        check_launch("lowrank shrink");
+        return v;
+    }
+    // out = base + v W, W (L, R, M) or, rank contiguous, (L, M, R)
+    void expand(const Tensor& base, Tensor& out, const Tensor& v, const Tensor& w, bool rcont,
+                hipStream_t st) const {
+        launch_expand(type, rcont, base.defined() ? base.data_ptr() : nullptr,
+                      base.defined() ? row_stride(base) : 0, out.data_ptr(), row_stride(out),
+                      v.data_ptr(), w.data_ptr(), (int)out.size(1), R, ip(order), ip(segs),
+                      ip(adapter), counts.data(), S, Bn, T, st);
+        check_launch("lowrank expand");
+    }
+    // sum over an adapter's rows of p^T q: (L, R, NP) or, rank contiguous, (L, NP, R)
+    Tensor outer(const Tensor& p, const Tensor& q, bool rcont, hipStream_t st) const {
+        const int np = (int)p.size(1), shift = lowrank_outer_shift(counts.data(), S, T, np);
+        const long tiles = lowrank_outer_tiles(counts.data(), S, T, shift);
+        auto part = at::empty({tiles * lowrank_rp(R) * ((np + 127) / 128 * 128)},
+                              p.options().dtype(at::kFloat));
+        auto out = rcont ? at::empty({L, np, R}, p.options()) : at::empty({L, R, np}, p.options());
+        launch_outer(type, rcont, p.data_ptr(), row_stride(p), np, q.data_ptr(),
+                     (float*)part.data_ptr(), ip(order), ip(segs), ip(adapter), counts.data(), S,
+                     Bn, T, shift, out.data_ptr(), R, L, st);
+        check_launch("lowrank outer");
+        return out;
+    }
+};
+
+// -> (out, v); out is y itself where `inplace`
+std::vector<Tensor> lowrank_fwd(Tensor y, Tensor x, Tensor a, Tensor b, Tensor order, Tensor segs,
+                                Tensor adapter, std::vector<int64_t> counts, OptTensor scale,
+                                double scale_all, bool inplace) {
+    const c10::DeviceGuard guard(x.device());
+    const Grouped g(x, y, a, b, order, segs, adapter, counts, scale, scale_all);
+    const hipStream_t st = stream_of(x);
+    const Tensor xr = rows_of(x), yr = inplace ? y : rows_of(y);
+    TORCH_CHECK(yr.size(1) <= 1 || yr.stride(1) == 1, "lowrank: y's rows must be contiguous");
+    Tensor out = inplace ? y : at::empty({g.N, (long)g.M}, y.options());
+    Tensor v = g.shrink(xr, a, false, st);
+    g.expand(yr, out, v, b, false, st);
+    return {out, v};
+}
+
+std::vector<OptTensor> lowrank_bwd(Tensor dy, Tensor x, Tensor a, Tensor b, Tensor v, Tensor order,
+                                   Tensor segs, Tensor adapter, std::vector<int64_t> counts,
+                                   OptTensor scale, double scale_all, OptTensor base_dx,
+                                   bool need_x, bool need_a, bool need_b) {
+    const c10::DeviceGuard guard(x.device());
+    const Grouped g(x, dy, a, b, order, segs, adapter, counts, scale, scale_all);
+    const hipStream_t st = stream_of(x);
+    TORCH_CHECK(v.dim() == 2 && v.size(0) == g.N && v.size(1) == lowrank_rp(g.R) &&
+                    v.is_contiguous() && v.scalar_type() == x.scalar_type(),
+                "lowrank_bwd: v as lowrank_fwd returned it");
+    check_on(v, x, "v");
+    const Tensor xr = rows_of(x), dr = rows_of(dy);
+    OptTensor dx, da, db;
+    if (need_x || need_a) {
+        const Tensor u = g.shrink(dr, b, true, st);
+        if (need_x) {
+            Tensor base;
+            if (base_dx.has_value()) {
+                TORCH_CHECK(base_dx->sizes() == x.sizes() &&
+                                base_dx->scalar_type() == x.scalar_type(), "lowrank_bwd: base_dx");
+                check_on(*base_dx, x, "base_dx");
+                base = rows_of(*base_dx);
+            }
+            Tensor out = at::empty({g.N, (long)g.K}, x.options());
+            g.expand(base, out, u, a, true, st);
+            dx = out;
+        }
+        if (need_a) da = g.outer(xr, u, true, st);
+    }
+    if (need_b) db = g.outer(dr, v, false, st);
+    return {dx, da, db};
+}
+
 }  // namespace
 
 void register_lm_ops(pybind11::module_& m) {
@@ -234,4 +386,13 @@ void register_lm_ops(pybind11::module_& m) {
           py::arg("repetition"), py::arg("repetition_all"), py::arg("presence"),
           py::arg("presence_all"), py::arg("frequency"), py::arg("frequency_all"),
           py::arg("bias_index"), py::arg("bias"), py::arg("allowed"));
+    m.def("lowrank_fwd", &lowrank_fwd, "y + s x A B by rows' adapters", py::arg("y"),
+          py::arg("x"), py::arg("a"), py::arg("b"), py::arg("order"), py::arg("segs"),
+          py::arg("adapter"), py::arg("counts"), py::arg("scale") = py::none(),
+          py::arg("scale_all") = 1.0, py::arg("inplace") = false);
+    m.def("lowrank_bwd", &lowrank_bwd, "gradients of lowrank_fwd", py::arg("dy"), py::arg("x"),
+          py::arg("a"), py::arg("b"), py::arg("v"), py::arg("order"), py::arg("segs"),
+          py::arg("adapter"), py::arg("counts"), py::arg("scale") = py::none(),
+          py::arg("scale_all") = 1.0, py::arg("base_dx") = py::none(), py::arg("need_x") = true,
+          py::arg("need_a") = true, py::arg("need_b") = true);
 }
