@@ -340,8 +340,8 @@ std::vector<Tensor> lowrank_fwd(Tensor y, Tensor x, Tensor a, Tensor b, Tensor o
 
 std::vector<OptTensor> lowrank_bwd(Tensor dy, Tensor x, Tensor a, Tensor b, Tensor v, Tensor order,
                                    Tensor segs, Tensor adapter, std::vector<int64_t> counts,
-                                   OptTensor scale, double scale_all, OptTensor base_dx,
-                                   bool need_x, bool need_a, bool need_b) {
+                                   OptTensor scale, double scale_all, bool need_x, bool need_a,
+                                   bool need_b) {
     const c10::DeviceGuard guard(x.device());
     const Grouped g(x, dy, a, b, order, segs, adapter, counts, scale, scale_all);
     const hipStream_t st = stream_of(x);
@@ -354,15 +354,8 @@ std::vector<OptTensor> lowrank_bwd(Tensor dy, Tensor x, Tensor a, Tensor b, Tens
     if (need_x || need_a) {
         const Tensor u = g.shrink(dr, b, true, st);
         if (need_x) {
-            Tensor base;
-            if (base_dx.has_value()) {
-                TORCH_CHECK(base_dx->sizes() == x.sizes() &&
-                                base_dx->scalar_type() == x.scalar_type(), "lowrank_bwd: base_dx");
-                check_on(*base_dx, x, "base_dx");
-                base = rows_of(*base_dx);
-            }
             Tensor out = at::empty({g.N, (long)g.K}, x.options());
-            g.expand(base, out, u, a, true, st);
+            g.expand(Tensor(), out, u, a, true, st);
             dx = out;
         }
         if (need_a) da = g.outer(xr, u, true, st);
@@ -393,6 +386,6 @@ void register_lm_ops(pybind11::module_& m) {
     m.def("lowrank_bwd", &lowrank_bwd, "gradients of lowrank_fwd", py::arg("dy"), py::arg("x"),
           py::arg("a"), py::arg("b"), py::arg("v"), py::arg("order"), py::arg("segs"),
           py::arg("adapter"), py::arg("counts"), py::arg("scale") = py::none(),
-          py::arg("scale_all") = 1.0, py::arg("base_dx") = py::none(), py::arg("need_x") = true,
-          py::arg("need_a") = true, py::arg("need_b") = true);
+          py::arg("scale_all") = 1.0, py::arg("need_x") = true, py::arg("need_a") = true,
+          py::arg("need_b") = true);
 }

@@ -67,6 +67,11 @@ class TrainConfig:
     # measure split-vs-fused recurrent path for THIS shape at init instead
     # of the built-in heuristic (ops/autotune.py)
     autotune: bool = False
+    # distillation (Trainer(..., teacher=model)): weight of the teacher's
+    # top logits against the labels, their temperature and their number
+    distill_alpha: float = 0.5
+    distill_temperature: float = 2.0
+    distill_top_k: int = 64
     # fault injection (failure-detection tests): raise on this rank at this
     # step; -1 = disabled
     fault_step: int = -1

@@ -29,6 +29,8 @@ import torch.nn.functional as F
 from ..config import ModelConfig
 from ..ops.lstm_layer import lstm_layer
 from ..ops import xent
+from ..ops.distill import distill_loss
+from ..ops.logits import LogitRules, RowRules
 
 
 def _pname(layer: int, rev: bool, which: str) -> str:
@@ -171,7 +173,7 @@ class LSTMModel(nn.Module):
                 p.copy_(src)
 
     # -- forward -----------------------------------------------------------
-    def _layer_io(self, x, layer: int, rev: bool, state=None):
+    def _layer_io(self, x, layer: int, rev: bool, state=None, adapters=None):
         B = x.shape[1]
         H = self.cfg.hidden_size
         w_x = self.weight(_pname(layer, rev, "W_x"))
@@ -193,15 +195,21 @@ class LSTMModel(nn.Module):
             h0, c0 = zs
         else:
             h0, c0 = state
-        return lstm_layer(x, h0, c0, w_x, w_h, b, reverse=rev)
+        add = None
+        if adapters is not None:
+            site = f"layer{layer}{'_rev' if rev else ''}"
+            add = lambda pre, x: adapters.add(pre, x, site)  # noqa: E731
+        return lstm_layer(x, h0, c0, w_x, w_h, b, reverse=rev, add=add)
 
-    def backbone(self, x: torch.Tensor, state: Optional[list] = None):
+    def backbone(self, x: torch.Tensor, state: Optional[list] = None,
+                 adapters=None):
         """Run embedding (if LM) + all LSTM layers.
 
         x: (T,B,input_size) features, or (T,B) long tokens for LM
            (TIME-MAJOR -- the engine's native layout, see ops/functional.py).
         state: per-(layer,dir) list of (h0, c0) carry (truncated BPTT), or
                None for zero state.
+        adapters: AdapterSet.rows(...) of the batch's columns, or None.
         Returns (features (T,B,H*D), new_state list).
         """
         cfg = self.cfg
@@ -223,9 +231,11 @@ class LSTMModel(nn.Module):
                 st = state[si + 1] if state is not None else None
                 with torch.cuda.stream(s2):
                     x.record_stream(s2)
-                    h_rev, hT_r, cT_r = self._layer_io(x, l, True, st)
+                    h_rev, hT_r, cT_r = self._layer_io(x, l, True, st,
+                                                     adapters)
                 st = state[si] if state is not None else None
-                h_fwd, hT_f, cT_f = self._layer_io(x, l, False, st)
+                h_fwd, hT_f, cT_f = self._layer_io(x, l, False, st,
+                                                 adapters)
                 cur.wait_stream(s2)            # before the concat reads
                 new_state += [(hT_f, cT_f), (hT_r, cT_r)]
                 si += 2
@@ -234,7 +244,7 @@ class LSTMModel(nn.Module):
                 outs = []
                 for rev in ([False, True] if cfg.bidirectional else [False]):
                     st = state[si] if state is not None else None
-                    h_seq, hT, cT = self._layer_io(x, l, rev, st)
+                    h_seq, hT, cT = self._layer_io(x, l, rev, st, adapters)
                     outs.append(h_seq)
                     new_state.append((hT, cT))
                     si += 1
@@ -243,19 +253,22 @@ class LSTMModel(nn.Module):
                 x = F.dropout(x, p=cfg.dropout)
         return x, new_state
 
-    def forward(self, x, state: Optional[list] = None):
+    def forward(self, x, state: Optional[list] = None, adapters=None):
         """Returns (output, new_state).
 
         output: logits -- (B,C) for "classifier", (T,B,C) for
         "seq_classifier", (T,B,V) for "lm", features (T,B,H*D) for "none".
         """
-        feats, new_state = self.backbone(x, state)
+        feats, new_state = self.backbone(x, state, adapters)
         cfg = self.cfg
         if cfg.head == "none":
             return feats, new_state
         w, b = self.weight("head/W"), self.weight("head/b")
         if cfg.head == "classifier":
-            return torch.addmm(b, feats[-1], w), new_state
+            out = torch.addmm(b, feats[-1], w)
+            if adapters is not None:
+                out = adapters.add(out, feats[-1], "head")
+            return out, new_state
         T, B, F_ = feats.shape
         flat = feats.reshape(T * B, F_)
         if (cfg.head == "lm" and feats.is_cuda
@@ -265,6 +278,8 @@ class LSTMModel(nn.Module):
             logits = _Fp8HeadFn.apply(flat, w, b).view(T, B, -1)
         else:
             logits = torch.addmm(b, flat, w).view(T, B, -1)
+        if adapters is not None:
+            logits = adapters.add(logits, feats, "head")
         return logits, new_state
 
     @staticmethod
@@ -289,6 +304,24 @@ class LSTMModel(nn.Module):
         # regression on features
         return F.mse_loss(output.float(), y.float())
 
+    def distill_loss(self, output: torch.Tensor, teacher: torch.Tensor,
+                     y: Optional[torch.Tensor], top_k: int = 64,
+                     alpha: float = 0.5,
+                     temperature: float = 2.0) -> torch.Tensor:
+        """Loss against a teacher's logits (same shape as `output`): its
+        top_k of every position at `temperature`, weighed by alpha against
+        the labels y (ops/distill.py)."""
+        if self.cfg.head == "none":
+            raise ValueError("distillation needs a head with logits")
+        if teacher.shape != output.shape:
+            raise ValueError(f"teacher's logits {tuple(teacher.shape)} and "
+                             f"the model's {tuple(output.shape)} differ")
+        C = output.shape[-1]
+        top = teacher.detach().reshape(-1, C).topk(min(top_k, C), dim=1)
+        return distill_loss(output.reshape(-1, C), top.indices, top.values,
+                            None if y is None else y.reshape(-1),
+                            alpha=alpha, temperature=temperature)
+
     def detach_state(self, state):
         """Detach the (h, c) carry for truncated BPTT."""
         if state is None:
@@ -302,7 +335,9 @@ class LSTMModel(nn.Module):
                  use_graph: Optional[bool] = None,
                  use_gemv: Optional[bool] = None,
                  top_k: int = 0, top_p: float = 0.0,
-                 eos_token: int = -1) -> torch.Tensor:
+                 eos_token: int = -1,
+                 rules: "Optional[LogitRules]" = None,
+                 adapters=None) -> torch.Tensor:
         """Autoregressive decode for the LM head (the serving path).
 
         prompt: (Tp, B) long tokens (time-major).  Returns (Tp+steps, B):
@@ -314,6 +349,9 @@ class LSTMModel(nn.Module):
         eos_token >= 0 stops a sequence at that token (a finished column
         keeps emitting eos); decode ends early once EVERY column is done
         (eager path only -- the graphed decode runs fixed steps).
+        rules: penalties, biases and a grammar for every column
+        (ops/logits.py); adapters: AdapterSet.rows(...) of the B columns
+        (both on the eager path only).
 
         use_graph (default: auto = greedy + CUDA + steps >= 16): capture
         ONE decode step as a hipGraph whose body copies its outputs back
@@ -328,27 +366,51 @@ class LSTMModel(nn.Module):
         self.eval()
         if use_graph is None:
             use_graph = (temperature <= 0 and prompt.is_cuda and steps >= 16
-                         and eos_token < 0)
+                         and eos_token < 0 and rules is None
+                         and adapters is None)
         assert not (use_graph and temperature > 0), \
             "the graphed decode step is greedy-only"
         assert not (use_graph and eos_token >= 0), \
             "eos early-stop needs the eager path (use_graph=False)"
+        assert not (use_graph and (rules is not None
+                                   or adapters is not None)), \
+            "rules and adapters need the eager path (use_graph=False)"
+        Tp, B = prompt.shape
+        if rules is not None:
+            rules.check(self.cfg.vocab_size)
+            every = RowRules([rules] * B, [Tp] * B, self.cfg.vocab_size,
+                             prompt.device)
+            seen = torch.zeros(B, Tp + max(steps, 1), dtype=torch.long,
+                               device=prompt.device)
+            seen[:, :Tp] = prompt.t()
+
+        def ruled(logits, length):
+            if rules is None:
+                return logits
+            past = seen[:, :length]
+            allowed = [rules.allows(t, logits.shape[1])
+                       for t in past.tolist()] if rules.grammar else ()
+            return every.apply(logits, past, None, allowed)
+
         try:
-            out, state = self.forward(prompt)          # (Tp, B, V)
-            cur = self._sample(out[-1], temperature, generator, top_k, top_p)
+            out, state = self.forward(prompt, None, adapters)  # (Tp, B, V)
+            cur = self._sample(ruled(out[-1], Tp), temperature, generator,
+                               top_k, top_p)
             if use_graph:
                 return torch.cat(
                     [prompt, self._graph_decode(cur, state, steps, use_gemv)],
                     dim=0)
             toks = [prompt]
             done = (cur == eos_token) if eos_token >= 0 else None
-            for _ in range(steps - 1):
+            for i in range(steps - 1):
                 toks.append(cur.unsqueeze(0))
                 if done is not None and bool(done.all()):
                     break
-                out, state = self.forward(cur.unsqueeze(0), state)
-                cur = self._sample(out[-1], temperature, generator,
-                                   top_k, top_p)
+                if rules is not None:
+                    seen[:, Tp + i] = cur
+                out, state = self.forward(cur.unsqueeze(0), state, adapters)
+                cur = self._sample(ruled(out[-1], Tp + i + 1), temperature,
+                                   generator, top_k, top_p)
                 if done is not None:
                     cur = torch.where(done, torch.full_like(cur, eos_token),
                                       cur)

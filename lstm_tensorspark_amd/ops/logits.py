@@ -16,8 +16,9 @@ the kernel on the GPU, the CPU and fp64 the reference below.
 """
 from __future__ import annotations
 
+import dataclasses
 import math
-from typing import Optional, Union
+from typing import Callable, Dict, List, Optional, Sequence, Union
 
 import torch
 
@@ -161,3 +162,101 @@ def adjust_logits(logits: torch.Tensor,
                        pres_all if pres is None else pres,
                        freq_all if freq is None else freq, bias_index, bias,
                        allowed)
+
+
+@dataclasses.dataclass
+class LogitRules:
+    """What one request wants done to its logits before a token is chosen.
+
+    bias: token -> what is added to its logit.
+    grammar: called with the request's tokens so far (prompt included) before
+    every token; returns the tokens that may follow as a (V,) bool tensor, on
+    any device.
+    """
+    repetition: float = 1.0
+    presence: float = 0.0
+    frequency: float = 0.0
+    bias: Optional[Dict[int, float]] = None
+    grammar: Optional[Callable[[List[int]], torch.Tensor]] = None
+
+    def check(self, vocab_size: int):
+        """Refuses what could leave a row without a finite logit to sample
+        from: the limits keep every adjusted logit of a bf16 model finite."""
+        if not 0.01 <= self.repetition <= 100.0:
+            raise ValueError("repetition must be in [0.01, 100], got "
+                             f"{self.repetition}")
+        for x in (self.presence, self.frequency):
+            if not abs(x) <= 1e4:
+                raise ValueError(f"penalties must be in [-1e4, 1e4], got {x}")
+        bias = self.bias or {}
+        if any(t < 0 or t >= vocab_size for t in bias):
+            raise ValueError(f"bias tokens must be in [0, {vocab_size})")
+        if not all(f == -math.inf or abs(f) <= 1e4 for f in bias.values()):
+            raise ValueError("a bias must be in [-1e4, 1e4] or -inf")
+        if sum(f == -math.inf for f in bias.values()) == vocab_size:
+            raise ValueError("the biases rule out every token")
+
+    @property
+    def penalizes(self) -> bool:
+        return (self.repetition != 1.0 or self.presence != 0.0
+                or self.frequency != 0.0)
+
+    def allows(self, tokens: List[int], vocab_size: int) -> torch.Tensor:
+        """The grammar's answer as a (V,) bool tensor, with a token in it
+        that no bias rules out."""
+        ok = self.grammar(tokens)
+        if (not isinstance(ok, torch.Tensor) or ok.dtype != torch.bool
+                or ok.shape != (vocab_size,)):
+            raise ValueError(f"a grammar returns a ({vocab_size},) bool tensor")
+        banned = [t for t, f in (self.bias or {}).items() if f == -math.inf]
+        if banned:
+            ok = ok.clone()
+            ok[banned] = False
+        if not bool(ok.any()):
+            raise ValueError(f"the grammar allows no token after {len(tokens)}")
+        return ok
+
+
+class RowRules:
+    """The rules (or None) of a batch's rows, for as long as the batch stays
+    the same: what does not change from token to token is uploaded once."""
+
+    def __init__(self, rules: Sequence[Optional[LogitRules]],
+                 prompt_lengths: Sequence[int], vocab_size: int, device):
+        self.rules = [r or LogitRules() for r in rules]
+        self.vocab_size, self.device = vocab_size, device
+        self.penalizes = any(r.penalizes for r in self.rules)
+        self.constant: dict = {}
+        if self.penalizes:
+            number = torch.tensor(
+                [[getattr(r, n) for r in self.rules]
+                 for n in ("repetition", "presence", "frequency")],
+                dtype=torch.float32).to(device)
+            self.constant.update(
+                repetition=number[0], presence=number[1], frequency=number[2],
+                prompt_lengths=torch.tensor(list(prompt_lengths)).to(device))
+        K = max(len(r.bias or ()) for r in self.rules)
+        if K:
+            pairs = [list((r.bias or {}).items()) for r in self.rules]
+            pairs = [p + [(-1, 0.0)] * (K - len(p)) for p in pairs]
+            self.constant["bias_index"] = torch.tensor(
+                [[t for t, _ in p] for p in pairs]).to(device)
+            self.constant["bias"] = torch.tensor(
+                [[f for _, f in p] for p in pairs],
+                dtype=torch.float32).to(device)
+
+    def apply(self, logits: torch.Tensor, history: Optional[torch.Tensor],
+              lengths: Optional[torch.Tensor],
+              allowed: Sequence[Optional[torch.Tensor]] = ()) -> torch.Tensor:
+        """`adjust_logits` on the rows' (B, V) logits.  history (B, L) and
+        lengths (B,) are needed where a row penalizes; allowed: what the
+        grammars (LogitRules.allows) said for each row, None without one."""
+        args = dict(self.constant)
+        if self.penalizes:
+            args.update(history=history, lengths=lengths)
+        if any(ok is not None for ok in allowed):
+            every = torch.ones(self.vocab_size, dtype=torch.bool)
+            args["allowed"] = pack_allowed(torch.stack(
+                [(every if ok is None else ok).to(self.device)
+                 for ok in allowed]))
+        return adjust_logits(logits, **args) if args else logits

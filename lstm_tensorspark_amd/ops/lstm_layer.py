@@ -275,6 +275,38 @@ class LSTMLayerFn(torch.autograd.Function):
         return dx, dh0, dc0, dw_x, dw_h, db, None
 
 
+class LSTMRecurrentFn(torch.autograd.Function):
+    """The time loop alone, from gates that the caller projected: the layer
+    as `LSTMLayerFn` runs it where something is added to the projection
+    (low-rank adapters), whose gradients autograd then takes from dpre."""
+
+    @staticmethod
+    def forward(ctx, pre, h0, c0, w_h, reverse: bool):
+        ctx.set_materialize_grads(False)
+        use_hip = extension.use_hip(pre.device, pre.dtype)
+        h_all, c_seq, acts, hT, cT = _seq_fwd(pre, w_h, h0, c0, reverse,
+                                              use_hip)
+        ctx.save_for_backward(c0, w_h, h_all, c_seq, acts)
+        ctx.reverse, ctx.use_hip = reverse, use_hip
+        return h_seq_view(h_all, reverse), hT, cT
+
+    @staticmethod
+    def backward(ctx, d_hseq, d_hT, d_cT):
+        c0, w_h, h_all, c_seq, acts = ctx.saved_tensors
+        dgates, dh0, dc0, _ = _seq_bwd(
+            d_hseq.contiguous() if d_hseq is not None else None,
+            d_hT.contiguous() if d_hT is not None else None,
+            d_cT.contiguous() if d_cT is not None else None,
+            w_h, acts, c_seq, c0, ctx.reverse, ctx.use_hip,
+        )
+        dw_h = None
+        if ctx.needs_input_grad[3]:
+            H = w_h.shape[0]
+            hprev = h_prev_view(h_all, ctx.reverse).reshape(-1, H)
+            dw_h = (hprev.t() @ dgates.reshape(-1, 4 * H)).to(w_h.dtype)
+        return dgates, dh0, dc0, dw_h, None
+
+
 def lstm_layer(
     x: torch.Tensor,
     h0: torch.Tensor,
@@ -283,9 +315,17 @@ def lstm_layer(
     w_h: torch.Tensor,
     b: torch.Tensor,
     reverse: bool = False,
+    add=None,
 ):
     """Run one LSTM layer (one direction) over (T,B,X) -> (T,B,H).
 
+    add: what is added to the input projection, a function (pre, x) -> pre
+    (models/adapters.py); None for the plain layer.
     Returns (h_seq, hT, cT); cT is fp32.
     """
+    if add is not None:
+        T, B, X = x.shape
+        pre = torch.addmm(b.to(x.dtype), x.reshape(T * B, X), w_x)
+        pre = add(pre.view(T, B, -1), x)
+        return LSTMRecurrentFn.apply(pre, h0, c0, w_h, reverse)
     return LSTMLayerFn.apply(x, h0, c0, w_x, w_h, b, reverse)

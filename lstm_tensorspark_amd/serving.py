@@ -36,14 +36,17 @@ from typing import Dict, List, Optional
 
 import torch
 
+from .ops.logits import LogitRules, RowRules
+
 
 class _Slot:
     __slots__ = ("rid", "tokens", "remaining", "prompt_len", "eos",
-                 "temperature", "top_k", "top_p", "gen")
+                 "temperature", "top_k", "top_p", "gen", "rules", "adapter",
+                 "error")
 
     def __init__(self, rid: int, tokens: List[int], remaining: int,
                  eos: int = -1, temperature: float = 0.0, top_k: int = 0,
-                 top_p: float = 0.0, gen=None):
+                 top_p: float = 0.0, gen=None, rules=None, adapter: int = -1):
         self.rid = rid
         self.tokens = list(tokens)
         self.prompt_len = len(tokens)
@@ -53,9 +56,12 @@ class _Slot:
         self.top_k = top_k
         self.top_p = top_p
         self.gen = gen
+        self.rules = rules
+        self.adapter = adapter
+        self.error: Optional[Exception] = None
 
     def finished(self) -> bool:
-        return (self.remaining <= 0
+        return (self.remaining <= 0 or self.error is not None
                 or (self.eos >= 0 and self.tokens[-1] == self.eos))
 
 
@@ -72,7 +78,9 @@ class ContinuousBatcher:
     are safe from any number of request threads.
     """
 
-    def __init__(self, model, max_batch: int = 64, max_steps: int = 4096):
+    def __init__(self, model, max_batch: int = 64, max_steps: int = 4096,
+                 adapters=None):
+        """adapters: an AdapterSet of the model, which requests pick one of."""
         assert model.cfg.head == "lm", "serving engine requires the LM head"
         assert not model.cfg.bidirectional, "decode is causal: fwd-only"
         self.model = model
@@ -90,24 +98,39 @@ class ContinuousBatcher:
         self._decode_steps = 0      # batched decode steps executed
         self._slot_steps = 0        # sum of active slots over those steps
         self._cancelled: set = set()  # rids retired by cancel()
+        self.adapters = adapters
+        # of the live slots, made anew when one joins or leaves
+        self._bound = None          # their adapters
+        self._rules = None          # their rules
+        self._history = None        # (B, longest) tokens, for penalties
 
     # ------------------------------------------------------------ requests
     def submit(self, tokens: List[int], steps: int,
                eos_token: int = -1, temperature: float = 0.0,
                top_k: int = 0, top_p: float = 0.0,
-               seed: Optional[int] = None) -> int:
+               seed: Optional[int] = None,
+               rules: Optional[LogitRules] = None, adapter: int = -1) -> int:
         """eos_token >= 0: the request finishes early when it emits that
         token (same semantics as model.generate(eos_token=...)).
 
         temperature > 0 samples with this request's OWN generator (seeded
         with `seed` when given), so a sampled request is reproducible and
         token-identical to a solo model.generate() with the same seed --
-        regardless of what else shares the batch."""
+        regardless of what else shares the batch.
+
+        rules: this request's penalties, biases and grammar; a grammar that
+        raises or allows nothing ends the request, and result() raises what
+        it raised.  adapter: one of the engine's AdapterSet, -1 for none."""
         V = self.model.cfg.vocab_size
         if not tokens or any(t < 0 or t >= V for t in tokens):
             raise ValueError(f"tokens must be in [0, {V})")
         if steps < 1 or steps > self.max_steps:
             raise ValueError(f"steps must be in [1, {self.max_steps}]")
+        if rules is not None:
+            rules.check(V)
+        count = self.adapters.count if self.adapters is not None else 0
+        if adapter < -1 or adapter >= count:
+            raise ValueError(f"adapter must be in [-1, {count})")
         gen = None
         if temperature > 0 and seed is not None:
             gen = torch.Generator(device=self.device)
@@ -115,7 +138,8 @@ class ContinuousBatcher:
         with self._cv:
             rid = next(self._ids)
             self._queue.append(_Slot(rid, tokens, steps, eos_token,
-                                     temperature, top_k, top_p, gen))
+                                     temperature, top_k, top_p, gen, rules,
+                                     adapter))
             self._cv.notify_all()
         return rid
 
@@ -124,7 +148,7 @@ class ContinuousBatcher:
         polling primitive for streaming responses."""
         with self._cv:
             if rid in self._results:
-                return list(self._results[rid]), True
+                return list(self._claimed(self._results[rid])), True
             for s in self._slots:
                 if s.rid == rid:
                     return list(s.tokens), False
@@ -151,9 +175,15 @@ class ContinuousBatcher:
                     return True
             return self._results.pop(rid, None) is not None
 
+    @staticmethod
+    def _claimed(result):
+        if isinstance(result, Exception):
+            raise result
+        return result
+
     def try_result(self, rid: int) -> Optional[List[int]]:
         with self._cv:
-            return self._results.pop(rid, None)
+            return self._claimed(self._results.pop(rid, None))
 
     def result(self, rid: int, timeout: Optional[float] = None) -> List[int]:
         """Block until request `rid` finishes (engine thread must be
@@ -163,7 +193,7 @@ class ContinuousBatcher:
                                    timeout=timeout)
             if not ok:
                 raise TimeoutError(f"request {rid} not done in {timeout}s")
-            return self._results.pop(rid)
+            return self._claimed(self._results.pop(rid))
 
     def stats(self) -> dict:
         with self._cv:
@@ -183,10 +213,18 @@ class ContinuousBatcher:
             slot = self._queue.popleft()
             prompt = torch.tensor(slot.tokens, dtype=torch.long,
                                   device=self.device).unsqueeze(1)
-            out, st = m.forward(prompt)              # (Tp, 1, V)
-            tok = int(self._pick(out[-1], slot)[0])
-            slot.tokens.append(tok)
-            slot.remaining -= 1
+            own = None if slot.adapter < 0 else \
+                self.adapters.rows([slot.adapter])
+            out, st = m.forward(prompt, None, own)   # (Tp, 1, V)
+            logits = out[-1]
+            if slot.rules is not None:
+                logits = self._row_rules([slot]).apply(
+                    logits, prompt.t(), None, self._allowed([slot]))
+            if slot.error is None:
+                tok = int(self._pick(logits, slot)[0])
+                slot.tokens.append(tok)
+                slot.remaining -= 1
+            self._bound = self._rules = self._history = None
             if self._state is None or not self._slots:
                 self._state = [(h, c) for h, c in st]
             else:
@@ -206,16 +244,61 @@ class ContinuousBatcher:
         m = self.model
         x = torch.tensor([[s.tokens[-1] for s in self._slots]],
                          dtype=torch.long, device=self.device)  # (1, B)
-        out, self._state = m.forward(x, self._state)            # (1, B, V)
-        logits = out[0]                                         # (B, V)
+        if self.adapters is not None and self._bound is None and \
+                any(s.adapter >= 0 for s in self._slots):
+            self._bound = self.adapters.rows([s.adapter for s in self._slots])
+        out, self._state = m.forward(x, self._state, self._bound)  # (1, B, V)
+        logits = self._ruled(out[0], x)                         # (B, V)
         greedy = logits.argmax(dim=-1)                          # (B,)
         for i, s in enumerate(self._slots):
+            if s.error is not None:
+                continue
             if s.temperature > 0:
                 s.tokens.append(int(self._pick(logits[i:i + 1], s)[0]))
             else:
                 s.tokens.append(int(greedy[i]))
             s.remaining -= 1
         self._retire_locked()
+
+    def _row_rules(self, slots) -> RowRules:
+        return RowRules([s.rules for s in slots],
+                        [s.prompt_len for s in slots],
+                        self.model.cfg.vocab_size, self.device)
+
+    def _allowed(self, slots) -> list:
+        """What the slots' grammars allow next; one that fails ends its
+        request."""
+        allowed: list = [None] * len(slots)
+        for i, s in enumerate(slots):
+            if s.rules is not None and s.rules.grammar:
+                try:
+                    allowed[i] = s.rules.allows(list(s.tokens),
+                                                self.model.cfg.vocab_size)
+                except Exception as e:
+                    s.error = e
+        return allowed
+
+    def _ruled(self, logits, x):
+        """The live slots' rules on their (B, V) logits.  Their history stays
+        on the device: a step adds the tokens x (1, B) that it feeds."""
+        if all(s.rules is None for s in self._slots):
+            return logits
+        if self._rules is None:
+            self._rules = self._row_rules(self._slots)
+        lengths = None
+        if self._rules.penalizes:
+            size = [len(s.tokens) for s in self._slots]
+            lengths = torch.tensor(size).to(self.device)
+            if self._history is None:
+                room = max(n + s.remaining
+                           for n, s in zip(size, self._slots))
+                self._history = torch.tensor(
+                    [s.tokens + [-1] * (room - n)
+                     for n, s in zip(size, self._slots)]).to(self.device)
+            else:
+                self._history.scatter_(1, (lengths - 1).unsqueeze(1), x.t())
+        return self._rules.apply(logits, self._history, lengths,
+                                 self._allowed(self._slots))
 
     def _pick(self, logits, slot: _Slot):
         """Next token for one slot from its (1, V) logits row -- the same
@@ -229,12 +312,14 @@ class ContinuousBatcher:
             (done if s.finished() else keep).append(i)
         if not done:
             return
+        self._bound = self._rules = self._history = None
         for i in done:
             s = self._slots[i]
             if s.rid in self._cancelled:
                 self._cancelled.discard(s.rid)   # drop, don't store
             else:
-                self._results[s.rid] = s.tokens
+                self._results[s.rid] = s.tokens if s.error is None \
+                    else s.error
         if keep:
             idx = torch.tensor(keep, device=self.device)
             self._state = [(h.index_select(0, idx), c.index_select(0, idx))

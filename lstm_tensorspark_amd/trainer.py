@@ -50,7 +50,10 @@ def compute_dtype(cfg: Config, device: torch.device) -> torch.dtype:
 
 class Trainer:
     def __init__(self, cfg: Config, model: Optional[LSTMModel] = None,
-                 dist_ctx: Optional[DistContext] = None, device=None):
+                 dist_ctx: Optional[DistContext] = None, device=None,
+                 teacher: Optional[LSTMModel] = None):
+        """teacher: a model of the same head size to distil from; the step
+        then learns its top logits beside the labels (train.distill_*)."""
         self.cfg = cfg
         self.ctx = dist_ctx or DistContext()
         self.device = torch.device(device) if device is not None else self.ctx.device
@@ -62,6 +65,14 @@ class Trainer:
         self.model = self.model.to(self.device)
         if self.dtype != torch.float32:
             self.model = self.model.to(self.dtype)
+        self.teacher = teacher
+        if teacher is not None:
+            t, own = teacher.cfg, self.model.cfg
+            if own.head == "none" or t.head != own.head or (
+                    t.vocab_size if t.head == "lm" else t.num_classes) != (
+                    own.vocab_size if own.head == "lm" else own.num_classes):
+                raise ValueError("teacher and model must have the same head")
+            self.teacher = teacher.to(self.device, self.dtype).eval()
         broadcast_parameters(self.model)  # belt-and-braces weight sync at init
         if self.ctx.world_size > 1 and self.ctx.rank > 0:
             # init above must be seed-identical on every rank, but the
@@ -122,7 +133,7 @@ class Trainer:
             # lr is baked into the captured kernels; accumulation needs
             # multiple backwards per step -- both fall back to eager
             and no_accum and not cfg.train.lr_schedule
-            and cfg.train.warmup_steps <= 0)
+            and cfg.train.warmup_steps <= 0 and teacher is None)
 
     # ------------------------------------------------------------------
     def _bptt_windows(self, x, y):
@@ -186,11 +197,19 @@ class Trainer:
         n_micro = len(batches)
         for bi, (x, y) in enumerate(batches):
             wins = self._bptt_windows(x, y)
-            state = None
+            state = t_state = None
             for wi, (wx, wy) in enumerate(wins):
                 out, state = self.model(wx, state)
                 state = self.model.detach_state(state)
-                loss = self.model.loss(out, wy)
+                if self.teacher is not None:
+                    with torch.no_grad():
+                        t_out, t_state = self.teacher(wx, t_state)
+                    loss = self.model.distill_loss(
+                        out, t_out, wy, cfg.train.distill_top_k,
+                        cfg.train.distill_alpha,
+                        cfg.train.distill_temperature)
+                else:
+                    loss = self.model.loss(out, wy)
                 scale = len(wins) * n_micro
                 if scale > 1:
                     loss = loss / scale
