@@ -49,6 +49,24 @@ template <typename T> DEVINL typename Frag<T>::type load_frag(const T* p, int le
     return v;
 }
 
+// An operand whose contraction runs down the rows of an LDS tile: column c (lane & 15) of rows
+// k0 + (lane >> 4) * 8 + [0, 8).  The hardware's transposing read takes 4 rows x 16 columns a
+// group of 16 lanes: lane L names row L >> 2 and four columns, lane i receives column i's four.
+// `c` is the address of that lane's four columns; tile rows are multiples of 8 bytes.
+template <typename T> DEVINL typename Frag<T>::type column_frag(const T* tile, int ld, int k0,
+                                                                int c) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s4 lds4;
+    const int lane = threadIdx.x & 63;
+    const T* p = tile + (k0 + (lane >> 4) * 8 + ((lane & 15) >> 2)) * ld + c;
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * ld));
+    return __builtin_bit_cast(typename Frag<T>::type,
+                              __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+DEVINL int own_columns() { return (threadIdx.x & 3) * 4; }     // of a lane, in 16 neighbours
+
 struct Rows {
     const int* order;       // (Bn,) columns, grouped by adapter
     const int4* segs;       // (S,) adapter (-1: none), start, count, 0
@@ -109,8 +127,9 @@ DEVINL long row_of(const Rows& r, const Tile& f, long j) {
 
 // ---------------------------------------------------------------------------
 // shrink: V[row] = s_l X[row] W_l.  A workgroup takes 128 rows of one adapter and `kper` of the
-// contraction; its four waves hold 32 rows each and share W's 128-step panel, which lies in LDS
-// with the contraction contiguous (transposed on the way in where W is (K, R)).
+// contraction; its four waves hold 32 rows each, straight from memory in the operand's layout,
+// and share W's 128-step panel in LDS.  The next step's rows and panel are on their way while
+// this one is multiplied.
 // ---------------------------------------------------------------------------
 constexpr int S_TM = 7;     // log2 rows a workgroup
 constexpr int S_KC = 128;   // contraction a step
@@ -122,8 +141,9 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
                                                 float* __restrict__ part, long N, int splits,
                                                 int kper) {
     typedef typename Frag<T>::type F;
-    constexpr int LD = S_KC + 8;
-    __shared__ __attribute__((aligned(16))) T w[RT * 16 * LD];
+    // rows of the panel: R of the contraction each (KCONT), or 128 of R each
+    constexpr int LD = KCONT ? S_KC + 8 : RT * 16 + (RT >= 4 ? 16 : 0);
+    __shared__ __attribute__((aligned(16))) T w[(KCONT ? RT * 16 : S_KC) * LD];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int split = blockIdx.x % splits;
     const Tile f = find_tile(rows, blockIdx.x / splits, S_TM);
@@ -146,8 +166,8 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
 #pragma unroll
         for (int t = 0; t < RT; ++t) acc[m][t] = f32x4{0, 0, 0, 0};
 
-    for (int k0 = split * kper; k0 < kend; k0 += S_KC) {
-        F x[2][4];
+    F x[2][4], wv[RT];      // RT * 16 * 128 elements of the panel: RT vectors a thread
+    auto load = [&](int k0) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -155,29 +175,43 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
                 const int k = k0 + s * 32 + (lane >> 4) * 8;
                 x[m][s] = load_frag(xp[m] + k, kend - k);
             }
-        __syncthreads();
-        if (KCONT) {
-            for (int u = tid; u < RT * 16 * (S_KC / 8); u += 256) {
-                const int r = u / (S_KC / 8), k = u % (S_KC / 8) * 8;
-                *(F*)(w + r * LD + k) =
-                    load_frag(Wl + (long)r * K + k0 + k, r < R ? kend - k0 - k : 0);
-            }
-        } else {
-            for (int u = tid; u < RT * 2 * S_KC; u += 256) {
-                const int k = u / (RT * 2), r = u % (RT * 2) * 8;
-                const F v = load_frag(Wl + (long)(k0 + k) * R + r, k0 + k < kend ? R - r : 0);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[(r + j) * LD + k] = v[j];
+        for (int i = 0; i < RT; ++i) {
+            const int u = i * 256 + tid;
+            if (KCONT) {
+                const int r = u / (S_KC / 8), k = k0 + u % (S_KC / 8) * 8;
+                wv[i] = load_frag(Wl + (long)r * K + k, r < R ? kend - k : 0);
+            } else {
+                const int k = k0 + u / (RT * 2), r = u % (RT * 2) * 8;
+                wv[i] = load_frag(Wl + (long)k * R + r, k < kend ? R - r : 0);
             }
         }
+    };
+    int k0 = split * kper;
+    if (k0 < kend) load(k0);
+    for (; k0 < kend; k0 += S_KC) {
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int u = i * 256 + tid, n = KCONT ? S_KC / 8 : RT * 2;
+            *(F*)(w + u / n * LD + u % n * 8) = wv[i];
+        }
+        F now[2][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) now[m][s] = x[m][s];
+        __syncthreads();
+        if (k0 + S_KC < kend) load(k0 + S_KC);
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                const F b = *(const F*)(w + (t * 16 + (lane & 15)) * LD + s * 32 + (lane >> 4) * 8);
+                const F b = KCONT ? *(const F*)(w + (t * 16 + (lane & 15)) * LD + s * 32 +
+                                                (lane >> 4) * 8)
+                                  : column_frag(w, LD, s * 32, t * 16 + own_columns());
 #pragma unroll
-                for (int m = 0; m < 2; ++m) acc[m][t] = mfma(x[m][s], b, acc[m][t]);
+                for (int m = 0; m < 2; ++m) acc[m][t] = mfma(now[m][s], b, acc[m][t]);
             }
     }
     const float sc = scale(f.adapter);
@@ -219,164 +253,239 @@ __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ pa
 
 // ---------------------------------------------------------------------------
 // expand: out[row] = base[row] + V[row] W_l (base may be out itself, or absent: zero).  A wave
-// keeps W for 64 columns in registers and streams the workgroup's rows past it, 16 at a time.
-// W is the A operand and the rows are B's columns, so that a lane ends up with neighbouring
-// columns of one row; columns are dealt to the tiles' rows such that two tiles make eight of
-// them: column of tile t, MFMA row i = (t >> 1) * 32 + (i >> 2) * 8 + (t & 1) * 4 + (i & 3).
+// keeps W for 64 columns in registers and streams the workgroup's rows past it, 32 at a time and
+// 32 ahead.  W is the A operand and the rows are B's columns, so that a lane ends up with
+// neighbouring columns of one row; columns are dealt to the tiles' rows such that two tiles make
+// eight of them: column of tile t, MFMA row i = (t >> 1) * 32 + (i >> 2) * 8 + (t & 1) * 4 + (i & 3).
 // ---------------------------------------------------------------------------
-constexpr int E_TM = 7;
-
 template <typename T, int RK, bool RCONT>
 __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, long os,
                                                 const T* __restrict__ V, int RP,
                                                 const T* __restrict__ W, int M, int R, Rows rows,
-                                                int strips) {
+                                                int strips, int shift) {
     typedef typename Frag<T>::type F;
+    typedef typename Vec8<T>::type U8;
+    constexpr int LD = 256 + 16;
+    __shared__ __attribute__((aligned(16))) T wt[RCONT ? 8 : RK * 32 * LD];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-    const Tile f = find_tile(rows, blockIdx.x / strips, E_TM);
-    const int m0 = blockIdx.x % strips * 256 + wave * 64;
-    if (m0 >= M) return;
+    const Tile f = find_tile(rows, blockIdx.x / strips, shift);
+    const int strip = blockIdx.x % strips * 256, m0 = strip + wave * 64;
+    const bool mine = f.adapter >= 0;
+    if (!mine && base == out) return;           // nothing to add in place
     F w[RK][4];
-    if (f.adapter >= 0) {
+    if (mine) {
         const T* Wl = W + (long)f.adapter * M * R;
+        if (RCONT) {
 #pragma unroll
-        for (int k = 0; k < RK; ++k)
+            for (int k = 0; k < RK; ++k)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int i = lane & 15;
-                const int m = m0 + (t >> 1) * 32 + (i >> 2) * 8 + (t & 1) * 4 + (i & 3);
-                const int r = k * 32 + g * 8;
-                if (RCONT) {
+                for (int t = 0; t < 4; ++t) {
+                    const int i = lane & 15, r = k * 32 + g * 8;
+                    const int m = m0 + (t >> 1) * 32 + (i >> 2) * 8 + (t & 1) * 4 + (i & 3);
                     w[k][t] = load_frag(Wl + (long)m * R + r, m < M ? R - r : 0);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        w[k][t][j] =
-                            m < M && r + j < R ? Wl[(long)(r + j) * M + m] : (T)0.f;
                 }
+        } else {
+#pragma unroll
+            for (int i = 0; i < RK * 4; ++i) {
+                const int u = i * 256 + tid, r = u / 32, m = strip + u % 32 * 8;
+                *(F*)(wt + r * LD + u % 32 * 8) =
+                    load_frag(Wl + (long)r * M + m, r < R ? M - m : 0);
             }
-    }
-    const long jend = min(f.n, f.j0 + (1l << E_TM));
-    for (long j0 = f.j0; j0 < jend; j0 += 16) {
-        const long j = j0 + (lane & 15);
-        const bool ok = j < jend;
-        const long row = row_of(rows, f, ok ? j : jend - 1);
-        f32x4 acc[4];
+            __syncthreads();
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] = f32x4{0, 0, 0, 0};
-        if (f.adapter >= 0) {
+            for (int k = 0; k < RK; ++k)
 #pragma unroll
-            for (int k = 0; k < RK; ++k) {
-                const F v = *(const F*)(V + row * RP + k * 32 + g * 8);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) acc[t] = mfma(w[k][t], v, acc[t]);
-            }
+                for (int t = 0; t < 4; ++t)
+                    w[k][t] = column_frag(wt, LD, k * 32, wave * 64 + (t >> 1) * 32 +
+                                                              (lane & 3) * 8 + (t & 1) * 4);
         }
-        if (!ok) continue;
+    }
+    if (m0 >= M) return;
+    const long jend = min(f.n, f.j0 + (1l << shift));
+    F v[2][RK];
+    U8 y[2][2];
+    long row[2];
+    auto load = [&](long j0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int m = m0 + h * 32 + g * 8;
-            float o[8] = {};
-            if (m + 8 <= M) {
-                if (base) load8(base + row * bs + m, o);
+            const long j = j0 + h * 16 + (lane & 15);
+            row[h] = row_of(rows, f, j < jend ? j : jend - 1);
+            if (mine)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    o[q] += acc[2 * h][q];
-                    o[4 + q] += acc[2 * h + 1][q];
+                for (int k = 0; k < RK; ++k) v[h][k] = *(const F*)(V + row[h] * RP + k * 32 + g * 8);
+            if (base)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int m = m0 + c * 32 + g * 8;
+                    if (m + 8 <= M) y[h][c] = *(const U8*)(base + row[h] * bs + m);
                 }
-                store8(out + row * os + m, o);
-            } else {
+        }
+    };
+    load(f.j0);
+    for (long j0 = f.j0; j0 < jend; j0 += 32) {
+        f32x4 acc[2][4];
+        U8 b[2][2];
+        long at[2];
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (m + q < M) {
-                        const float b = base ? (float)base[row * bs + m + q] : 0.f;
-                        out[row * os + m + q] = (T)(b + acc[2 * h + (q >> 2)][q & 3]);
-                    }
+        for (int h = 0; h < 2; ++h) {
+            at[h] = row[h];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) b[h][c] = y[h][c];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                acc[h][t] = f32x4{0, 0, 0, 0};
+                if (mine)
+#pragma unroll
+                    for (int k = 0; k < RK; ++k) acc[h][t] = mfma(w[k][t], v[h][k], acc[h][t]);
+            }
+        }
+        if (j0 + 32 < jend) load(j0 + 32);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (j0 + h * 16 + (lane & 15) >= jend) continue;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int m = m0 + c * 32 + g * 8;
+                if (m + 8 <= M) {
+                    U8 o;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        o[q] = (T)((base ? (float)b[h][c][q] : 0.f) + acc[h][2 * c + (q >> 2)][q & 3]);
+                    *(U8*)(out + at[h] * os + m) = o;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        if (m + q < M) {
+                            const float was = base ? (float)base[at[h] * bs + m + q] : 0.f;
+                            out[at[h] * os + m + q] = (T)(was + acc[h][2 * c + (q >> 2)][q & 3]);
+                        }
+                }
             }
         }
     }
 }
 
 // ---------------------------------------------------------------------------
-// outer: part[tile][r][p] = sum over the tile's rows of P[row][p] Q[row][r].  The contraction
-// runs over rows, so both operands are transposed on their way into LDS: a thread takes two
-// rows' eight neighbours and writes eight row pairs.  LDS rows hold 64 of the contraction (128
-// bytes, all banks); the 16-byte chunk is XORed with the row so that neither the writes (16
-// column groups at once) nor the 16-byte reads (16 rows at once) meet in a bank.
+// outer: part[tile][r][p] = sum over the tile's rows of P[row][p] Q[row][r].  A workgroup owns 64
+// CT columns and walks the tile's rows 64 at a time: they pass through LDS as they are, and both
+// operands are read from there with their columns' rows side by side.
+//
+// DV: the rows meet W on the way too, partv[strip][row][r] = sum over the strip's columns of
+// P[row][p] W_l[r][p] -- the backward pass's u, in shares of 256 columns.  dy is then read once
+// for both; the shares cost 8 R bytes a row and strip (written, read again) beside the 512 of a
+// second reading of dy.
 // ---------------------------------------------------------------------------
-DEVINL int swz(int p, int chunk) { return p * 64 + ((chunk ^ (p ^ (p >> 3))) & 7) * 8; }
-
-template <typename T>
-DEVINL void stage_pair(T* lds, int p0, int pair, typename Frag<T>::type a,
-                       typename Frag<T>::type b) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        typedef T two __attribute__((ext_vector_type(2)));
-        *(two*)(lds + swz(p0 + j, pair >> 2) + (pair & 3) * 2) = two{a[j], b[j]};
-    }
-}
-
-template <typename T, int RT>
+template <typename T, int RT, int CT, bool DV>
 __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps, int NP,
                                                const T* __restrict__ Q, int RP,
-                                               float* __restrict__ part, Rows rows, int strips,
-                                               int shift) {
+                                               float* __restrict__ part,
+                                               const T* __restrict__ W, int R,
+                                               float* __restrict__ partv, long N, Rows rows,
+                                               int strips, int shift) {
     typedef typename Frag<T>::type F;
-    __shared__ __attribute__((aligned(16))) T pt[128 * 64];
-    __shared__ __attribute__((aligned(16))) T qt[RT * 16 * 64];
-    __shared__ long at[64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int tile = blockIdx.x / strips, p0 = blockIdx.x % strips * 128;
+    constexpr int PC = 64 * CT, S = PC / 32, LP = PC + 16, LQ = RT * 16 + (RT >= 4 ? 16 : 0);
+    constexpr int LW = PC + 8;
+    __shared__ __attribute__((aligned(16))) T pt[64 * LP];
+    __shared__ __attribute__((aligned(16))) T qt[64 * LQ];
+    __shared__ __attribute__((aligned(16))) T wt[DV ? RT * 16 * LW : 8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const int tile = blockIdx.x / strips, strip = blockIdx.x % strips, p0 = strip * PC;
     const Tile f = find_tile(rows, tile, shift);
     if (f.adapter < 0) return;
-    f32x4 acc[2][RT];
+    if (DV) {
+        const T* Wl = W + (long)f.adapter * NP * R;
+        for (int u = tid; u < RT * 16 * (PC / 8); u += 256) {
+            const int r = u / (PC / 8), c = u % (PC / 8) * 8;
+            *(F*)(wt + r * LW + c) = load_frag(Wl + (long)r * NP + p0 + c, r < R ? NP - p0 - c : 0);
+        }
+    }
+    f32x4 acc[CT][RT];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[m][t] = f32x4{0, 0, 0, 0};
+        for (int t = 0; t < RT; ++t) acc[c][t] = f32x4{0, 0, 0, 0};
     const long jend = min(f.n, f.j0 + (1l << shift));
+    constexpr int QV = (64 * RT * 2 + 255) / 256;       // vectors of Q a thread
+    F x[S], q[QV];
+    long row = 0;
+    bool ok = false;
+    auto load = [&](long j0) {
+        const long j = j0 + wave * 16 + (lane & 15);
+        ok = j < jend;
+        row = row_of(rows, f, ok ? j : jend - 1);
+        const T* xp = P + row * ps + p0 + g * 8;
+#pragma unroll
+        for (int s = 0; s < S; ++s) x[s] = load_frag(xp + s * 32, ok ? NP - p0 - s * 32 - g * 8 : 0);
+#pragma unroll
+        for (int i = 0; i < QV; ++i) {
+            const int u = i * 256 + tid, n = u / (RT * 2);
+            if (n >= 64) continue;
+            const long k = j0 + n;
+            const long r = row_of(rows, f, k < jend ? k : jend - 1);
+            q[i] = load_frag(Q + r * RP + u % (RT * 2) * 8, k < jend ? 8 : 0);
+        }
+    };
+    load(f.j0);
     for (long j0 = f.j0; j0 < jend; j0 += 64) {
         __syncthreads();
-        if (tid < 64) at[tid] = j0 + tid < jend ? row_of(rows, f, j0 + tid) : -1;
-        __syncthreads();
-        for (int u = tid; u < 32 * 16; u += 256) {
-            const int c = u & 15, pair = u >> 4, p = p0 + c * 8;
-            const long a = at[pair * 2], b = at[pair * 2 + 1];
-            stage_pair(pt, c * 8, pair, load_frag(P + a * ps + p, a < 0 ? 0 : NP - p),
-                       load_frag(P + b * ps + p, b < 0 ? 0 : NP - p));
-        }
-        for (int u = tid; u < 32 * RT * 2; u += 256) {
-            const int c = u % (RT * 2), pair = u / (RT * 2);
-            const long a = at[pair * 2], b = at[pair * 2 + 1];
-            stage_pair(qt, c * 8, pair, load_frag(Q + a * RP + c * 8, a < 0 ? 0 : 8),
-                       load_frag(Q + b * RP + c * 8, b < 0 ? 0 : 8));
-        }
-        __syncthreads();
+        F now[S];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            F a[2];
+        for (int s = 0; s < S; ++s) {
+            now[s] = x[s];
+            *(F*)(pt + (wave * 16 + (lane & 15)) * LP + s * 32 + g * 8) = x[s];
+        }
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
-                a[m] = *(const F*)(pt + swz(wave * 32 + m * 16 + (lane & 15), s * 4 + (lane >> 4)));
+        for (int i = 0; i < QV; ++i) {
+            const int u = i * 256 + tid, n = u / (RT * 2);
+            if (n < 64) *(F*)(qt + n * LQ + u % (RT * 2) * 8) = q[i];
+        }
+        const long at = row;
+        const bool good = ok;
+        __syncthreads();
+        if (j0 + 64 < jend) load(j0 + 64);
+        if (DV) {
+            f32x4 u[RT];
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                const F b = *(const F*)(qt + swz(t * 16 + (lane & 15), s * 4 + (lane >> 4)));
+                u[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int m = 0; m < 2; ++m) acc[m][t] = mfma(a[m], b, acc[m][t]);
+                for (int s = 0; s < S; ++s)
+                    u[t] = mfma(now[s], *(const F*)(wt + (t * 16 + (lane & 15)) * LW + s * 32 +
+                                                    g * 8), u[t]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const long r = __shfl(at, g * 4 + i, 64);
+                if (__shfl((int)good, g * 4 + i, 64))
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+                        partv[((long)strip * N + r) * (RT * 16) + t * 16 + (lane & 15)] = u[t][i];
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            F b[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) b[t] = column_frag(qt, LQ, s * 32, t * 16 + own_columns());
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                const F a = column_frag(pt, LP, s * 32, (wave * CT + c) * 16 + own_columns());
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[c][t] = mfma(a, b[t], acc[c][t]);
             }
         }
     }
-    const int LP = strips * 128;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int t = 0; t < RT; ++t)
-            *(f32x4*)(part + ((long)tile * RT * 16 + t * 16 + (lane & 15)) * LP + p0 + wave * 32 +
-                      m * 16 + (lane >> 4) * 4) = acc[m][t];
+            *(f32x4*)(part + ((long)tile * RT * 16 + t * 16 + (lane & 15)) * (strips * PC) + p0 +
+                      (wave * CT + c) * 16 + g * 4) = acc[c][t];
 }
 
-// The weights' gradient: an adapter's tiles in their order, rounded once.  An adapter without
-// rows gets zeros.  out is (L, R, NP) or, RCONT, (L, NP, R).
+// The weights' gradient: an adapter's tiles in a fixed order, rounded once.  An adapter without
+// rows gets zeros.  out is (L, R, NP) or, RCONT, (L, NP, R).  32 lanes take 128 columns of one r,
+// eight groups share the tiles.
 template <typename T, bool RCONT>
 __global__ __launch_bounds__(256) void k_outer_sum(const float* __restrict__ part, int R16, int LP,
                                                    Rows rows, int shift, T* __restrict__ out,
@@ -402,12 +511,24 @@ __global__ __launch_bounds__(256) void k_outer_sum(const float* __restrict__ par
         }
         base += __shfl(sum, 63, 64);
     }
-    const long i = (long)(blockIdx.x % blocks) * 256 + threadIdx.x;
-    if (i >= (long)NP * R) return;
-    const int p = (int)(i % NP), r = (int)(i / NP);
-    float s = 0.f;
-    for (int t = first; t < first + tiles; ++t) s += part[((long)t * R16 + r) * LP + p];
-    out[(long)l * NP * R + (RCONT ? (long)p * R + r : i)] = (T)s;
+    __shared__ f32x4 sums[256];
+    const int b = blockIdx.x % blocks, cols = (NP + 127) / 128;
+    const int r = b / cols, p = b % cols * 128 + (threadIdx.x & 31) * 4, group = threadIdx.x >> 5;
+    f32x4 s = f32x4{0, 0, 0, 0};
+    const float* q = part + (long)r * LP + p;       // LP is a multiple of 128
+#pragma unroll 4
+    for (int t = first + group; t < first + tiles; t += 8)
+        s += *(const f32x4*)(q + (long)t * R16 * LP);
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sums[k * 32 + threadIdx.x];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (p + j < NP)
+            out[(long)l * NP * R + (RCONT ? (long)(p + j) * R + r : (long)r * NP + p + j)] =
+                (T)s[j];
 }
 
 int tiles_of(const long* counts, int S, long T, int shift) {
@@ -416,62 +537,60 @@ int tiles_of(const long* counts, int S, long T, int shift) {
     return (int)n;
 }
 
-template <typename T, int RT, bool KCONT>
-void shrink_rt(const void* X, long xs, const void* W, int K, int R, const Rows& rows, int tiles,
-               const Scale& scale, void* V, int RP, float* part, long N, int splits, int kper,
-               hipStream_t st) {
-    k_shrink<T, RT, KCONT><<<(unsigned)(tiles * splits), 256, 0, st>>>(
-        (const T*)X, xs, (const T*)W, K, R, rows, scale, (T*)V, RP, part, N, splits, kper);
-}
+int r16_of(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
 template <typename T, bool KCONT>
 void shrink(const void* X, long xs, const void* W, int K, int R, const Rows& rows, int tiles,
             const Scale& scale, void* V, int RP, float* part, long N, int splits, int kper,
             hipStream_t st) {
 #define GO(RT)                                                                                   \
-    shrink_rt<T, RT, KCONT>(X, xs, W, K, R, rows, tiles, scale, V, RP, part, N, splits, kper, st)
-    const int R16 = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
+    k_shrink<T, RT, KCONT><<<(unsigned)(tiles * splits), 256, 0, st>>>(                          \
+        (const T*)X, xs, (const T*)W, K, R, rows, scale, (T*)V, RP, part, N, splits, kper)
+    const int R16 = r16_of(R);
     if (R16 == 16) GO(1);
     else if (R16 == 32) GO(2);
     else if (R16 == 64) GO(4);
     else GO(8);
 #undef GO
-    if (splits > 1) {
-        const long n = N * RP;
-        k_shrink_sum<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(part, N, R16, splits, rows,
-                                                                     scale, (T*)V, RP);
-    }
 }
 
 template <typename T, bool RCONT>
 void expand(const void* base, long bs, void* out, long os, const void* V, int RP, const void* W,
-            int M, int R, const Rows& rows, int tiles, hipStream_t st) {
+            int M, int R, const Rows& rows, int tiles, int shift, hipStream_t st) {
     const int strips = (M + 255) / 256;
 #define GO(RK)                                                                                   \
     k_expand<T, RK, RCONT><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
-        (const T*)base, bs, (T*)out, os, (const T*)V, RP, (const T*)W, M, R, rows, strips)
+        (const T*)base, bs, (T*)out, os, (const T*)V, RP, (const T*)W, M, R, rows, strips, shift)
     if (RP == 32) GO(1);
     else if (RP == 64) GO(2);
     else GO(4);
 #undef GO
 }
 
+// Columns that a workgroup of outer owns: 256, or 128 where a rank of 128 fills the registers.
+int outer_columns(int R) { return R > 64 ? 128 : 256; }
+
 template <typename T, bool RCONT>
-void outer(const void* P, long ps, int NP, const void* Q, int RP, float* part, const Rows& rows,
-           int tiles, int shift, void* out, int R, int L, hipStream_t st) {
-    const int strips = (NP + 127) / 128, R16 = R <= 16 ? 16 : RP;
-#define GO(RT)                                                                                   \
-    k_outer<T, RT><<<(unsigned)tiles * strips, 256, 0, st>>>((const T*)P, ps, NP, (const T*)Q,   \
-                                                             RP, part, rows, strips, shift)
+void outer(const void* P, long ps, int NP, const void* Q, int RP, float* part, const void* W,
+           float* partv, long N, const Rows& rows, int tiles, int shift, void* out, int R, int L,
+           hipStream_t st) {
+    const int PC = outer_columns(R), strips = (NP + PC - 1) / PC, R16 = r16_of(R);
+#define GO(RT, CT, DV)                                                                           \
+    k_outer<T, RT, CT, DV><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
+        (const T*)P, ps, NP, (const T*)Q, RP, part, (const T*)W, R, partv, N, rows, strips, shift)
     if (tiles == 0) {           // no row has an adapter: the sum below writes zeros
-    } else if (R16 == 16) GO(1);
-    else if (R16 == 32) GO(2);
-    else if (R16 == 64) GO(4);
-    else GO(8);
+    } else if (R16 == 16) {
+        if (W) GO(1, 4, true);
+        else GO(1, 4, false);
+    } else if (R16 == 32) {
+        if (W) GO(2, 4, true);
+        else GO(2, 4, false);
+    } else if (R16 == 64) GO(4, 4, false);
+    else GO(8, 2, false);
 #undef GO
-    const int blocks = (int)(((long)NP * R + 255) / 256);
+    const int blocks = (NP + 127) / 128 * R;
     k_outer_sum<T, RCONT><<<(unsigned)L * blocks, 256, 0, st>>>(
-        part, R16, strips * 128, rows, shift, (T*)out, NP, R, blocks);
+        part, R16, strips * PC, rows, shift, (T*)out, NP, R, blocks);
 }
 
 }  // namespace
@@ -488,6 +607,7 @@ int lowrank_splits(const long* counts, int S, long T, int K) {
     return want < 1 ? 1 : want > most ? most : want;
 }
 
+// `part` (splits, N, R16) is left unsummed for launch_shrink_sum where splits > 1.
 void launch_shrink(int type, int kcont, const void* X, long xs, const void* W, int K, int R,
                    const int* order, const int* segs, const int* adapter, const long* counts,
                    int S, int Bn, long T, const float* scale, float scale_all, void* V,
@@ -511,44 +631,73 @@ void launch_shrink(int type, int kcont, const void* X, long xs, const void* W, i
                                      kper, st);
 }
 
+void launch_shrink_sum(int type, int R, const int* order, const int* segs, const int* adapter,
+                       int S, int Bn, long T, const float* scale, float scale_all, void* V,
+                       const float* part, int splits, hipStream_t st) {
+    const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
+    const Scale sc{scale, scale_all};
+    const int RP = lowrank_rp(R), R16 = r16_of(R);
+    const long N = T * Bn, blocks = (N * RP + 255) / 256;
+    if (type == LM_BF16)
+        k_shrink_sum<bf16_t><<<(unsigned)blocks, 256, 0, st>>>(part, N, R16, splits, rows, sc,
+                                                               (bf16_t*)V, RP);
+    else
+        k_shrink_sum<f16_t><<<(unsigned)blocks, 256, 0, st>>>(part, N, R16, splits, rows, sc,
+                                                              (f16_t*)V, RP);
+}
+
 void launch_expand(int type, int rcont, const void* base, long bs, void* out, long os,
                    const void* V, const void* W, int M, int R, const int* order, const int* segs,
                    const int* adapter, const long* counts, int S, int Bn, long T,
                    hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
-    const int tiles = tiles_of(counts, S, T, E_TM), RP = lowrank_rp(R);
+    // rows a workgroup: as many as leave four workgroups a CU, 256 at most, 32 at least
+    const long strips = (M + 255) / 256;
+    int shift = 8;
+    while (shift > 5 && tiles_of(counts, S, T, shift) * strips < 1024) --shift;
+    const int tiles = tiles_of(counts, S, T, shift), RP = lowrank_rp(R);
     if (tiles == 0) return;
     if (type == LM_BF16)
-        rcont ? expand<bf16_t, true>(base, bs, out, os, V, RP, W, M, R, rows, tiles, st)
-              : expand<bf16_t, false>(base, bs, out, os, V, RP, W, M, R, rows, tiles, st);
+        rcont ? expand<bf16_t, true>(base, bs, out, os, V, RP, W, M, R, rows, tiles, shift, st)
+              : expand<bf16_t, false>(base, bs, out, os, V, RP, W, M, R, rows, tiles, shift, st);
     else
-        rcont ? expand<f16_t, true>(base, bs, out, os, V, RP, W, M, R, rows, tiles, st)
-              : expand<f16_t, false>(base, bs, out, os, V, RP, W, M, R, rows, tiles, st);
+        rcont ? expand<f16_t, true>(base, bs, out, os, V, RP, W, M, R, rows, tiles, shift, st)
+              : expand<f16_t, false>(base, bs, out, os, V, RP, W, M, R, rows, tiles, shift, st);
 }
 
-// log2 of the rows that one partial gradient sums: about two workgroups a CU over the strips,
+int lowrank_strips(int NP, int R) { return (NP + outer_columns(R) - 1) / outer_columns(R); }
+// log2 of the rows that one partial gradient sums: about four workgroups a CU over the strips,
 // never fewer than 64 rows (a step) nor more than 4096.
-int lowrank_outer_shift(const long* counts, int S, long T, int NP) {
-    const int strips = (NP + 127) / 128;
+int lowrank_outer_shift(const long* counts, int S, long T, int NP, int R) {
+    const long strips = lowrank_strips(NP, R);
     int shift = 12;
-    while (shift > 6 && (long)tiles_of(counts, S, T, shift) * strips < 1024) --shift;
+    while (shift > 6 && tiles_of(counts, S, T, shift) * strips < 1024) --shift;
     return shift;
 }
 int lowrank_outer_tiles(const long* counts, int S, long T, int shift) {
     return tiles_of(counts, S, T, shift);
 }
+// Whether the backward pass reads dy once for u and dB (k_outer's DV): not where the shares of u
+// would be as many bytes as dy.
+int lowrank_one_reading(int R) { return R <= 32; }
 
 void launch_outer(int type, int rcont, const void* P, long ps, int NP, const void* Q, float* part,
-                  const int* order, const int* segs, const int* adapter, const long* counts,
-                  int S, int Bn, long T, int shift, void* out, int R, int L, hipStream_t st) {
+                  const void* W, float* partv, const int* order, const int* segs,
+                  const int* adapter, const long* counts, int S, int Bn, long T, int shift,
+                  void* out, int R, int L, hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const int tiles = tiles_of(counts, S, T, shift), RP = lowrank_rp(R);
+    const long N = T * Bn;
     if (type == LM_BF16)
-        rcont ? outer<bf16_t, true>(P, ps, NP, Q, RP, part, rows, tiles, shift, out, R, L, st)
-              : outer<bf16_t, false>(P, ps, NP, Q, RP, part, rows, tiles, shift, out, R, L, st);
+        rcont ? outer<bf16_t, true>(P, ps, NP, Q, RP, part, W, partv, N, rows, tiles, shift, out,
+                                    R, L, st)
+              : outer<bf16_t, false>(P, ps, NP, Q, RP, part, W, partv, N, rows, tiles, shift, out,
+                                     R, L, st);
     else
-        rcont ? outer<f16_t, true>(P, ps, NP, Q, RP, part, rows, tiles, shift, out, R, L, st)
-              : outer<f16_t, false>(P, ps, NP, Q, RP, part, rows, tiles, shift, out, R, L, st);
+        rcont ? outer<f16_t, true>(P, ps, NP, Q, RP, part, W, partv, N, rows, tiles, shift, out,
+                                   R, L, st)
+              : outer<f16_t, false>(P, ps, NP, Q, RP, part, W, partv, N, rows, tiles, shift, out,
+                                    R, L, st);
 }
 
 }  // extern "C"

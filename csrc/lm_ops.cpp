@@ -12,29 +12,33 @@
 #include <vector>
 
 extern "C" {
-int distill_splits(long N, int V);
+int distill_in_registers(int V);
 void launch_distill_fwd(int, const void*, long, const void*, long, int, const void*, long, int,
-                        const long*, int, float*, float*, float*, float*, float*, long, int,
-                        float, float,
-                        hipStream_t);
+                        const long*, int, void*, float*, float*, float*, void*, long, int, float,
+                        float, float, hipStream_t);
 void launch_distill_bwd(int, const void*, long, const void*, long, int, const void*, long, int,
-                        const long*, int, const float*, const float*, const float*, void*, long,
-                        int, float, float, hipStream_t);
+                        const long*, int, const void*, const float*, const float*, void*, int,
+                        long, int, float, float, hipStream_t);
 void launch_adjust(int, const void*, long, void*, const void*, long, int, int, const void*, int,
                    const void*, int, const float*, float, const float*, float, const float*,
                    float, const void*, long, int, const float*, long, int, const unsigned*, long,
                    long, int, hipStream_t);
 int lowrank_rp(int R);
 int lowrank_splits(const long* counts, int S, long T, int K);
-int lowrank_outer_shift(const long* counts, int S, long T, int NP);
+int lowrank_strips(int NP, int R);
+int lowrank_outer_shift(const long* counts, int S, long T, int NP, int R);
 int lowrank_outer_tiles(const long* counts, int S, long T, int shift);
+int lowrank_one_reading(int R);
 void launch_shrink(int, int, const void*, long, const void*, int, int, const int*, const int*,
                    const int*, const long*, int, int, long, const float*, float, void*, float*,
                    hipStream_t);
+void launch_shrink_sum(int, int, const int*, const int*, const int*, int, int, long, const float*,
+                       float, void*, const float*, int, hipStream_t);
 void launch_expand(int, int, const void*, long, void*, long, const void*, const void*, int, int,
                    const int*, const int*, const int*, const long*, int, int, long, hipStream_t);
-void launch_outer(int, int, const void*, long, int, const void*, float*, const int*, const int*,
-                  const int*, const long*, int, int, long, int, void*, int, int, hipStream_t);
+void launch_outer(int, int, const void*, long, int, const void*, float*, const void*, float*,
+                  const int*, const int*, const int*, const long*, int, int, long, int, void*,
+                  int, int, hipStream_t);
 }
 
 namespace {
@@ -105,6 +109,7 @@ struct Distill {
         N = z.size(0);
         V = (int)z.size(1);
         K = (int)t.size(1);
+        TORCH_CHECK(N < (1l << 32) / (V > 8192 ? 1024 : 256), "distill: too many rows");
         tp = nullptr;
         if (y.has_value()) {
             TORCH_CHECK(y->dim() == 1 && y->size(0) == N && y->scalar_type() == at::kLong,
@@ -116,44 +121,72 @@ struct Distill {
     }
 };
 
-// -> (loss, 1 / counted rows, stats (N, 8) fp32; the last two for the backward pass)
-std::vector<Tensor> distill_fwd(Tensor logits, Tensor index, Tensor teacher, OptTensor targets,
-                                double alpha, double tau) {
-    const Distill d(logits, index, teacher, targets);
-    const c10::DeviceGuard guard(logits.device());
-    const auto f32 = logits.options().dtype(at::kFloat);
-    const int splits = distill_splits(d.N, d.V);
-    auto loss = at::empty({}, f32), inv = at::empty({}, f32), stats = at::empty({d.N, 8}, f32);
-    auto work = at::empty({d.N * (2 + 3 * (long)splits)}, f32);
-    float* rows = (float*)work.data_ptr();
-    launch_distill_fwd(d.type, d.z.data_ptr(), row_stride(d.z), d.index.data_ptr(),
-                       row_stride(d.index), d.index64, d.teacher.data_ptr(),
-                       row_stride(d.teacher), d.ttype, d.tp, d.K, rows + 2 * d.N,
-                       (float*)stats.data_ptr(), rows, (float*)loss.data_ptr(),
-                       (float*)inv.data_ptr(), d.N, d.V, (float)alpha, (float)tau, stream_of(logits));
-    check_launch("distill_fwd");
-    return {loss, inv, stats};
-}
+// The gradient is written with the loss where that can be; the backward pass then only looks
+// whether it is scaled (csrc/distill.hip).
+struct DistillLoss : public torch::autograd::Function<DistillLoss> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor logits, Tensor index,
+                          Tensor teacher, OptTensor targets, double alpha, double tau,
+                          double weight, bool need) {
+        const Distill d(logits, index, teacher, targets);
+        const c10::DeviceGuard guard(logits.device());
+        const auto f32 = logits.options().dtype(at::kFloat);
+        auto loss = at::empty({}, f32), inv = at::empty({}, f32), stats = at::empty({d.N, 8}, f32);
+        auto rows = at::empty({d.N}, f32);
+        Tensor dz;
+        if (need && d.N > 0 && distill_in_registers(d.V))
+            dz = at::empty({d.N, (long)d.V}, logits.options());
+        launch_distill_fwd(d.type, d.z.data_ptr(), row_stride(d.z), d.index.data_ptr(),
+                           row_stride(d.index), d.index64, d.teacher.data_ptr(),
+                           row_stride(d.teacher), d.ttype, d.tp, d.K, stats.data_ptr(),
+                           (float*)rows.data_ptr(), (float*)loss.data_ptr(),
+                           (float*)inv.data_ptr(), dz.defined() ? dz.data_ptr() : nullptr, d.N,
+                           d.V, (float)alpha, (float)tau, (float)weight, stream_of(logits));
+        check_launch("distill_loss");
+        if (need) {
+            ctx->save_for_backward({logits, index, teacher, targets.value_or(Tensor()), stats,
+                                    inv});
+            ctx->saved_data["alpha"] = alpha;
+            ctx->saved_data["tau"] = tau;
+            if (dz.defined()) ctx->saved_data["dz"] = dz;
+        }
+        return loss;
+    }
 
-Tensor distill_bwd(Tensor logits, Tensor index, Tensor teacher, OptTensor targets, Tensor stats,
-                   Tensor inv, Tensor grad, double alpha, double tau) {
-    const Distill d(logits, index, teacher, targets);
-    const c10::DeviceGuard guard(logits.device());
-    TORCH_CHECK(stats.is_contiguous() && stats.numel() == d.N * 8 && inv.numel() == 1,
-                "distill_bwd: stats and inv as distill_fwd returned them");
-    check_on(grad, logits, "grad");
-    const Tensor g = grad.to(at::kFloat).contiguous();
-    TORCH_CHECK(g.numel() == 1, "distill_bwd: the gradient of the loss is one number");
-    auto dz = at::empty({d.N, (long)d.V}, logits.options());
-    if (d.N == 0) return dz;
-    launch_distill_bwd(d.type, d.z.data_ptr(), row_stride(d.z), d.index.data_ptr(),
-                       row_stride(d.index), d.index64, d.teacher.data_ptr(),
-                       row_stride(d.teacher), d.ttype, d.tp, d.K,
-                       (const float*)stats.data_ptr(), (const float*)inv.data_ptr(),
-                       (const float*)g.data_ptr(), dz.data_ptr(), d.N, d.V, (float)alpha,
-                       (float)tau, stream_of(logits));
-    check_launch("distill_bwd");
-    return dz;
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "distill_loss is differentiable once");
+        const auto v = ctx->get_saved_variables();
+        const Tensor &logits = v[0], &g = grads[0];
+        torch::autograd::variable_list out(8);
+        if (!g.defined()) return out;
+        const Distill d(logits, v[1], v[2], v[3].defined() ? OptTensor(v[3]) : OptTensor());
+        const c10::DeviceGuard guard(logits.device());
+        // handed out once: a second backward pass over a kept graph computes its own
+        const auto had = ctx->saved_data.find("dz");
+        const bool done = had != ctx->saved_data.end();
+        if (done) {
+            out[0] = had->second.toTensor();
+            ctx->saved_data.erase(had);
+        } else {
+            out[0] = at::empty({d.N, (long)d.V}, logits.options());
+        }
+        if (d.N > 0)
+            launch_distill_bwd(d.type, d.z.data_ptr(), row_stride(d.z), d.index.data_ptr(),
+                               row_stride(d.index), d.index64, d.teacher.data_ptr(),
+                               row_stride(d.teacher), d.ttype, d.tp, d.K, v[4].data_ptr(),
+                               (const float*)v[5].data_ptr(), (const float*)g.data_ptr(),
+                               out[0].data_ptr(), done, d.N, d.V,
+                               (float)ctx->saved_data["alpha"].toDouble(),
+                               (float)ctx->saved_data["tau"].toDouble(), stream_of(logits));
+        check_launch("distill_loss backward");
+        return out;
+    }
+};
+
+Tensor distill_loss(Tensor logits, Tensor index, Tensor teacher, OptTensor targets, double alpha,
+                    double tau, double weight) {
+    const bool need = at::GradMode::is_enabled() && logits.requires_grad();
+    return DistillLoss::apply(logits, index, teacher, targets, alpha, tau, weight, need);
 }
 
 // ------------------------------------------------------------------ logits of a decode step
@@ -245,11 +278,12 @@ struct Grouped {
             double all)
         : order(order_), segs(segs_), adapter(adapter_), counts(counts_.begin(), counts_.end()),
           scale_all((float)all) {
-        TORCH_CHECK(x.is_cuda() && x.dim() == 2 && y.dim() == 2 && x.size(0) == y.size(0),
-                    "lowrank: x (N, K) and y (N, M) on GPU");
+        TORCH_CHECK(x.is_cuda() && x.dim() >= 2 && x.dim() == y.dim() &&
+                        x.sizes().slice(0, x.dim() - 1) == y.sizes().slice(0, y.dim() - 1),
+                    "lowrank: x (..., Bn, K) and y (..., Bn, M) on GPU");
         TORCH_CHECK(a.dim() == 3 && b.dim() == 3 && a.size(0) == b.size(0) &&
-                        a.size(2) == b.size(1) && a.size(1) == x.size(1) &&
-                        b.size(2) == y.size(1),
+                        a.size(2) == b.size(1) && a.size(1) == x.size(-1) &&
+                        b.size(2) == y.size(-1),
                     "lowrank: a (L, K, R), b (L, R, M)");
         TORCH_CHECK(a.is_contiguous() && b.is_contiguous(), "lowrank: a and b contiguous");
         for (const Tensor* t : {&y, &a, &b}) {
@@ -266,7 +300,8 @@ struct Grouped {
         K = (int)a.size(1);
         R = (int)a.size(2);
         M = (int)b.size(2);
-        N = x.size(0);
+        TORCH_CHECK(x.numel() > 0 && y.numel() > 0, "lowrank: no rows");
+        N = x.numel() / K;
         Bn = (int)order.numel();
         S = (int)counts.size();
         TORCH_CHECK(R >= 1 && R <= 128 && K >= 1 && M >= 1 && K < (1 << 30) && M < (1 << 30),
@@ -296,8 +331,13 @@ struct Grouped {
         launch_shrink(type, kcont, x.data_ptr(), row_stride(x), w.data_ptr(), k, R, ip(order),
                       ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
                       v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, st);
+        if (splits > 1) sum(v, part, splits, st);
         check_launch("lowrank shrink");
         return v;
+    }
+    void sum(Tensor& v, const Tensor& part, int splits, hipStream_t st) const {
+        launch_shrink_sum(type, R, ip(order), ip(segs), ip(adapter), S, Bn, T, float_ptr(scale),
+                          scale_all, v.data_ptr(), (const float*)part.data_ptr(), splits, st);
     }
     // out = base + v W, W (L, R, M) or, rank contiguous, (L, M, R)
     void expand(const Tensor& base, Tensor& out, const Tensor& v, const Tensor& w, bool rcont,
@@ -308,84 +348,122 @@ struct Grouped {
                       ip(adapter), counts.data(), S, Bn, T, st);
         check_launch("lowrank expand");
     }
-    // sum over an adapter's rows of p^T q: (L, R, NP) or, rank contiguous, (L, NP, R)
-    Tensor outer(const Tensor& p, const Tensor& q, bool rcont, hipStream_t st) const {
-        const int np = (int)p.size(1), shift = lowrank_outer_shift(counts.data(), S, T, np);
+    // sum over an adapter's rows of p^T q: (L, R, NP) or, rank contiguous, (L, NP, R).  With w
+    // (L, R, NP) also `u` (N, RP) = s p w^T, from the same reading of p.
+    Tensor outer(const Tensor& p, const Tensor& q, bool rcont, hipStream_t st,
+                 const Tensor& w = Tensor(), Tensor* u = nullptr) const {
+        const int np = (int)p.size(1), strips = lowrank_strips(np, R), rp = lowrank_rp(R);
+        const int shift = lowrank_outer_shift(counts.data(), S, T, np, R);
         const long tiles = lowrank_outer_tiles(counts.data(), S, T, shift);
-        auto part = at::empty({tiles * lowrank_rp(R) * ((np + 127) / 128 * 128)},
-                              p.options().dtype(at::kFloat));
+        const auto f32 = p.options().dtype(at::kFloat);
+        auto part = at::empty({tiles * rp * strips * 256l}, f32);
+        Tensor partv;
+        if (u) partv = at::empty({strips * N * rp}, f32);
         auto out = rcont ? at::empty({L, np, R}, p.options()) : at::empty({L, R, np}, p.options());
         launch_outer(type, rcont, p.data_ptr(), row_stride(p), np, q.data_ptr(),
-                     (float*)part.data_ptr(), ip(order), ip(segs), ip(adapter), counts.data(), S,
-                     Bn, T, shift, out.data_ptr(), R, L, st);
+                     (float*)part.data_ptr(), u ? w.data_ptr() : nullptr,
+                     u ? (float*)partv.data_ptr() : nullptr, ip(order), ip(segs), ip(adapter),
+                     counts.data(), S, Bn, T, shift, out.data_ptr(), R, L, st);
+        if (u) {
+            *u = at::empty({N, (long)rp}, p.options());
+            sum(*u, partv, strips, st);
+        }
         check_launch("lowrank outer");
         return out;
     }
 };
 
-// -> (out, v); out is y itself where `inplace`
-std::vector<Tensor> lowrank_fwd(Tensor y, Tensor x, Tensor a, Tensor b, Tensor order, Tensor segs,
-                                Tensor adapter, std::vector<int64_t> counts, OptTensor scale,
-                                double scale_all, bool inplace) {
-    const c10::DeviceGuard guard(x.device());
-    const Grouped g(x, y, a, b, order, segs, adapter, counts, scale, scale_all);
+// y + s x A B, y and x of any leading shape over rows of Bn columns; `v` for the backward pass.
+Tensor lowrank_forward(const Grouped& g, const Tensor& y, const Tensor& x, const Tensor& a,
+                       const Tensor& b, bool inplace, Tensor* v) {
     const hipStream_t st = stream_of(x);
-    const Tensor xr = rows_of(x), yr = inplace ? y : rows_of(y);
-    TORCH_CHECK(yr.size(1) <= 1 || yr.stride(1) == 1, "lowrank: y's rows must be contiguous");
-    Tensor out = inplace ? y : at::empty({g.N, (long)g.M}, y.options());
-    Tensor v = g.shrink(xr, a, false, st);
-    g.expand(yr, out, v, b, false, st);
-    return {out, v};
+    Tensor out = inplace ? y : at::empty(y.sizes(), y.options());
+    Tensor rows = out.view({g.N, (long)g.M});
+    *v = g.shrink(rows_of(x.reshape({g.N, (long)g.K})), a, false, st);
+    g.expand(inplace ? rows : rows_of(y.reshape({g.N, (long)g.M})), rows, *v, b, false, st);
+    return out;
 }
 
-std::vector<OptTensor> lowrank_bwd(Tensor dy, Tensor x, Tensor a, Tensor b, Tensor v, Tensor order,
-                                   Tensor segs, Tensor adapter, std::vector<int64_t> counts,
-                                   OptTensor scale, double scale_all, bool need_x, bool need_a,
-                                   bool need_b) {
-    const c10::DeviceGuard guard(x.device());
-    const Grouped g(x, dy, a, b, order, segs, adapter, counts, scale, scale_all);
-    const hipStream_t st = stream_of(x);
-    TORCH_CHECK(v.dim() == 2 && v.size(0) == g.N && v.size(1) == lowrank_rp(g.R) &&
-                    v.is_contiguous() && v.scalar_type() == x.scalar_type(),
-                "lowrank_bwd: v as lowrank_fwd returned it");
-    check_on(v, x, "v");
-    const Tensor xr = rows_of(x), dr = rows_of(dy);
-    OptTensor dx, da, db;
-    if (need_x || need_a) {
-        const Tensor u = g.shrink(dr, b, true, st);
-        if (need_x) {
-            Tensor out = at::empty({g.N, (long)g.K}, x.options());
-            g.expand(Tensor(), out, u, a, true, st);
-            dx = out;
-        }
-        if (need_a) da = g.outer(xr, u, true, st);
+struct LowRankAdd : public torch::autograd::Function<LowRankAdd> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor y, Tensor x, Tensor a,
+                          Tensor b, Tensor order, Tensor segs, Tensor adapter,
+                          std::vector<int64_t> counts, OptTensor scale, double scale_all) {
+        const c10::DeviceGuard guard(x.device());
+        const Grouped g(x, y, a, b, order, segs, adapter, counts, scale, scale_all);
+        Tensor v, out = lowrank_forward(g, y, x, a, b, false, &v);
+        ctx->save_for_backward({x, a, b, v, order, segs, adapter, scale.value_or(Tensor())});
+        ctx->saved_data["counts"] = counts;
+        ctx->saved_data["scale"] = scale_all;
+        ctx->saved_data["need"] = std::vector<bool>{y.requires_grad(), x.requires_grad(),
+                                                    a.requires_grad(), b.requires_grad()};
+        return out;
     }
-    if (need_b) db = g.outer(dr, v, false, st);
-    return {dx, da, db};
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "lowrank_add is differentiable once");
+        torch::autograd::variable_list out(10);
+        const Tensor& dy = grads[0];
+        if (!dy.defined()) return out;
+        const auto s = ctx->get_saved_variables();
+        const Tensor &x = s[0], &a = s[1], &b = s[2], &v = s[3];
+        const c10::DeviceGuard guard(x.device());
+        const Grouped g(x, dy, a, b, s[4], s[5], s[6], ctx->saved_data["counts"].toIntVector(),
+                        s[7].defined() ? OptTensor(s[7]) : OptTensor(),
+                        ctx->saved_data["scale"].toDouble());
+        const hipStream_t st = stream_of(x);
+        const auto need = ctx->saved_data["need"].toBoolList();
+        const bool need_u = need[1] || need[2];
+        if (need[0]) out[0] = dy;
+        if (!need_u && !need[3]) return out;
+        const Tensor dr = rows_of(dy.reshape({g.N, (long)g.M}));
+        Tensor u;
+        if (need[3] && need_u && lowrank_one_reading(g.R)) {
+            out[3] = g.outer(dr, v, false, st, b, &u);
+        } else {
+            if (need[3]) out[3] = g.outer(dr, v, false, st);
+            if (need_u) u = g.shrink(dr, b, true, st);
+        }
+        if (need[1]) {
+            out[1] = at::empty(x.sizes(), x.options());
+            Tensor rows = out[1].view({g.N, (long)g.K});
+            g.expand(Tensor(), rows, u, a, true, st);
+        }
+        if (need[2]) out[2] = g.outer(rows_of(x.reshape({g.N, (long)g.K})), u, true, st);
+        return out;
+    }
+};
+
+Tensor lowrank_add(Tensor y, Tensor x, Tensor a, Tensor b, Tensor order, Tensor segs,
+                   Tensor adapter, std::vector<int64_t> counts, OptTensor scale, double scale_all,
+                   bool inplace) {
+    if (!inplace && at::GradMode::is_enabled() &&
+        (y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad()))
+        return LowRankAdd::apply(y, x, a.contiguous(), b.contiguous(), order, segs, adapter,
+                                 counts, scale, scale_all);
+    const at::NoGradGuard off;
+    const c10::DeviceGuard guard(x.device());
+    const Tensor ac = a.contiguous(), bc = b.contiguous();
+    const Grouped g(x, y, ac, bc, order, segs, adapter, counts, scale, scale_all);
+    TORCH_CHECK(!inplace || y.is_contiguous(), "lowrank: y must be contiguous");
+    Tensor v;
+    return lowrank_forward(g, y, x, ac, bc, inplace, &v);
 }
 
 }  // namespace
 
 void register_lm_ops(pybind11::module_& m) {
     namespace py = pybind11;
-    m.def("distill_fwd", &distill_fwd, "distillation from a teacher's top logits: loss, stats",
-          py::arg("logits"), py::arg("index"), py::arg("teacher"), py::arg("targets") = py::none(),
-          py::arg("alpha"), py::arg("tau"));
-    m.def("distill_bwd", &distill_bwd, "gradient of distill_fwd", py::arg("logits"),
-          py::arg("index"), py::arg("teacher"), py::arg("targets") = py::none(), py::arg("stats"),
-          py::arg("inv"), py::arg("grad"), py::arg("alpha"), py::arg("tau"));
+    m.def("distill_loss", &distill_loss, "distillation from a teacher's top logits",
+          py::arg("logits"), py::arg("index"), py::arg("teacher"), py::arg("targets"),
+          py::arg("alpha"), py::arg("tau"), py::arg("weight"));
     m.def("adjust_logits", &adjust, "penalties, biases and masks on decode logits",
           py::arg("logits"), py::arg("history"), py::arg("lengths"), py::arg("prompt_lengths"),
           py::arg("repetition"), py::arg("repetition_all"), py::arg("presence"),
           py::arg("presence_all"), py::arg("frequency"), py::arg("frequency_all"),
           py::arg("bias_index"), py::arg("bias"), py::arg("allowed"));
-    m.def("lowrank_fwd", &lowrank_fwd, "y + s x A B by rows' adapters", py::arg("y"),
+    m.def("lowrank_add", &lowrank_add, "y + s x A B by rows' adapters", py::arg("y"),
           py::arg("x"), py::arg("a"), py::arg("b"), py::arg("order"), py::arg("segs"),
           py::arg("adapter"), py::arg("counts"), py::arg("scale") = py::none(),
           py::arg("scale_all") = 1.0, py::arg("inplace") = false);
-    m.def("lowrank_bwd", &lowrank_bwd, "gradients of lowrank_fwd", py::arg("dy"), py::arg("x"),
-          py::arg("a"), py::arg("b"), py::arg("v"), py::arg("order"), py::arg("segs"),
-          py::arg("adapter"), py::arg("counts"), py::arg("scale") = py::none(),
-          py::arg("scale_all") = 1.0, py::arg("need_x") = true, py::arg("need_a") = true,
-          py::arg("need_b") = true);
 }

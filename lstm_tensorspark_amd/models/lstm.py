@@ -306,11 +306,11 @@ class LSTMModel(nn.Module):
 
     def distill_loss(self, output: torch.Tensor, teacher: torch.Tensor,
                      y: Optional[torch.Tensor], top_k: int = 64,
-                     alpha: float = 0.5,
-                     temperature: float = 2.0) -> torch.Tensor:
+                     alpha: float = 0.5, temperature: float = 2.0,
+                     weight: float = 1.0) -> torch.Tensor:
         """Loss against a teacher's logits (same shape as `output`): its
         top_k of every position at `temperature`, weighed by alpha against
-        the labels y (ops/distill.py)."""
+        the labels y, the whole multiplied by weight (ops/distill.py)."""
         if self.cfg.head == "none":
             raise ValueError("distillation needs a head with logits")
         if teacher.shape != output.shape:
@@ -320,7 +320,8 @@ class LSTMModel(nn.Module):
         top = teacher.detach().reshape(-1, C).topk(min(top_k, C), dim=1)
         return distill_loss(output.reshape(-1, C), top.indices, top.values,
                             None if y is None else y.reshape(-1),
-                            alpha=alpha, temperature=temperature)
+                            alpha=alpha, temperature=temperature,
+                            weight=weight)
 
     def detach_state(self, state):
         """Detach the (h, c) carry for truncated BPTT."""

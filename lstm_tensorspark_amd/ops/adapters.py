@@ -102,37 +102,6 @@ def _launch_args(rows: AdapterRows, scale):
                 counts=rows.counts, scale_all=float(scale))
 
 
-class LowRankFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, x, a, b, rows, scale):
-        K, M = x.shape[-1], y.shape[-1]
-        x2 = x.reshape(-1, K)
-        out, v = extension.get_extension().lowrank_fwd(
-            y.reshape(-1, M), x2, a, b, **_launch_args(rows, scale))
-        ctx.save_for_backward(x2, a, b, v, scale if isinstance(
-            scale, torch.Tensor) else None)
-        ctx.rows, ctx.scale, ctx.shape = rows, scale, x.shape
-        if isinstance(scale, torch.Tensor):
-            ctx.scale = None
-        return out.view(y.shape)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x2, a, b, v, scale = ctx.saved_tensors
-        scale = ctx.scale if scale is None else scale
-        ng = ctx.needs_input_grad
-        dx = da = db = None
-        if any(ng[1:4]):
-            dx, da, db = extension.get_extension().lowrank_bwd(
-                dy.reshape(-1, dy.shape[-1]), x2, a, b, v,
-                need_x=ng[1], need_a=ng[2], need_b=ng[3],
-                **_launch_args(ctx.rows, scale))
-        if dx is not None:
-            dx = dx.view(ctx.shape)
-        return dy if ng[0] else None, dx, da, db, None, None
-
-
 def _check(y, x, a, b, rows, scale):
     if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] \
             or a.shape[2] != b.shape[1]:
@@ -184,7 +153,8 @@ def lowrank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
     _check(y, x, a, b, rows, scale)
     if not _kernels(x) or x.numel() == 0 or y.numel() == 0:
         return _ref_lowrank(y, x, a, b, rows, scale)
-    return LowRankFn.apply(y, x, a.contiguous(), b.contiguous(), rows, scale)
+    return extension.get_extension().lowrank_add(
+        y, x, a, b, **_launch_args(rows, scale))
 
 
 @torch.no_grad()
@@ -198,7 +168,6 @@ def lowrank_add_(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
         raise ValueError("y must be contiguous")
     if not _kernels(x) or x.numel() == 0 or y.numel() == 0:
         return y.copy_(_ref_lowrank(y, x, a, b, rows, scale))
-    extension.get_extension().lowrank_fwd(
-        y.view(-1, y.shape[-1]), x.reshape(-1, x.shape[-1]), a.contiguous(),
-        b.contiguous(), inplace=True, **_launch_args(rows, scale))
+    extension.get_extension().lowrank_add(
+        y, x, a, b, inplace=True, **_launch_args(rows, scale))
     return y

@@ -10,9 +10,8 @@ all of its mass.  One row of `distill_loss` is
           + (1 - alpha) * (logsumexp(z) - z[y])
 
 and the loss is the sum of the rows over the number of rows that list an
-entry or carry a label.  Both terms come out of ONE pass over the logits in
-the forward and one in the backward (csrc/distill.hip); no (N, V) fp32
-intermediate.  bf16, fp16 and fp32 logits run the kernels on the GPU, the
+entry or carry a label.  Loss and gradient come out of ONE pass over the logits
+(csrc/distill.hip); no (N, V) fp32 intermediate.  bf16, fp16 and fp32 logits run the kernels on the GPU, the
 CPU and fp64 the reference below.
 """
 from __future__ import annotations
@@ -61,31 +60,11 @@ def _ref_distill(logits, index, teacher, targets, alpha, tau):
     return rows.sum() / (soft | label).sum().clamp_min(1)
 
 
-class DistillFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, index, teacher, targets, alpha, tau):
-        ext = extension.get_extension()
-        loss, inv, stats = ext.distill_fwd(logits, index, teacher, targets,
-                                           alpha, tau)
-        ctx.save_for_backward(logits, index, teacher, targets, stats, inv)
-        ctx.alpha, ctx.tau = alpha, tau
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        logits, index, teacher, targets, stats, inv = ctx.saved_tensors
-        # grad_out stays on the device: the kernel reads it
-        dz = extension.get_extension().distill_bwd(
-            logits, index, teacher, targets, stats, inv, grad_out, ctx.alpha,
-            ctx.tau)
-        return dz, None, None, None, None, None
-
-
 def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
                  teacher_logits: torch.Tensor,
                  targets: Optional[torch.Tensor] = None, *,
-                 alpha: float = 1.0, temperature: float = 1.0) -> torch.Tensor:
+                 alpha: float = 1.0, temperature: float = 1.0,
+                 weight: float = 1.0) -> torch.Tensor:
     """Mean loss (fp32 scalar; fp64 for fp64 logits) over the rows that list
     a teacher's entry or carry a label.
 
@@ -97,6 +76,10 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
     targets: (N,) int64 labels or None; one outside [0, V) is no label.
     alpha weighs the teacher against the labels (without labels it has to be
     1), `temperature` applies to the teacher's term alone.
+    weight multiplies the loss.  Given here (1 / micro-batches, a loss scale)
+    and not afterwards, it keeps the incoming gradient at 1, for which the
+    forward has already written the logits' gradient; for any other the
+    backward computes it anew.
     A row of padding (no entry and no label) adds nothing, is not counted
     and gets a zero gradient.
     """
@@ -118,6 +101,8 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
         raise ValueError(f"alpha must be in [0, 1], got {alpha}")
     if not (temperature > 0.0 and math.isfinite(temperature)):
         raise ValueError(f"temperature must be positive, got {temperature}")
+    if not math.isfinite(weight):
+        raise ValueError(f"weight must be finite, got {weight}")
     if targets is None and alpha != 1.0:
         raise ValueError("alpha < 1 needs targets")
     if targets is not None and (targets.dtype != torch.long
@@ -129,7 +114,9 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
     if extension.use_hip_lm(logits):
         if teacher_logits.dtype == torch.float64:
             teacher_logits = teacher_logits.float()
-        return DistillFn.apply(logits, teacher_index, teacher_logits.detach(),
-                               targets, float(alpha), float(temperature))
-    return _ref_distill(logits, teacher_index, teacher_logits, targets,
+        return extension.get_extension().distill_loss(
+            logits, teacher_index, teacher_logits.detach(), targets, alpha,
+            temperature, weight)
+    loss = _ref_distill(logits, teacher_index, teacher_logits, targets,
                         float(alpha), float(temperature))
+    return loss * weight

@@ -201,18 +201,18 @@ class Trainer:
             for wi, (wx, wy) in enumerate(wins):
                 out, state = self.model(wx, state)
                 state = self.model.detach_state(state)
+                scale = len(wins) * n_micro
                 if self.teacher is not None:
                     with torch.no_grad():
                         t_out, t_state = self.teacher(wx, t_state)
                     loss = self.model.distill_loss(
                         out, t_out, wy, cfg.train.distill_top_k,
                         cfg.train.distill_alpha,
-                        cfg.train.distill_temperature)
+                        cfg.train.distill_temperature, weight=1.0 / scale)
                 else:
                     loss = self.model.loss(out, wy)
-                scale = len(wins) * n_micro
-                if scale > 1:
-                    loss = loss / scale
+                    if scale > 1:
+                        loss = loss / scale
                 if self.bucketer is not None:
                     # grads accumulate across windows/micro-batches into the
                     # bucket buffers; only the LAST backward launches the

@@ -272,16 +272,22 @@ def test_kernel_strides():
 
 @pytest.mark.gpu
 def test_kernel_some_gradients_only():
-    t, rows, scale = make(20, 6, 80, 90, 8, 3, dtype=torch.bfloat16,
-                          dev="cuda")
-    full = check_on_gpu(t, rows, scale)
-    g = torch.Generator().manual_seed(99)
-    dy = torch.randn(t["y"].shape, generator=g).to(t["y"])
-    for name in "xab":
-        v = {n: p.clone().requires_grad_(n == name) for n, p in t.items()}
-        out = lowrank_add(**v, rows=rows, scale=scale)
-        got, = torch.autograd.grad(out, v[name], dy)
-        assert torch.equal(got, full[name])
+    for R in (8, 40):
+        t, rows, scale = make(20, 6, 80, 90, R, 3, dtype=torch.bfloat16,
+                              dev="cuda")
+        g = torch.Generator().manual_seed(99)
+        dy = torch.randn(t["y"].shape, generator=g).to(t["y"])
+        want, err = bounds(t, dy, rows, scale)
+        for names in ("x", "a", "b", "xa", "xb", "ab"):
+            v = {n: p.clone().requires_grad_(n in names)
+                 for n, p in t.items()}
+            out = lowrank_add(**v, rows=rows, scale=scale)
+            got = torch.autograd.grad(out, [v[n] for n in names], dy)
+            for n, p in zip(names, got):
+                assert ((p.double().cpu() - want[n]).abs() <= err[n]).all()
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(lowrank_add(**v, rows=rows, scale=scale),
+                                v["a"], dy, create_graph=True)
 
 
 @pytest.mark.gpu

@@ -135,6 +135,7 @@ def test_refusals():
             ((z, i, t, y), dict(alpha=math.nan)),
             ((z, i, t, y), dict(temperature=0.0)),
             ((z, i, t, y), dict(temperature=math.inf)),
+            ((z, i, t, y), dict(weight=math.nan)),
             ((z[:, :0], i, t, y), ok)]:
         with pytest.raises(ValueError):
             distill_loss(*args, **kw)
@@ -345,6 +346,37 @@ def test_kernel_captured_and_replayed():
         torch.cuda.synchronize()
         want = check_on_gpu(z2, i2, t2, y2, 0.5, 2.0)
         assert torch.equal(loss.detach(), want[0]) and torch.equal(g, want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [300, 9000, 40000, 57344, 57345])
+def test_kernel_weight_and_incoming_gradients(V, dtype):
+    """The gradient that the forward leaves (g = 1), the one that the backward
+    computes anew, and a kept graph's second and third pass."""
+    z, i, t, y = make(9, V, 12, seed=15, dtype=dtype, dev="cuda")
+    i[4, 1] = i[4, 0]
+    for tau in (1.0, 2.0, 3.0, 4.0):
+        _, one = check_on_gpu(z, i, t, y, 0.5, tau)
+        _, quarter = check_on_gpu(z, i, t, y, 0.5, tau, scale=0.25)
+        zs = z.clone().requires_grad_()
+        kw = dict(alpha=0.5, temperature=tau)
+        loss = distill_loss(zs, i, t, y, weight=0.25, **kw)
+        g = [torch.autograd.grad(loss, zs, retain_graph=True)[0]
+             for _ in range(2)]
+        full, = torch.autograd.grad(4.0 * loss, zs)
+        plain = distill_loss(z, i, t, y, **kw)
+        with torch.no_grad():
+            assert torch.equal(plain, distill_loss(zs, i, t, y, **kw))
+        assert abs(float(loss.detach()) - float(plain) / 4) <= \
+            2 ** -23 * abs(float(plain))
+        # the sums are the same: a factor of 4 moves only subnormal roundings
+        tiny = torch.finfo(dtype).smallest_normal
+        for a, b in ((g[0], quarter), (g[1], quarter), (full, one)):
+            assert ((a == b) | ((a - b).abs() <= tiny)).all()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(distill_loss(zs, i, t, y, alpha=0.5), zs,
+                            create_graph=True)
 
 
 @pytest.mark.gpu
