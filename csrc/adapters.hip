@@ -75,6 +75,14 @@ struct Rows {
     long T;
 };
 
+// Workgroups go round the eight XCDs by their number, each with an L2 of its own.  This order
+// hands an XCD neighbouring work: strips that share a line at their border (rows of an odd width
+// have no aligned ones) meet in one L2, also half-written.
+DEVINL int by_xcd() {
+    const int n = gridDim.x, b = blockIdx.x, x = b & 7, q = n >> 3, r = n & 7;
+    return x * q + (x < r ? x : r) + (b >> 3);
+}
+
 struct Scale {              // one number an adapter, or one for all
     const float* p;
     float all;
@@ -223,7 +231,7 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
             const long r = __shfl(row[m], src, 64);
             const int good = __shfl((int)ok[m], src, 64);
             if (!good) continue;
-            if (splits > 1) {
+            if (part) {
                 float* p = part + ((long)split * N + r) * (RT * 16) + (lane & 15);
 #pragma unroll
                 for (int t = 0; t < RT; ++t) p[t * 16] = acc[m][t][i];
@@ -236,27 +244,35 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
         }
 }
 
+// The shares summed in their order, scaled and rounded; four of a row's R a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ part, long N, int R16,
                                                     int splits, Rows rows, Scale scale,
                                                     T* __restrict__ V, int RP) {
+    typedef T out4 __attribute__((ext_vector_type(4)));
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= N * RP) return;
-    const long row = i / RP;
-    const int r = (int)(i % RP), l = rows.adapter[row % rows.Bn];
+    if (i >= N * (RP / 4)) return;
+    const long row = i / (RP / 4);
+    const int r = (int)(i % (RP / 4)) * 4, l = rows.adapter[(unsigned)row % (unsigned)rows.Bn];
     if (l < 0) return;
-    float s = 0.f;
-    if (r < R16)
-        for (int k = 0; k < splits; ++k) s += part[((long)k * N + row) * R16 + r];
-    V[i] = (T)(s * scale(l));
+    f32x4 s = f32x4{0, 0, 0, 0};
+    if (r < R16) {
+        const float* p = part + row * R16 + r;
+#pragma unroll 8
+        for (int k = 0; k < splits; ++k) s += *(const f32x4*)(p + (long)k * N * R16);
+    }
+    const float sc = scale(l);
+    *(out4*)(V + row * RP + r) = out4{(T)(s[0] * sc), (T)(s[1] * sc), (T)(s[2] * sc),
+                                      (T)(s[3] * sc)};
 }
 
 // ---------------------------------------------------------------------------
 // expand: out[row] = base[row] + V[row] W_l (base may be out itself, or absent: zero).  A wave
-// keeps W for 64 columns in registers and streams the workgroup's rows past it, 32 at a time and
-// 32 ahead.  W is the A operand and the rows are B's columns, so that a lane ends up with
-// neighbouring columns of one row; columns are dealt to the tiles' rows such that two tiles make
-// eight of them: column of tile t, MFMA row i = (t >> 1) * 32 + (i >> 2) * 8 + (t & 1) * 4 + (i & 3).
+// keeps W for 64 columns in registers and multiplies 32 of the workgroup's rows at a time.  W is
+// the A operand and the rows are B's columns, so that a lane holds four neighbouring columns of
+// one row; the products pass through LDS in fp32 to the lanes that hold base for whole rows of
+// 256 columns: read and written as 512 neighbouring bytes (in the operand's layout, 64 at a time,
+// rows of 50000 ran at 3.5 TB/s), loaded one step ahead.
 // ---------------------------------------------------------------------------
 template <typename T, int RK, bool RCONT>
 __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, long os,
@@ -265,13 +281,20 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, 
                                                 int strips, int shift) {
     typedef typename Frag<T>::type F;
     typedef typename Vec8<T>::type U8;
-    constexpr int LD = 256 + 16;
-    __shared__ __attribute__((aligned(16))) T wt[RCONT ? 8 : RK * 32 * LD];
+    constexpr int LD = 256 + 16, LS = 256 + 4;
+    constexpr int BYTES = RCONT || RK * 32 * LD * 2 < 32 * LS * 4 ? 32 * LS * 4 : RK * 32 * LD * 2;
+    __shared__ __attribute__((aligned(16))) char lds[BYTES];
+    __shared__ int at[256];                     // the tile's rows, divided out once
+    T* const wt = (T*)lds;                      // W, and when it is in registers
+    float* const sums = (float*)lds;            // the products
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-    const Tile f = find_tile(rows, blockIdx.x / strips, shift);
-    const int strip = blockIdx.x % strips * 256, m0 = strip + wave * 64;
+    const int block = by_xcd();
+    const Tile f = find_tile(rows, block / strips, shift);
+    const int strip = block % strips * 256, m0 = strip + wave * 64;
     const bool mine = f.adapter >= 0;
     if (!mine && base == out) return;           // nothing to add in place
+    const long jend = min(f.n, f.j0 + (1l << shift));
+    if (f.j0 + tid < jend) at[tid] = (int)row_of(rows, f, f.j0 + tid);
     F w[RK][4];
     if (mine) {
         const T* Wl = W + (long)f.adapter * M * R;
@@ -280,8 +303,7 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, 
             for (int k = 0; k < RK; ++k)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    const int i = lane & 15, r = k * 32 + g * 8;
-                    const int m = m0 + (t >> 1) * 32 + (i >> 2) * 8 + (t & 1) * 4 + (i & 3);
+                    const int m = m0 + t * 16 + (lane & 15), r = k * 32 + g * 8;
                     w[k][t] = load_frag(Wl + (long)m * R + r, m < M ? R - r : 0);
                 }
         } else {
@@ -291,76 +313,182 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, 
                 *(F*)(wt + r * LD + u % 32 * 8) =
                     load_frag(Wl + (long)r * M + m, r < R ? M - m : 0);
             }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < RK; ++k)
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    w[k][t] = column_frag(wt, LD, k * 32, wave * 64 + (t >> 1) * 32 +
-                                                              (lane & 3) * 8 + (t & 1) * 4);
         }
     }
-    if (m0 >= M) return;
-    const long jend = min(f.n, f.j0 + (1l << shift));
+    __syncthreads();
+    // a lane's share of base and out: eight columns of every eighth row
+    const int m = strip + (tid & 31) * 8;
+    const bool whole = m + 8 <= M;
+    U8 y[4];
+    auto load_base = [&](long j0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long j = j0 + i * 8 + (tid >> 5);
+            if (base && whole && j < jend) y[i] = *(const U8*)(base + at[j - f.j0] * bs + m);
+        }
+    };
     F v[2][RK];
-    U8 y[2][2];
-    long row[2];
-    auto load = [&](long j0) {
+    auto load_rows = [&](long j0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const long j = j0 + h * 16 + (lane & 15);
-            row[h] = row_of(rows, f, j < jend ? j : jend - 1);
-            if (mine)
+            const long row = at[(j < jend ? j : jend - 1) - f.j0];
 #pragma unroll
-                for (int k = 0; k < RK; ++k) v[h][k] = *(const F*)(V + row[h] * RP + k * 32 + g * 8);
-            if (base)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int m = m0 + c * 32 + g * 8;
-                    if (m + 8 <= M) y[h][c] = *(const U8*)(base + row[h] * bs + m);
-                }
+            for (int k = 0; k < RK; ++k) v[h][k] = *(const F*)(V + row * RP + k * 32 + g * 8);
         }
     };
-    load(f.j0);
+    load_base(f.j0);
+    if (mine) load_rows(f.j0);
+    if (mine && !RCONT) {
+#pragma unroll
+        for (int k = 0; k < RK; ++k)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                w[k][t] = column_frag(wt, LD, k * 32, wave * 64 + t * 16 + own_columns());
+    }
     for (long j0 = f.j0; j0 < jend; j0 += 32) {
         f32x4 acc[2][4];
-        U8 b[2][2];
-        long at[2];
+        U8 b[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            at[h] = row[h];
+        for (int i = 0; i < 4; ++i) b[i] = y[i];
+        if (mine) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) b[h][c] = y[h][c];
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                acc[h][t] = f32x4{0, 0, 0, 0};
-                if (mine)
+                for (int t = 0; t < 4; ++t) {
+                    acc[h][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int k = 0; k < RK; ++k) acc[h][t] = mfma(w[k][t], v[h][k], acc[h][t]);
+                }
+        }
+        if (j0 + 32 < jend) {
+            load_base(j0 + 32);
+            if (mine) load_rows(j0 + 32);
+        }
+        __syncthreads();                        // W, or the last step's products, are read
+        if (mine) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    *(f32x4*)(sums + (h * 16 + (lane & 15)) * LS + wave * 64 + t * 16 + g * 4) =
+                        acc[h][t];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = i * 8 + (tid >> 5);
+            if (j0 + n >= jend || m >= M) continue;
+            const long row = at[j0 + n - f.j0];
+            f32x4 lo = f32x4{0, 0, 0, 0}, hi = lo;
+            if (mine) {
+                lo = *(const f32x4*)(sums + n * LS + (tid & 31) * 8);
+                hi = *(const f32x4*)(sums + n * LS + (tid & 31) * 8 + 4);
+            }
+            if (whole) {
+                U8 o;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    o[q] = (T)((base ? (float)b[i][q] : 0.f) + (q < 4 ? lo[q & 3] : hi[q & 3]));
+                *(U8*)(out + row * os + m) = o;
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (m + q < M) {
+                        const float was = base ? (float)base[row * bs + m + q] : 0.f;
+                        out[row * os + m + q] = (T)(was + (q < 4 ? lo[q & 3] : hi[q & 3]));
+                    }
             }
         }
-        if (j0 + 32 < jend) load(j0 + 32);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The same for a decode step, where an adapter has a row or a few and its weights are most of
+// what is read: a wave takes 512 columns, eight a lane, and up to four rows, and multiplies W as
+// it comes, whole lines of one r, without staging.  The shares of V are summed here, which saves
+// the launch that does it elsewhere; V is rounded to the type all the same.
+// ---------------------------------------------------------------------------
+constexpr int FEW = 2;      // log2 rows a wave
+
+template <typename T>
+__global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* out, long os,
+                                                   const float* __restrict__ part, long N, int R16,
+                                                   int splits, Scale scale,
+                                                   const T* __restrict__ W, int M, int R,
+                                                   Rows rows, int strips) {
+    constexpr int NR = 1 << FEW, U = 16;
+    typedef typename Vec8<T>::type U8;
+    __shared__ float v[NR * 128];
+    const int lane = threadIdx.x;
+    const Tile f = find_tile(rows, blockIdx.x / strips, FEW);
+    const bool mine = f.adapter >= 0;
+    if (!mine && base == out) return;
+    const int n = (int)min((long)NR, f.n - f.j0), m = blockIdx.x % strips * 512 + lane * 8;
+    long row[NR];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (j0 + h * 16 + (lane & 15) >= jend) continue;
+    for (int i = 0; i < NR; ++i) row[i] = row_of(rows, f, f.j0 + (i < n ? i : 0));
+    float acc[NR][8] = {};
+    if (mine) {
+        const float sc = scale(f.adapter);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int m = m0 + c * 32 + g * 8;
-                if (m + 8 <= M) {
-                    U8 o;
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        o[q] = (T)((base ? (float)b[h][c][q] : 0.f) + acc[h][2 * c + (q >> 2)][q & 3]);
-                    *(U8*)(out + at[h] * os + m) = o;
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        if (m + q < M) {
-                            const float was = base ? (float)base[at[h] * bs + m + q] : 0.f;
-                            out[at[h] * os + m + q] = (T)(was + acc[h][2 * c + (q >> 2)][q & 3]);
-                        }
+        for (int i = 0; i < NR; ++i)
+            if (i < n)
+                for (int r = lane; r < R; r += 64) {
+                    float s = 0.f;
+                    for (int k = 0; k < splits; ++k) s += part[((long)k * N + row[i]) * R16 + r];
+                    v[i * 128 + r] = (float)(T)(s * sc);
                 }
+        __syncthreads();
+        const T* Wl = W + (long)f.adapter * M * R + m;
+        if (m + 8 <= M) {
+            int r0 = 0;
+            for (; r0 + U <= R; r0 += U) {
+                U8 w[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) w[u] = *(const U8*)(Wl + (long)(r0 + u) * M);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < NR; ++i)
+                        if (i < n)
+#pragma unroll
+                            for (int q = 0; q < 8; ++q)
+                                acc[i][q] += v[i * 128 + r0 + u] * (float)w[u][q];
             }
+            for (; r0 < R; ++r0) {
+                const U8 w = *(const U8*)(Wl + (long)r0 * M);
+#pragma unroll
+                for (int i = 0; i < NR; ++i)
+                    if (i < n)
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) acc[i][q] += v[i * 128 + r0] * (float)w[q];
+            }
+        } else {
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float w = m + q < M ? (float)Wl[(long)r * M + q] : 0.f;
+#pragma unroll
+                    for (int i = 0; i < NR; ++i)
+                        if (i < n) acc[i][q] += v[i * 128 + r] * w;
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        if (i >= n) continue;
+        if (m + 8 <= M) {
+            float y[8];
+            load8(base + row[i] * bs + m, y);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) y[q] += acc[i][q];
+            store8(out + row[i] * os + m, y);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (m + q < M)
+                    out[row[i] * os + m + q] = (T)((float)base[row[i] * bs + m + q] + acc[i][q]);
         }
     }
 }
@@ -370,123 +498,156 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, 
 // CT columns and walks the tile's rows 64 at a time: they pass through LDS as they are, and both
 // operands are read from there with their columns' rows side by side.
 //
-// DV: the rows meet W on the way too, partv[strip][row][r] = sum over the strip's columns of
-// P[row][p] W_l[r][p] -- the backward pass's u, in shares of 256 columns.  dy is then read once
-// for both; the shares cost 8 R bytes a row and strip (written, read again) beside the 512 of a
-// second reading of dy.
+// NS > 0: the rows meet W on the way too, partv[share][row][r] = sum over the workgroup's columns
+// of P[row][p] W_l[r][p] -- the backward pass's u, in shares of NS times as many columns.  dy is
+// then read once for both; a share costs 8 R bytes a row (written, read again), a second reading
+// of dy 128 CT NS.
 // ---------------------------------------------------------------------------
-template <typename T, int RT, int CT, bool DV>
+template <typename T, int RT, int CT, int NS>
 __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps, int NP,
                                                const T* __restrict__ Q, int RP,
                                                float* __restrict__ part,
                                                const T* __restrict__ W, int R,
                                                float* __restrict__ partv, long N, Rows rows,
-                                               int strips, int shift) {
+                                               int shares, int shift) {
     typedef typename Frag<T>::type F;
+    constexpr bool DV = NS > 0;
+    constexpr int C = DV ? NS : 1;                  // strips of PC columns
     constexpr int PC = 64 * CT, S = PC / 32, LP = PC + 16, LQ = RT * 16 + (RT >= 4 ? 16 : 0);
-    constexpr int LW = PC + 8;
+    constexpr int LW = C * PC + 8;
     __shared__ __attribute__((aligned(16))) T pt[64 * LP];
     __shared__ __attribute__((aligned(16))) T qt[64 * LQ];
     __shared__ __attribute__((aligned(16))) T wt[DV ? RT * 16 * LW : 8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-    const int tile = blockIdx.x / strips, strip = blockIdx.x % strips, p0 = strip * PC;
+    const int block = by_xcd(), tile = block / shares, share = block % shares;
+    const int p0 = share * C * PC;
     const Tile f = find_tile(rows, tile, shift);
     if (f.adapter < 0) return;
     if (DV) {
         const T* Wl = W + (long)f.adapter * NP * R;
-        for (int u = tid; u < RT * 16 * (PC / 8); u += 256) {
-            const int r = u / (PC / 8), c = u % (PC / 8) * 8;
+        for (int u = tid; u < RT * 16 * (C * PC / 8); u += 256) {
+            const int r = u / (C * PC / 8), c = u % (C * PC / 8) * 8;
             *(F*)(wt + r * LW + c) = load_frag(Wl + (long)r * NP + p0 + c, r < R ? NP - p0 - c : 0);
         }
     }
-    f32x4 acc[CT][RT];
+    f32x4 acc[C][CT][RT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
+    for (int k = 0; k < C; ++k)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[c][t] = f32x4{0, 0, 0, 0};
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[k][c][t] = f32x4{0, 0, 0, 0};
     const long jend = min(f.n, f.j0 + (1l << shift));
     constexpr int QV = (64 * RT * 2 + 255) / 256;       // vectors of Q a thread
-    F x[S], q[QV];
-    long row = 0;
-    bool ok = false;
-    auto load = [&](long j0) {
-        const long j = j0 + wave * 16 + (lane & 15);
-        ok = j < jend;
-        row = row_of(rows, f, ok ? j : jend - 1);
-        const T* xp = P + row * ps + p0 + g * 8;
+    constexpr int PV = 64 * PC / 8 / 256, PW = PC / 8;  // of P; a row's
+    F x[PV], q[QV];
+    // Rows of this step (for u), the next (loading) and the one behind it, divided out by one wave.
+    __shared__ int at[3][64];
+    auto find_rows = [&](long j0, int slot) {
+        const long k = j0 + lane;
+        if (wave == 3) at[slot][lane] = (int)row_of(rows, f, k < jend ? k : jend - 1);
+    };
+    find_rows(f.j0, 0);
+    find_rows(f.j0 + 64, 1);
+    __syncthreads();
+    int slot = 0;
+    // a row's columns side by side over the lanes: rows of an odd width straddle few lines
+    auto load = [&](long j0, int slot, int first) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) x[s] = load_frag(xp + s * 32, ok ? NP - p0 - s * 32 - g * 8 : 0);
+        for (int i = 0; i < PV; ++i) {
+            const int n = i * (256 / PW) + tid / PW, c = first + tid % PW * 8;
+            const long k = j0 + n, r = at[slot][n];
+            x[i] = load_frag(P + r * ps + c, k < jend ? NP - c : 0);
+        }
+    };
+    auto load_q = [&](long j0, int slot) {
 #pragma unroll
         for (int i = 0; i < QV; ++i) {
             const int u = i * 256 + tid, n = u / (RT * 2);
             if (n >= 64) continue;
-            const long k = j0 + n;
-            const long r = row_of(rows, f, k < jend ? k : jend - 1);
+            const long k = j0 + n, r = at[slot][n];
             q[i] = load_frag(Q + r * RP + u % (RT * 2) * 8, k < jend ? 8 : 0);
         }
     };
-    load(f.j0);
+    load(f.j0, 0, p0);
+    load_q(f.j0, 0);
     for (long j0 = f.j0; j0 < jend; j0 += 64) {
-        __syncthreads();
-        F now[S];
+        const int next = slot == 2 ? 0 : slot + 1, behind = next == 2 ? 0 : next + 1;
+        const bool more = j0 + 64 < jend;
+        f32x4 u[RT];
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            now[s] = x[s];
-            *(F*)(pt + (wave * 16 + (lane & 15)) * LP + s * 32 + g * 8) = x[s];
-        }
+        for (int t = 0; t < RT; ++t) u[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < QV; ++i) {
-            const int u = i * 256 + tid, n = u / (RT * 2);
-            if (n < 64) *(F*)(qt + n * LQ + u % (RT * 2) * 8) = q[i];
-        }
-        const long at = row;
-        const bool good = ok;
-        __syncthreads();
-        if (j0 + 64 < jend) load(j0 + 64);
-        if (DV) {
-            f32x4 u[RT];
+        for (int k = 0; k < C; ++k) {
+            __syncthreads();
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                u[t] = f32x4{0, 0, 0, 0};
+            for (int i = 0; i < PV; ++i)
+                *(F*)(pt + (i * (256 / PW) + tid / PW) * LP + tid % PW * 8) = x[i];
+            if (k == 0)
 #pragma unroll
-                for (int s = 0; s < S; ++s)
-                    u[t] = mfma(now[s], *(const F*)(wt + (t * 16 + (lane & 15)) * LW + s * 32 +
-                                                    g * 8), u[t]);
+                for (int i = 0; i < QV; ++i) {
+                    const int u = i * 256 + tid, n = u / (RT * 2);
+                    if (n < 64) *(F*)(qt + n * LQ + u % (RT * 2) * 8) = q[i];
+                }
+            __syncthreads();
+            if (k + 1 < C) {
+                load(j0, slot, p0 + (k + 1) * PC);
+            } else if (more) {
+                load(j0 + 64, next, p0);
+                load_q(j0 + 64, next);
             }
+            if (DV) {           // a wave takes 16 of the rows
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const long r = __shfl(at, g * 4 + i, 64);
-                if (__shfl((int)good, g * 4 + i, 64))
+                for (int s = 0; s < S; ++s) {
+                    const F a = *(const F*)(pt + (wave * 16 + (lane & 15)) * LP + s * 32 + g * 8);
 #pragma unroll
                     for (int t = 0; t < RT; ++t)
-                        partv[((long)strip * N + r) * (RT * 16) + t * 16 + (lane & 15)] = u[t][i];
+                        u[t] = mfma(a, *(const F*)(wt + (t * 16 + (lane & 15)) * LW + k * PC +
+                                                   s * 32 + g * 8), u[t]);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                F b[RT];
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    b[t] = column_frag(qt, LQ, s * 32, t * 16 + own_columns());
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const F a = column_frag(pt, LP, s * 32, (wave * CT + c) * 16 + own_columns());
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) acc[k][c][t] = mfma(a, b[t], acc[k][c][t]);
+                }
             }
         }
+        if (DV) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            F b[RT];
+            for (int i = 0; i < 4; ++i) {
+                const int n = wave * 16 + g * 4 + i;
+                if (j0 + n >= jend) continue;
+                float* v = partv + ((long)share * N + at[slot][n]) * (RT * 16) + (lane & 15);
 #pragma unroll
-            for (int t = 0; t < RT; ++t) b[t] = column_frag(qt, LQ, s * 32, t * 16 + own_columns());
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                const F a = column_frag(pt, LP, s * 32, (wave * CT + c) * 16 + own_columns());
-#pragma unroll
-                for (int t = 0; t < RT; ++t) acc[c][t] = mfma(a, b[t], acc[c][t]);
+                for (int t = 0; t < RT; ++t) v[t * 16] = u[t][i];
             }
         }
+        find_rows(j0 + 128, behind);
+        slot = next;
     }
+    const int LO = shares * C * PC;
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
+    for (int k = 0; k < C; ++k)
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
-            *(f32x4*)(part + ((long)tile * RT * 16 + t * 16 + (lane & 15)) * (strips * PC) + p0 +
-                      (wave * CT + c) * 16 + g * 4) = acc[c][t];
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+                *(f32x4*)(part + ((long)tile * RT * 16 + t * 16 + (lane & 15)) * LO + p0 + k * PC +
+                          (wave * CT + c) * 16 + g * 4) = acc[k][c][t];
 }
 
 // The weights' gradient: an adapter's tiles in a fixed order, rounded once.  An adapter without
-// rows gets zeros.  out is (L, R, NP) or, RCONT, (L, NP, R).  32 lanes take 128 columns of one r,
-// eight groups share the tiles.
-template <typename T, bool RCONT>
+// rows gets zeros.  out is (L, R, NP) or, RCONT, (L, NP, R).  A thread takes four columns of one
+// r; GR groups of threads share the tiles where there are many.
+template <typename T, bool RCONT, int GR>
 __global__ __launch_bounds__(256) void k_outer_sum(const float* __restrict__ part, int R16, int LP,
                                                    Rows rows, int shift, T* __restrict__ out,
                                                    int NP, int R, int blocks) {
@@ -511,19 +672,24 @@ __global__ __launch_bounds__(256) void k_outer_sum(const float* __restrict__ par
         }
         base += __shfl(sum, 63, 64);
     }
-    __shared__ f32x4 sums[256];
-    const int b = blockIdx.x % blocks, cols = (NP + 127) / 128;
-    const int r = b / cols, p = b % cols * 128 + (threadIdx.x & 31) * 4, group = threadIdx.x >> 5;
+    constexpr int TH = 256 / GR;
+    __shared__ f32x4 sums[GR > 1 ? 256 : 1];
+    const int b = blockIdx.x % blocks, cols = (NP + TH * 4 - 1) / (TH * 4);
+    const int r = b / cols, group = threadIdx.x / TH;
+    const int p = (b % cols * TH + threadIdx.x % TH) * 4;
     f32x4 s = f32x4{0, 0, 0, 0};
-    const float* q = part + (long)r * LP + p;       // LP is a multiple of 128
+    const float* q = part + (long)r * LP + p;       // LP >= NP is a multiple of four
+    if (p < NP)
 #pragma unroll 4
-    for (int t = first + group; t < first + tiles; t += 8)
-        s += *(const f32x4*)(q + (long)t * R16 * LP);
-    sums[threadIdx.x] = s;
-    __syncthreads();
-    if (group) return;
+        for (int t = first + group; t < first + tiles; t += GR)
+            s += *(const f32x4*)(q + (long)t * R16 * LP);
+    if (GR > 1) {
+        sums[threadIdx.x] = s;
+        __syncthreads();
+        if (group) return;
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sums[k * 32 + threadIdx.x];
+        for (int k = 1; k < GR; ++k) s += sums[k * TH + threadIdx.x];
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (p + j < NP)
@@ -567,30 +733,39 @@ void expand(const void* base, long bs, void* out, long os, const void* V, int RP
 #undef GO
 }
 
-// Columns that a workgroup of outer owns: 256, or 128 where a rank of 128 fills the registers.
-int outer_columns(int R) { return R > 64 ? 128 : 256; }
+// Columns that a workgroup of outer owns: 256, or 128 where a rank of 128 fills the registers;
+// 1024 or 512 of those whose u it sums, as many as the accumulators leave room for.
+int outer_columns(int R, int with_u) {
+    return R > 64 ? 128 : !with_u ? 256 : R <= 16 ? 1024 : 512;
+}
 
 template <typename T, bool RCONT>
 void outer(const void* P, long ps, int NP, const void* Q, int RP, float* part, const void* W,
            float* partv, long N, const Rows& rows, int tiles, int shift, void* out, int R, int L,
            hipStream_t st) {
-    const int PC = outer_columns(R), strips = (NP + PC - 1) / PC, R16 = r16_of(R);
-#define GO(RT, CT, DV)                                                                           \
-    k_outer<T, RT, CT, DV><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
+    const int PC = outer_columns(R, W != nullptr), strips = (NP + PC - 1) / PC, R16 = r16_of(R);
+#define GO(RT, CT, NS)                                                                           \
+    k_outer<T, RT, CT, NS><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
         (const T*)P, ps, NP, (const T*)Q, RP, part, (const T*)W, R, partv, N, rows, strips, shift)
     if (tiles == 0) {           // no row has an adapter: the sum below writes zeros
     } else if (R16 == 16) {
-        if (W) GO(1, 4, true);
-        else GO(1, 4, false);
+        if (W) GO(1, 4, 4);
+        else GO(1, 4, 0);
     } else if (R16 == 32) {
-        if (W) GO(2, 4, true);
-        else GO(2, 4, false);
-    } else if (R16 == 64) GO(4, 4, false);
-    else GO(8, 2, false);
+        if (W) GO(2, 4, 2);
+        else GO(2, 4, 0);
+    } else if (R16 == 64) GO(4, 4, 0);
+    else GO(8, 2, 0);
 #undef GO
-    const int blocks = (NP + 127) / 128 * R;
-    k_outer_sum<T, RCONT><<<(unsigned)L * blocks, 256, 0, st>>>(
-        part, R16, strips * PC, rows, shift, (T*)out, NP, R, blocks);
+    if (tiles > 4 * L) {
+        const int blocks = (NP + 127) / 128 * R;
+        k_outer_sum<T, RCONT, 8><<<(unsigned)L * blocks, 256, 0, st>>>(
+            part, R16, strips * PC, rows, shift, (T*)out, NP, R, blocks);
+    } else {
+        const int blocks = (NP + 1023) / 1024 * R;
+        k_outer_sum<T, RCONT, 1><<<(unsigned)L * blocks, 256, 0, st>>>(
+            part, R16, strips * PC, rows, shift, (T*)out, NP, R, blocks);
+    }
 }
 
 }  // namespace
@@ -607,7 +782,7 @@ int lowrank_splits(const long* counts, int S, long T, int K) {
     return want < 1 ? 1 : want > most ? most : want;
 }
 
-// `part` (splits, N, R16) is left unsummed for launch_shrink_sum where splits > 1.
+// With `part` (splits, N, R16) the shares are left there unscaled and V is not written.
 void launch_shrink(int type, int kcont, const void* X, long xs, const void* W, int K, int R,
                    const int* order, const int* segs, const int* adapter, const long* counts,
                    int S, int Bn, long T, const float* scale, float scale_all, void* V,
@@ -637,7 +812,7 @@ void launch_shrink_sum(int type, int R, const int* order, const int* segs, const
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const Scale sc{scale, scale_all};
     const int RP = lowrank_rp(R), R16 = r16_of(R);
-    const long N = T * Bn, blocks = (N * RP + 255) / 256;
+    const long N = T * Bn, blocks = (N * (RP / 4) + 255) / 256;
     if (type == LM_BF16)
         k_shrink_sum<bf16_t><<<(unsigned)blocks, 256, 0, st>>>(part, N, R16, splits, rows, sc,
                                                                (bf16_t*)V, RP);
@@ -665,11 +840,39 @@ void launch_expand(int type, int rcont, const void* base, long bs, void* out, lo
               : expand<f16_t, false>(base, bs, out, os, V, RP, W, M, R, rows, tiles, shift, st);
 }
 
-int lowrank_strips(int NP, int R) { return (NP + outer_columns(R) - 1) / outer_columns(R); }
+// A decode step: no adapter has so many rows that W would pass more than four times.
+int lowrank_few(const long* counts, int S, long T) {
+    for (int s = 0; s < S; ++s)
+        if (T * counts[s] > 4 << FEW) return 0;
+    return 1;
+}
+
+void launch_expand_few(int type, const void* base, long bs, void* out, long os, const float* part,
+                       const void* W, int M, int R, const int* order, const int* segs,
+                       const int* adapter, const long* counts, int S, int Bn, long T,
+                       const float* scale, float scale_all, int splits, hipStream_t st) {
+    const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
+    const Scale sc{scale, scale_all};
+    const int tiles = tiles_of(counts, S, T, FEW), strips = (M + 511) / 512, R16 = r16_of(R);
+    const long N = T * Bn;
+    if (type == LM_BF16)
+        k_expand_few<bf16_t><<<(unsigned)tiles * strips, 64, 0, st>>>(
+            (const bf16_t*)base, bs, (bf16_t*)out, os, part, N, R16, splits, sc,
+            (const bf16_t*)W, M, R, rows, strips);
+    else
+        k_expand_few<f16_t><<<(unsigned)tiles * strips, 64, 0, st>>>(
+            (const f16_t*)base, bs, (f16_t*)out, os, part, N, R16, splits, sc, (const f16_t*)W, M,
+            R, rows, strips);
+}
+
+int lowrank_strips(int NP, int R, int with_u) {
+    const int PC = outer_columns(R, with_u);
+    return (NP + PC - 1) / PC;
+}
 // log2 of the rows that one partial gradient sums: about four workgroups a CU over the strips,
 // never fewer than 64 rows (a step) nor more than 4096.
-int lowrank_outer_shift(const long* counts, int S, long T, int NP, int R) {
-    const long strips = lowrank_strips(NP, R);
+int lowrank_outer_shift(const long* counts, int S, long T, int NP, int R, int with_u) {
+    const long strips = lowrank_strips(NP, R, with_u);
     int shift = 12;
     while (shift > 6 && tiles_of(counts, S, T, shift) * strips < 1024) --shift;
     return shift;

@@ -25,8 +25,12 @@ void launch_adjust(int, const void*, long, void*, const void*, long, int, int, c
                    long, int, hipStream_t);
 int lowrank_rp(int R);
 int lowrank_splits(const long* counts, int S, long T, int K);
-int lowrank_strips(int NP, int R);
-int lowrank_outer_shift(const long* counts, int S, long T, int NP, int R);
+int lowrank_strips(int NP, int R, int with_u);
+int lowrank_outer_shift(const long* counts, int S, long T, int NP, int R, int with_u);
+int lowrank_few(const long* counts, int S, long T);
+void launch_expand_few(int, const void*, long, void*, long, const float*, const void*, int, int,
+                       const int*, const int*, const int*, const long*, int, int, long,
+                       const float*, float, int, hipStream_t);
 int lowrank_outer_tiles(const long* counts, int S, long T, int shift);
 int lowrank_one_reading(int R);
 void launch_shrink(int, int, const void*, long, const void*, int, int, const int*, const int*,
@@ -339,6 +343,20 @@ struct Grouped {
         launch_shrink_sum(type, R, ip(order), ip(segs), ip(adapter), S, Bn, T, float_ptr(scale),
                           scale_all, v.data_ptr(), (const float*)part.data_ptr(), splits, st);
     }
+    // out = base + s x A B of a few rows an adapter, in two launches
+    void few(const Tensor& base, Tensor& out, const Tensor& x, const Tensor& a, const Tensor& b,
+             hipStream_t st) const {
+        const int splits = lowrank_splits(counts.data(), S, T, K);
+        auto part = at::empty({(long)splits * N * lowrank_rp(R)}, x.options().dtype(at::kFloat));
+        launch_shrink(type, 0, x.data_ptr(), row_stride(x), a.data_ptr(), K, R, ip(order),
+                      ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
+                      nullptr, (float*)part.data_ptr(), st);
+        launch_expand_few(type, base.data_ptr(), row_stride(base), out.data_ptr(),
+                          row_stride(out), (const float*)part.data_ptr(), b.data_ptr(), M, R,
+                          ip(order), ip(segs), ip(adapter), counts.data(), S, Bn, T,
+                          float_ptr(scale), scale_all, splits, st);
+        check_launch("lowrank few");
+    }
     // out = base + v W, W (L, R, M) or, rank contiguous, (L, M, R)
     void expand(const Tensor& base, Tensor& out, const Tensor& v, const Tensor& w, bool rcont,
                 hipStream_t st) const {
@@ -352,11 +370,12 @@ struct Grouped {
     // (L, R, NP) also `u` (N, RP) = s p w^T, from the same reading of p.
     Tensor outer(const Tensor& p, const Tensor& q, bool rcont, hipStream_t st,
                  const Tensor& w = Tensor(), Tensor* u = nullptr) const {
-        const int np = (int)p.size(1), strips = lowrank_strips(np, R), rp = lowrank_rp(R);
-        const int shift = lowrank_outer_shift(counts.data(), S, T, np, R);
+        const int np = (int)p.size(1), strips = lowrank_strips(np, R, u != nullptr);
+        const int rp = lowrank_rp(R);
+        const int shift = lowrank_outer_shift(counts.data(), S, T, np, R, u != nullptr);
         const long tiles = lowrank_outer_tiles(counts.data(), S, T, shift);
         const auto f32 = p.options().dtype(at::kFloat);
-        auto part = at::empty({tiles * rp * strips * 256l}, f32);
+        auto part = at::empty({tiles * rp * strips * (u ? 1024l : 256l)}, f32);
         Tensor partv;
         if (u) partv = at::empty({strips * N * rp}, f32);
         auto out = rcont ? at::empty({L, np, R}, p.options()) : at::empty({L, R, np}, p.options());
@@ -373,14 +392,22 @@ struct Grouped {
     }
 };
 
-// y + s x A B, y and x of any leading shape over rows of Bn columns; `v` for the backward pass.
+// y + s x A B, y and x of any leading shape over rows of Bn columns; `v`, where it is asked for,
+// is x A for the backward pass.
 Tensor lowrank_forward(const Grouped& g, const Tensor& y, const Tensor& x, const Tensor& a,
                        const Tensor& b, bool inplace, Tensor* v) {
     const hipStream_t st = stream_of(x);
     Tensor out = inplace ? y : at::empty(y.sizes(), y.options());
     Tensor rows = out.view({g.N, (long)g.M});
-    *v = g.shrink(rows_of(x.reshape({g.N, (long)g.K})), a, false, st);
-    g.expand(inplace ? rows : rows_of(y.reshape({g.N, (long)g.M})), rows, *v, b, false, st);
+    const Tensor base = inplace ? rows : rows_of(y.reshape({g.N, (long)g.M}));
+    const Tensor xr = rows_of(x.reshape({g.N, (long)g.K}));
+    if (!v && lowrank_few(g.counts.data(), g.S, g.T)) {
+        g.few(base, rows, xr, a, b, st);
+        return out;
+    }
+    const Tensor made = g.shrink(xr, a, false, st);
+    g.expand(base, rows, made, b, false, st);
+    if (v) *v = made;
     return out;
 }
 
@@ -446,8 +473,7 @@ Tensor lowrank_add(Tensor y, Tensor x, Tensor a, Tensor b, Tensor order, Tensor 
     const Tensor ac = a.contiguous(), bc = b.contiguous();
     const Grouped g(x, y, ac, bc, order, segs, adapter, counts, scale, scale_all);
     TORCH_CHECK(!inplace || y.is_contiguous(), "lowrank: y must be contiguous");
-    Tensor v;
-    return lowrank_forward(g, y, x, ac, bc, inplace, &v);
+    return lowrank_forward(g, y, x, ac, bc, inplace, nullptr);
 }
 
 }  // namespace

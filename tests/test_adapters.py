@@ -169,6 +169,9 @@ def check_on_gpu(t, rows, scale, grad=True):
         assert p.dtype == t["x"].dtype and p.shape == want[n].shape
         off = (p.detach().double().cpu() - want[n]).abs()
         assert (off <= err[n]).all(), (n, float((off / err[n]).max()))
+    with torch.no_grad():       # nothing kept for a backward pass
+        plain = lowrank_add(**t, rows=rows, scale=scale)
+    assert (plain.double().cpu() - want["out"]).abs().le(err["out"]).all()
     y = t["y"].detach().clone()
     lowrank_add_(y, *(t[n] for n in "xab"), rows=rows, scale=scale)
     assert (y.double().cpu() - want["out"]).abs().le(err["out"]).all()
