@@ -35,18 +35,25 @@ DEVINL f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Eight neighbours of which `left` exist; the others are zero.
-template <typename T> DEVINL typename Frag<T>::type load_frag(const T* p, int left) {
-    typename Frag<T>::type v;
-    if (left >= 8) {
-        const auto u = *(const typename Vec8<T>::type*)p;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = u[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : (T)0.f;
-    }
-    return v;
+// Eight neighbours from element e of a matrix that has `limit` elements, without a branch: near
+// the very end the last eight are taken, and `trim` shifts them into place.  Loads that differ
+// from lane to lane in their form would wait for each other at the point where they join.
+template <typename T> DEVINL typename Frag<T>::type eight(const T* p, long e, long limit) {
+    return __builtin_bit_cast(typename Frag<T>::type,
+                              *(const typename Vec8<T>::type*)(p + min(e, limit - 8)));
+}
+// What `eight` gave for element e, with zeros for all but the first `left`.
+template <typename F> DEVINL F trim(F v, long e, long limit, int left) {
+    typedef unsigned long long u2 __attribute__((ext_vector_type(2)));
+    u2 u = __builtin_bit_cast(u2, v);
+    const int over = (int)(e - min(e, limit - 8)), s = over * 16;
+    if (over >= 8) u = u2{0, 0};
+    else if (s >= 64) u = u2{u[1] >> (s - 64), 0};
+    else if (s > 0) u = u2{u[0] >> s | u[1] << (64 - s), u[1] >> s};
+    const int keep = min(max(left, 0), 8) * 16;
+    if (keep < 64) u = u2{u[0] & ((1ull << keep) - 1), 0};
+    else if (keep < 128) u = u2{u[0], u[1] & ((1ull << (keep - 64)) - 1)};
+    return __builtin_bit_cast(F, u);
 }
 
 // An operand whose contraction runs down the rows of an LDS tile: column c (lane & 15) of rows
@@ -143,9 +150,9 @@ constexpr int S_TM = 7;     // log2 rows a workgroup
 constexpr int S_KC = 128;   // contraction a step
 
 template <typename T, int RT, bool KCONT>
-__global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs,
-                                                const T* __restrict__ W, int K, int R, Rows rows,
-                                                Scale scale, T* __restrict__ V, int RP,
+__global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs, long xlimit,
+                                                const T* __restrict__ W, long wlimit, int K, int R,
+                                                Rows rows, Scale scale, T* __restrict__ V, int RP,
                                                 float* __restrict__ part, long N, int splits,
                                                 int kper) {
     typedef typename Frag<T>::type F;
@@ -156,17 +163,15 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
     const int split = blockIdx.x % splits;
     const Tile f = find_tile(rows, blockIdx.x / splits, S_TM);
     if (f.adapter < 0) return;
-    const T* Wl = W + (long)f.adapter * K * R;
+    const long wl = (long)f.adapter * K * R;
     const int kend = min(K, (split + 1) * kper);
     long row[2];
     bool ok[2];
-    const T* xp[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         const long j = f.j0 + wave * 32 + m * 16 + (lane & 15);
         ok[m] = j < f.n;
         row[m] = row_of(rows, f, ok[m] ? j : f.n - 1);
-        xp[m] = X + row[m] * xs;
     }
     f32x4 acc[2][RT];
 #pragma unroll
@@ -175,40 +180,53 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
         for (int t = 0; t < RT; ++t) acc[m][t] = f32x4{0, 0, 0, 0};
 
     F x[2][4], wv[RT];      // RT * 16 * 128 elements of the panel: RT vectors a thread
+    // element of W that vector i starts with, and how many of it belong to the panel
+    auto of_panel = [&](int i, int k0, int& left) {
+        const int u = i * 256 + tid;
+        if (KCONT) {
+            const int r = u / (S_KC / 8), k = k0 + u % (S_KC / 8) * 8;
+            left = r < R ? kend - k : 0;
+            return wl + (long)r * K + k;
+        }
+        const int k = k0 + u / (RT * 2), r = u % (RT * 2) * 8;
+        left = k < kend ? R - r : 0;
+        return wl + (long)k * R + r;
+    };
     auto load = [&](int k0) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int k = k0 + s * 32 + (lane >> 4) * 8;
-                x[m][s] = load_frag(xp[m] + k, kend - k);
-            }
+            for (int s = 0; s < 4; ++s)
+                x[m][s] = eight(X, row[m] * xs + k0 + s * 32 + (lane >> 4) * 8, xlimit);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            const int u = i * 256 + tid;
-            if (KCONT) {
-                const int r = u / (S_KC / 8), k = k0 + u % (S_KC / 8) * 8;
-                wv[i] = load_frag(Wl + (long)r * K + k, r < R ? kend - k : 0);
-            } else {
-                const int k = k0 + u / (RT * 2), r = u % (RT * 2) * 8;
-                wv[i] = load_frag(Wl + (long)k * R + r, k < kend ? R - r : 0);
-            }
+            int left;
+            wv[i] = eight(W, of_panel(i, k0, left), wlimit);
         }
     };
     int k0 = split * kper;
     if (k0 < kend) load(k0);
     for (; k0 < kend; k0 += S_KC) {
+        const bool tail = k0 + S_KC > kend;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             const int u = i * 256 + tid, n = KCONT ? S_KC / 8 : RT * 2;
+            if (tail || R != RT * 16) {
+                int left;
+                const long e = of_panel(i, k0, left);
+                wv[i] = trim(wv[i], e, wlimit, left);
+            }
             *(F*)(w + u / n * LD + u % n * 8) = wv[i];
         }
         F now[2][4];
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) now[m][s] = x[m][s];
+            for (int s = 0; s < 4; ++s) {
+                const int k = k0 + s * 32 + (lane >> 4) * 8;
+                now[m][s] = tail ? trim(x[m][s], row[m] * xs + k, xlimit, kend - k) : x[m][s];
+            }
         __syncthreads();
         if (k0 + S_KC < kend) load(k0 + S_KC);
 #pragma unroll
@@ -275,10 +293,10 @@ __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ pa
 // rows of 50000 ran at 3.5 TB/s), loaded one step ahead.
 // ---------------------------------------------------------------------------
 template <typename T, int RK, bool RCONT>
-__global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, long os,
-                                                const T* __restrict__ V, int RP,
-                                                const T* __restrict__ W, int M, int R, Rows rows,
-                                                int strips, int shift) {
+__global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long blimit, T* out,
+                                                long os, const T* __restrict__ V, int RP,
+                                                const T* __restrict__ W, long wlimit, int M, int R,
+                                                Rows rows, int strips, int shift) {
     typedef typename Frag<T>::type F;
     typedef typename Vec8<T>::type U8;
     constexpr int LD = 256 + 16, LS = 256 + 4;
@@ -297,21 +315,29 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, 
     if (f.j0 + tid < jend) at[tid] = (int)row_of(rows, f, f.j0 + tid);
     F w[RK][4];
     if (mine) {
-        const T* Wl = W + (long)f.adapter * M * R;
+        const long wl = (long)f.adapter * M * R;
         if (RCONT) {
 #pragma unroll
             for (int k = 0; k < RK; ++k)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     const int m = m0 + t * 16 + (lane & 15), r = k * 32 + g * 8;
-                    w[k][t] = load_frag(Wl + (long)m * R + r, m < M ? R - r : 0);
+                    const long e = wl + (long)m * R + r;
+                    w[k][t] = trim(eight(W, e, wlimit), e, wlimit, m < M ? R - r : 0);
                 }
         } else {
+            F v[RK * 4];
+#pragma unroll
+            for (int i = 0; i < RK * 4; ++i) {
+                const int u = i * 256 + tid;
+                v[i] = eight(W, wl + (long)(u / 32) * M + strip + u % 32 * 8, wlimit);
+            }
 #pragma unroll
             for (int i = 0; i < RK * 4; ++i) {
                 const int u = i * 256 + tid, r = u / 32, m = strip + u % 32 * 8;
-                *(F*)(wt + r * LD + u % 32 * 8) =
-                    load_frag(Wl + (long)r * M + m, r < R ? M - m : 0);
+                if (R != RK * 32 || strip + 256 > M)
+                    v[i] = trim(v[i], wl + (long)r * M + m, wlimit, r < R ? M - m : 0);
+                *(F*)(wt + r * LD + u % 32 * 8) = v[i];
             }
         }
     }
@@ -319,12 +345,13 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, 
     // a lane's share of base and out: eight columns of every eighth row
     const int m = strip + (tid & 31) * 8;
     const bool whole = m + 8 <= M;
-    U8 y[4];
+    F y[4];
     auto load_base = [&](long j0) {
+        if (!base) return;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const long j = j0 + i * 8 + (tid >> 5);
-            if (base && whole && j < jend) y[i] = *(const U8*)(base + at[j - f.j0] * bs + m);
+            y[i] = eight(base, at[(j < jend ? j : jend - 1) - f.j0] * bs + m, blimit);
         }
     };
     F v[2][RK];
@@ -348,7 +375,7 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, 
     }
     for (long j0 = f.j0; j0 < jend; j0 += 32) {
         f32x4 acc[2][4];
-        U8 b[4];
+        F b[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) b[i] = y[i];
         if (mine) {
@@ -392,12 +419,12 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, T* out, 
                     o[q] = (T)((base ? (float)b[i][q] : 0.f) + (q < 4 ? lo[q & 3] : hi[q & 3]));
                 *(U8*)(out + row * os + m) = o;
             } else {
+                const F was = trim(b[i], row * bs + m, blimit, M - m);
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    if (m + q < M) {
-                        const float was = base ? (float)base[row * bs + m + q] : 0.f;
-                        out[row * os + m + q] = (T)(was + (q < 4 ? lo[q & 3] : hi[q & 3]));
-                    }
+                    if (m + q < M)
+                        out[row * os + m + q] =
+                            (T)((base ? (float)was[q] : 0.f) + (q < 4 ? lo[q & 3] : hi[q & 3]));
             }
         }
     }
@@ -424,66 +451,74 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
     const Tile f = find_tile(rows, blockIdx.x / strips, FEW);
     const bool mine = f.adapter >= 0;
     if (!mine && base == out) return;
-    const int n = (int)min((long)NR, f.n - f.j0), m = blockIdx.x % strips * 512 + lane * 8;
+    const int n = (int)min((long)NR, f.n - f.j0), own = blockIdx.x % strips * 512 + lane * 8;
+    // The last lane of an odd width takes the last eight columns, and stores those that are its
+    // own; lanes behind it take them too and store nothing.
+    const bool whole = M >= 8;
+    const int m = whole && own > M - 8 ? M - 8 : own;
     long row[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) row[i] = row_of(rows, f, f.j0 + (i < n ? i : 0));
     float acc[NR][8] = {};
+    U8 y[NR], w[U];
+    // base and the first of W are on their way before V is known
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+        if (whole && i < n) y[i] = *(const U8*)(base + row[i] * bs + m);
     if (mine) {
-        const float sc = scale(f.adapter);
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-            if (i < n)
-                for (int r = lane; r < R; r += 64) {
-                    float s = 0.f;
-                    for (int k = 0; k < splits; ++k) s += part[((long)k * N + row[i]) * R16 + r];
-                    v[i * 128 + r] = (float)(T)(s * sc);
-                }
-        __syncthreads();
         const T* Wl = W + (long)f.adapter * M * R + m;
-        if (m + 8 <= M) {
-            int r0 = 0;
-            for (; r0 + U <= R; r0 += U) {
-                U8 w[U];
+        auto load = [&](int r0) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) w[u] = *(const U8*)(Wl + (long)(r0 + u) * M);
+            for (int u = 0; u < U; ++u)
+                if (whole && r0 + u < R) w[u] = *(const U8*)(Wl + (long)(r0 + u) * M);
+        };
+        load(0);
+        const float sc = scale(f.adapter);
+        for (int u = lane; u < n * R16; u += 64) {
+            const int i = u / R16, r = u - i * R16;
+            const float* p = part + row_of(rows, f, f.j0 + i) * R16 + r;
+            float s = 0.f;
+#pragma unroll 8
+            for (int k = 0; k < splits; ++k) s += p[(long)k * N * R16];
+            v[i * 128 + r] = (float)(T)(s * sc);
+        }
+        __syncthreads();
+        if (whole) {
+            for (int r0 = 0; r0 < R; r0 += U) {
+                if (r0) load(r0);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
+                    if (r0 + u < R)
 #pragma unroll
-                    for (int i = 0; i < NR; ++i)
-                        if (i < n)
+                        for (int i = 0; i < NR; ++i)
+                            if (i < n)
 #pragma unroll
-                            for (int q = 0; q < 8; ++q)
-                                acc[i][q] += v[i * 128 + r0 + u] * (float)w[u][q];
+                                for (int q = 0; q < 8; ++q)
+                                    acc[i][q] += v[i * 128 + r0 + u] * (float)w[u][q];
             }
-            for (; r0 < R; ++r0) {
-                const U8 w = *(const U8*)(Wl + (long)r0 * M);
-#pragma unroll
-                for (int i = 0; i < NR; ++i)
-                    if (i < n)
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) acc[i][q] += v[i * 128 + r0] * (float)w[q];
-            }
-        } else {
+        } else if (m < M) {
             for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    const float w = m + q < M ? (float)Wl[(long)r * M + q] : 0.f;
+                    const float x = m + q < M ? (float)Wl[(long)r * M + q] : 0.f;
 #pragma unroll
                     for (int i = 0; i < NR; ++i)
-                        if (i < n) acc[i][q] += v[i * 128 + r] * w;
+                        if (i < n) acc[i][q] += v[i * 128 + r] * x;
                 }
         }
     }
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
         if (i >= n) continue;
-        if (m + 8 <= M) {
-            float y[8];
-            load8(base + row[i] * bs + m, y);
+        if (whole) {
+            float o[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) y[q] += acc[i][q];
-            store8(out + row[i] * os + m, y);
+            for (int q = 0; q < 8; ++q) o[q] = (float)y[i][q] + acc[i][q];
+            if (m == own) store8(out + row[i] * os + m, o);
+            else
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (m + q >= own) out[row[i] * os + m + q] = (T)o[q];
         } else {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
@@ -504,10 +539,10 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
 // of dy 128 CT NS.
 // ---------------------------------------------------------------------------
 template <typename T, int RT, int CT, int NS>
-__global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps, int NP,
-                                               const T* __restrict__ Q, int RP,
+__global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps, long plimit,
+                                               int NP, const T* __restrict__ Q, int RP,
                                                float* __restrict__ part,
-                                               const T* __restrict__ W, int R,
+                                               const T* __restrict__ W, long wlimit, int R,
                                                float* __restrict__ partv, long N, Rows rows,
                                                int shares, int shift) {
     typedef typename Frag<T>::type F;
@@ -524,10 +559,11 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
     const Tile f = find_tile(rows, tile, shift);
     if (f.adapter < 0) return;
     if (DV) {
-        const T* Wl = W + (long)f.adapter * NP * R;
+#pragma unroll 4
         for (int u = tid; u < RT * 16 * (C * PC / 8); u += 256) {
             const int r = u / (C * PC / 8), c = u % (C * PC / 8) * 8;
-            *(F*)(wt + r * LW + c) = load_frag(Wl + (long)r * NP + p0 + c, r < R ? NP - p0 - c : 0);
+            const long e = (long)f.adapter * NP * R + (long)r * NP + p0 + c;
+            *(F*)(wt + r * LW + c) = trim(eight(W, e, wlimit), e, wlimit, r < R ? NP - p0 - c : 0);
         }
     }
     f32x4 acc[C][CT][RT];
@@ -540,7 +576,8 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
     const long jend = min(f.n, f.j0 + (1l << shift));
     constexpr int QV = (64 * RT * 2 + 255) / 256;       // vectors of Q a thread
     constexpr int PV = 64 * PC / 8 / 256, PW = PC / 8;  // of P; a row's
-    F x[PV], q[QV];
+    constexpr int D = C > 1 ? 2 : 1;                    // strips of P ahead
+    F x[D][PV], q[QV];
     // Rows of this step (for u), the next (loading) and the one behind it, divided out by one wave.
     __shared__ int at[3][64];
     auto find_rows = [&](long j0, int slot) {
@@ -552,12 +589,11 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
     __syncthreads();
     int slot = 0;
     // a row's columns side by side over the lanes: rows of an odd width straddle few lines
-    auto load = [&](long j0, int slot, int first) {
+    auto load = [&](F (&x)[PV], long j0, int slot, int first) {
 #pragma unroll
         for (int i = 0; i < PV; ++i) {
             const int n = i * (256 / PW) + tid / PW, c = first + tid % PW * 8;
-            const long k = j0 + n, r = at[slot][n];
-            x[i] = load_frag(P + r * ps + c, k < jend ? NP - c : 0);
+            x[i] = eight(P, at[slot][n] * ps + c, plimit);
         }
     };
     auto load_q = [&](long j0, int slot) {
@@ -565,11 +601,11 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
         for (int i = 0; i < QV; ++i) {
             const int u = i * 256 + tid, n = u / (RT * 2);
             if (n >= 64) continue;
-            const long k = j0 + n, r = at[slot][n];
-            q[i] = load_frag(Q + r * RP + u % (RT * 2) * 8, k < jend ? 8 : 0);
+            q[i] = *(const F*)(Q + (long)at[slot][n] * RP + u % (RT * 2) * 8);
         }
     };
-    load(f.j0, 0, p0);
+    load(x[0], f.j0, 0, p0);
+    if (D > 1) load(x[D - 1], f.j0, 0, p0 + PC);
     load_q(f.j0, 0);
     for (long j0 = f.j0; j0 < jend; j0 += 64) {
         const int next = slot == 2 ? 0 : slot + 1, behind = next == 2 ? 0 : next + 1;
@@ -580,22 +616,28 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
 #pragma unroll
         for (int k = 0; k < C; ++k) {
             __syncthreads();
+            // columns behind the last and rows behind the tile's are zero on both sides
+            const bool edge = p0 + (k + 1) * PC > NP || !(j0 + 64 <= jend);
 #pragma unroll
-            for (int i = 0; i < PV; ++i)
-                *(F*)(pt + (i * (256 / PW) + tid / PW) * LP + tid % PW * 8) = x[i];
+            for (int i = 0; i < PV; ++i) {
+                const int n = i * (256 / PW) + tid / PW, c = p0 + k * PC + tid % PW * 8;
+                F v = x[k % D][i];
+                if (edge) v = trim(v, at[slot][n] * ps + c, plimit, j0 + n < jend ? NP - c : 0);
+                *(F*)(pt + n * LP + tid % PW * 8) = v;
+            }
             if (k == 0)
 #pragma unroll
                 for (int i = 0; i < QV; ++i) {
                     const int u = i * 256 + tid, n = u / (RT * 2);
-                    if (n < 64) *(F*)(qt + n * LQ + u % (RT * 2) * 8) = q[i];
+                    if (n >= 64) continue;
+                    F v = q[i];
+                    if (edge) v = trim(v, 0, 8, j0 + n < jend ? 8 : 0);
+                    *(F*)(qt + n * LQ + u % (RT * 2) * 8) = v;
                 }
             __syncthreads();
-            if (k + 1 < C) {
-                load(j0, slot, p0 + (k + 1) * PC);
-            } else if (more) {
-                load(j0 + 64, next, p0);
-                load_q(j0 + 64, next);
-            }
+            if (k + D < C) load(x[k % D], j0, slot, p0 + (k + D) * PC);
+            else if (more) load(x[k % D], j0 + 64, next, p0 + (k + D - C) * PC);
+            if (k + 1 == C && more) load_q(j0 + 64, next);
             if (DV) {           // a wave takes 16 of the rows
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
@@ -706,12 +748,13 @@ int tiles_of(const long* counts, int S, long T, int shift) {
 int r16_of(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
 template <typename T, bool KCONT>
-void shrink(const void* X, long xs, const void* W, int K, int R, const Rows& rows, int tiles,
+void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int K, int R, const Rows& rows, int tiles,
             const Scale& scale, void* V, int RP, float* part, long N, int splits, int kper,
             hipStream_t st) {
 #define GO(RT)                                                                                   \
     k_shrink<T, RT, KCONT><<<(unsigned)(tiles * splits), 256, 0, st>>>(                          \
-        (const T*)X, xs, (const T*)W, K, R, rows, scale, (T*)V, RP, part, N, splits, kper)
+        (const T*)X, xs, xlimit, (const T*)W, wlimit, K, R, rows, scale, (T*)V, RP, part, N,     \
+        splits, kper)
     const int R16 = r16_of(R);
     if (R16 == 16) GO(1);
     else if (R16 == 32) GO(2);
@@ -721,43 +764,51 @@ void shrink(const void* X, long xs, const void* W, int K, int R, const Rows& row
 }
 
 template <typename T, bool RCONT>
-void expand(const void* base, long bs, void* out, long os, const void* V, int RP, const void* W,
-            int M, int R, const Rows& rows, int tiles, int shift, hipStream_t st) {
+void expand(const void* base, long bs, long blimit, void* out, long os, const void* V, int RP,
+            const void* W, long wlimit, int M, int R, const Rows& rows, int tiles, int shift, hipStream_t st) {
     const int strips = (M + 255) / 256;
 #define GO(RK)                                                                                   \
     k_expand<T, RK, RCONT><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
-        (const T*)base, bs, (T*)out, os, (const T*)V, RP, (const T*)W, M, R, rows, strips, shift)
+        (const T*)base, bs, blimit, (T*)out, os, (const T*)V, RP, (const T*)W, wlimit, M, R,     \
+        rows, strips, shift)
     if (RP == 32) GO(1);
     else if (RP == 64) GO(2);
     else GO(4);
 #undef GO
 }
 
-// Columns that a workgroup of outer owns: 256, or 128 where a rank of 128 fills the registers;
-// 1024 or 512 of those whose u it sums, as many as the accumulators leave room for.
-int outer_columns(int R, int with_u) {
-    return R > 64 ? 128 : !with_u ? 256 : R <= 16 ? 1024 : 512;
+// Columns that a workgroup of outer owns: 256, or 128 where a rank of 128 fills the registers.
+// With u 1024 or 512, as many as the accumulators leave room for (65536 rows of 4096, rank 16: u's
+// shares 9 us to sum, 17 at 256 columns), but 256 where that would leave CUs without work (1073
+// rows of 2049: 9 us, 20 at 1024).
+int outer_columns(int R, int with_u, long row_tiles, int NP) {
+    if (R > 64) return 128;
+    const int wide = R <= 16 ? 1024 : 512;
+    return with_u && row_tiles * ((NP + wide - 1) / wide) >= 512 ? wide : 256;
 }
 
 template <typename T, bool RCONT>
-void outer(const void* P, long ps, int NP, const void* Q, int RP, float* part, const void* W,
-           float* partv, long N, const Rows& rows, int tiles, int shift, void* out, int R, int L,
-           hipStream_t st) {
-    const int PC = outer_columns(R, W != nullptr), strips = (NP + PC - 1) / PC, R16 = r16_of(R);
+void outer(const void* P, long ps, long plimit, int NP, const void* Q, int RP, float* part,
+           const void* W, long wlimit, float* partv, long N, const Rows& rows, int tiles, int shift, int columns, void* out,
+           int R, int L, hipStream_t st) {
+    const int PC = columns, strips = (NP + PC - 1) / PC, R16 = r16_of(R);
 #define GO(RT, CT, NS)                                                                           \
     k_outer<T, RT, CT, NS><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
-        (const T*)P, ps, NP, (const T*)Q, RP, part, (const T*)W, R, partv, N, rows, strips, shift)
+        (const T*)P, ps, plimit, NP, (const T*)Q, RP, part, (const T*)W, wlimit, R, partv, N,    \
+        rows, strips, shift)
     if (tiles == 0) {           // no row has an adapter: the sum below writes zeros
     } else if (R16 == 16) {
-        if (W) GO(1, 4, 4);
-        else GO(1, 4, 0);
+        if (!W) GO(1, 4, 0);
+        else if (PC > 256) GO(1, 4, 4);
+        else GO(1, 4, 1);
     } else if (R16 == 32) {
-        if (W) GO(2, 4, 2);
-        else GO(2, 4, 0);
+        if (!W) GO(2, 4, 0);
+        else if (PC > 256) GO(2, 4, 2);
+        else GO(2, 4, 1);
     } else if (R16 == 64) GO(4, 4, 0);
     else GO(8, 2, 0);
 #undef GO
-    if (tiles > 4 * L) {
+    if (tiles > 16 * L) {           // many tiles an adapter
         const int blocks = (NP + 127) / 128 * R;
         k_outer_sum<T, RCONT, 8><<<(unsigned)L * blocks, 256, 0, st>>>(
             part, R16, strips * PC, rows, shift, (T*)out, NP, R, blocks);
@@ -783,7 +834,8 @@ int lowrank_splits(const long* counts, int S, long T, int K) {
 }
 
 // With `part` (splits, N, R16) the shares are left there unscaled and V is not written.
-void launch_shrink(int type, int kcont, const void* X, long xs, const void* W, int K, int R,
+void launch_shrink(int type, int kcont, const void* X, long xs, long xlimit, const void* W,
+                   long wlimit, int K, int R,
                    const int* order, const int* segs, const int* adapter, const long* counts,
                    int S, int Bn, long T, const float* scale, float scale_all, void* V,
                    float* part, hipStream_t st) {
@@ -795,14 +847,14 @@ void launch_shrink(int type, int kcont, const void* X, long xs, const void* W, i
     const long N = T * Bn;
     const int RP = lowrank_rp(R);
     if (type == LM_BF16)
-        kcont ? shrink<bf16_t, true>(X, xs, W, K, R, rows, tiles, sc, V, RP, part, N, splits,
+        kcont ? shrink<bf16_t, true>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part, N, splits,
                                      kper, st)
-              : shrink<bf16_t, false>(X, xs, W, K, R, rows, tiles, sc, V, RP, part, N, splits,
+              : shrink<bf16_t, false>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part, N, splits,
                                       kper, st);
     else
-        kcont ? shrink<f16_t, true>(X, xs, W, K, R, rows, tiles, sc, V, RP, part, N, splits, kper,
+        kcont ? shrink<f16_t, true>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part, N, splits, kper,
                                     st)
-              : shrink<f16_t, false>(X, xs, W, K, R, rows, tiles, sc, V, RP, part, N, splits,
+              : shrink<f16_t, false>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part, N, splits,
                                      kper, st);
 }
 
@@ -821,8 +873,8 @@ void launch_shrink_sum(int type, int R, const int* order, const int* segs, const
                                                               (f16_t*)V, RP);
 }
 
-void launch_expand(int type, int rcont, const void* base, long bs, void* out, long os,
-                   const void* V, const void* W, int M, int R, const int* order, const int* segs,
+void launch_expand(int type, int rcont, const void* base, long bs, long blimit, void* out,
+                   long os, const void* V, const void* W, long wlimit, int M, int R, const int* order, const int* segs,
                    const int* adapter, const long* counts, int S, int Bn, long T,
                    hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
@@ -833,11 +885,11 @@ void launch_expand(int type, int rcont, const void* base, long bs, void* out, lo
     const int tiles = tiles_of(counts, S, T, shift), RP = lowrank_rp(R);
     if (tiles == 0) return;
     if (type == LM_BF16)
-        rcont ? expand<bf16_t, true>(base, bs, out, os, V, RP, W, M, R, rows, tiles, shift, st)
-              : expand<bf16_t, false>(base, bs, out, os, V, RP, W, M, R, rows, tiles, shift, st);
+        rcont ? expand<bf16_t, true>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows, tiles, shift, st)
+              : expand<bf16_t, false>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows, tiles, shift, st);
     else
-        rcont ? expand<f16_t, true>(base, bs, out, os, V, RP, W, M, R, rows, tiles, shift, st)
-              : expand<f16_t, false>(base, bs, out, os, V, RP, W, M, R, rows, tiles, shift, st);
+        rcont ? expand<f16_t, true>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows, tiles, shift, st)
+              : expand<f16_t, false>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows, tiles, shift, st);
 }
 
 // A decode step: no adapter has so many rows that W would pass more than four times.
@@ -865,16 +917,14 @@ void launch_expand_few(int type, const void* base, long bs, void* out, long os, 
             R, rows, strips);
 }
 
-int lowrank_strips(int NP, int R, int with_u) {
-    const int PC = outer_columns(R, with_u);
-    return (NP + PC - 1) / PC;
+int lowrank_outer_columns(const long* counts, int S, long T, int NP, int R, int with_u) {
+    return outer_columns(R, with_u, tiles_of(counts, S, T, 6), NP);
 }
 // log2 of the rows that one partial gradient sums: about four workgroups a CU over the strips,
 // never fewer than 64 rows (a step) nor more than 4096.
-int lowrank_outer_shift(const long* counts, int S, long T, int NP, int R, int with_u) {
-    const long strips = lowrank_strips(NP, R, with_u);
+int lowrank_outer_shift(const long* counts, int S, long T, int strips) {
     int shift = 12;
-    while (shift > 6 && tiles_of(counts, S, T, shift) * strips < 1024) --shift;
+    while (shift > 6 && (long)tiles_of(counts, S, T, shift) * strips < 1024) --shift;
     return shift;
 }
 int lowrank_outer_tiles(const long* counts, int S, long T, int shift) {
@@ -884,23 +934,23 @@ int lowrank_outer_tiles(const long* counts, int S, long T, int shift) {
 // would be as many bytes as dy.
 int lowrank_one_reading(int R) { return R <= 32; }
 
-void launch_outer(int type, int rcont, const void* P, long ps, int NP, const void* Q, float* part,
-                  const void* W, float* partv, const int* order, const int* segs,
+void launch_outer(int type, int rcont, const void* P, long ps, long plimit, int NP,
+                  const void* Q, float* part, const void* W, long wlimit, float* partv, const int* order, const int* segs,
                   const int* adapter, const long* counts, int S, int Bn, long T, int shift,
-                  void* out, int R, int L, hipStream_t st) {
+                  int columns, void* out, int R, int L, hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const int tiles = tiles_of(counts, S, T, shift), RP = lowrank_rp(R);
     const long N = T * Bn;
     if (type == LM_BF16)
-        rcont ? outer<bf16_t, true>(P, ps, NP, Q, RP, part, W, partv, N, rows, tiles, shift, out,
-                                    R, L, st)
-              : outer<bf16_t, false>(P, ps, NP, Q, RP, part, W, partv, N, rows, tiles, shift, out,
-                                     R, L, st);
+        rcont ? outer<bf16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
+                                    columns, out, R, L, st)
+              : outer<bf16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
+                                     columns, out, R, L, st);
     else
-        rcont ? outer<f16_t, true>(P, ps, NP, Q, RP, part, W, partv, N, rows, tiles, shift, out,
-                                   R, L, st)
-              : outer<f16_t, false>(P, ps, NP, Q, RP, part, W, partv, N, rows, tiles, shift, out,
-                                    R, L, st);
+        rcont ? outer<f16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
+                                   columns, out, R, L, st)
+              : outer<f16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
+                                    columns, out, R, L, st);
 }
 
 }  // extern "C"

@@ -25,24 +25,25 @@ void launch_adjust(int, const void*, long, void*, const void*, long, int, int, c
                    long, int, hipStream_t);
 int lowrank_rp(int R);
 int lowrank_splits(const long* counts, int S, long T, int K);
-int lowrank_strips(int NP, int R, int with_u);
-int lowrank_outer_shift(const long* counts, int S, long T, int NP, int R, int with_u);
+int lowrank_outer_columns(const long* counts, int S, long T, int NP, int R, int with_u);
+int lowrank_outer_shift(const long* counts, int S, long T, int strips);
 int lowrank_few(const long* counts, int S, long T);
 void launch_expand_few(int, const void*, long, void*, long, const float*, const void*, int, int,
                        const int*, const int*, const int*, const long*, int, int, long,
                        const float*, float, int, hipStream_t);
 int lowrank_outer_tiles(const long* counts, int S, long T, int shift);
 int lowrank_one_reading(int R);
-void launch_shrink(int, int, const void*, long, const void*, int, int, const int*, const int*,
-                   const int*, const long*, int, int, long, const float*, float, void*, float*,
-                   hipStream_t);
+void launch_shrink(int, int, const void*, long, long, const void*, long, int, int, const int*,
+                   const int*, const int*, const long*, int, int, long, const float*, float,
+                   void*, float*, hipStream_t);
 void launch_shrink_sum(int, int, const int*, const int*, const int*, int, int, long, const float*,
                        float, void*, const float*, int, hipStream_t);
-void launch_expand(int, int, const void*, long, void*, long, const void*, const void*, int, int,
-                   const int*, const int*, const int*, const long*, int, int, long, hipStream_t);
-void launch_outer(int, int, const void*, long, int, const void*, float*, const void*, float*,
-                  const int*, const int*, const int*, const long*, int, int, long, int, void*,
-                  int, int, hipStream_t);
+void launch_expand(int, int, const void*, long, long, void*, long, const void*, const void*, long,
+                   int, int, const int*, const int*, const int*, const long*, int, int, long,
+                   hipStream_t);
+void launch_outer(int, int, const void*, long, long, int, const void*, float*, const void*, long,
+                  float*, const int*, const int*, const int*, const long*, int, int, long, int, int,
+                  void*, int, int, hipStream_t);
 }
 
 namespace {
@@ -323,16 +324,28 @@ struct Grouped {
             scale = scale_->to(at::kFloat).contiguous();
         }
     }
+    // Elements of the storage from the tensor's first on: the kernels read eight at a time, past a
+    // row's end if need be but never past this.  Where there are not even eight, in a copy.
+    static long room(const Tensor& t) {
+        return (long)(t.storage().nbytes() / t.element_size()) - t.storage_offset();
+    }
+    static Tensor readable(const Tensor& t) {
+        if (!t.defined() || room(t) >= 8) return t;
+        Tensor copy = at::zeros({t.numel() + 8}, t.options()).narrow(0, 0, t.numel()).view(t.sizes());
+        return copy.copy_(t);
+    }
     const int* ip(const Tensor& t) const { return (const int*)t.data_ptr(); }
 
     // v (N, RP) = s x W, W (L, K, R) or, contraction contiguous, (L, R, K)
-    Tensor shrink(const Tensor& x, const Tensor& w, bool kcont, hipStream_t st) const {
+    Tensor shrink(const Tensor& x_, const Tensor& w_, bool kcont, hipStream_t st) const {
+        const Tensor x = readable(x_), w = readable(w_);
         const int k = (int)x.size(1), splits = lowrank_splits(counts.data(), S, T, k);
         auto v = at::empty({N, (long)lowrank_rp(R)}, x.options());
         Tensor part;
         if (splits > 1)
             part = at::empty({(long)splits * N * lowrank_rp(R)}, x.options().dtype(at::kFloat));
-        launch_shrink(type, kcont, x.data_ptr(), row_stride(x), w.data_ptr(), k, R, ip(order),
+        launch_shrink(type, kcont, x.data_ptr(), row_stride(x), room(x), w.data_ptr(), room(w),
+                      k, R, ip(order),
                       ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
                       v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, st);
         if (splits > 1) sum(v, part, splits, st);
@@ -344,11 +357,13 @@ struct Grouped {
                           scale_all, v.data_ptr(), (const float*)part.data_ptr(), splits, st);
     }
     // out = base + s x A B of a few rows an adapter, in two launches
-    void few(const Tensor& base, Tensor& out, const Tensor& x, const Tensor& a, const Tensor& b,
+    void few(const Tensor& base, Tensor& out, const Tensor& x_, const Tensor& a_, const Tensor& b,
              hipStream_t st) const {
+        const Tensor x = readable(x_), a = readable(a_);
         const int splits = lowrank_splits(counts.data(), S, T, K);
         auto part = at::empty({(long)splits * N * lowrank_rp(R)}, x.options().dtype(at::kFloat));
-        launch_shrink(type, 0, x.data_ptr(), row_stride(x), a.data_ptr(), K, R, ip(order),
+        launch_shrink(type, 0, x.data_ptr(), row_stride(x), room(x), a.data_ptr(), room(a), K,
+                      R, ip(order),
                       ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
                       nullptr, (float*)part.data_ptr(), st);
         launch_expand_few(type, base.data_ptr(), row_stride(base), out.data_ptr(),
@@ -358,31 +373,35 @@ struct Grouped {
         check_launch("lowrank few");
     }
     // out = base + v W, W (L, R, M) or, rank contiguous, (L, M, R)
-    void expand(const Tensor& base, Tensor& out, const Tensor& v, const Tensor& w, bool rcont,
+    void expand(const Tensor& base_, Tensor& out, const Tensor& v, const Tensor& w_, bool rcont,
                 hipStream_t st) const {
+        const Tensor base = readable(base_), w = readable(w_);
         launch_expand(type, rcont, base.defined() ? base.data_ptr() : nullptr,
-                      base.defined() ? row_stride(base) : 0, out.data_ptr(), row_stride(out),
-                      v.data_ptr(), w.data_ptr(), (int)out.size(1), R, ip(order), ip(segs),
+                      base.defined() ? row_stride(base) : 0, base.defined() ? room(base) : 8,
+                      out.data_ptr(), row_stride(out), v.data_ptr(), w.data_ptr(), room(w),
+                      (int)out.size(1), R, ip(order), ip(segs),
                       ip(adapter), counts.data(), S, Bn, T, st);
         check_launch("lowrank expand");
     }
     // sum over an adapter's rows of p^T q: (L, R, NP) or, rank contiguous, (L, NP, R).  With w
     // (L, R, NP) also `u` (N, RP) = s p w^T, from the same reading of p.
-    Tensor outer(const Tensor& p, const Tensor& q, bool rcont, hipStream_t st,
-                 const Tensor& w = Tensor(), Tensor* u = nullptr) const {
-        const int np = (int)p.size(1), strips = lowrank_strips(np, R, u != nullptr);
-        const int rp = lowrank_rp(R);
-        const int shift = lowrank_outer_shift(counts.data(), S, T, np, R, u != nullptr);
+    Tensor outer(const Tensor& p_, const Tensor& q, bool rcont, hipStream_t st,
+                 const Tensor& w_ = Tensor(), Tensor* u = nullptr) const {
+        const Tensor p = readable(p_), w = readable(w_);
+        const int np = (int)p.size(1), rp = lowrank_rp(R);
+        const int columns = lowrank_outer_columns(counts.data(), S, T, np, R, u != nullptr);
+        const int strips = (np + columns - 1) / columns;
+        const int shift = lowrank_outer_shift(counts.data(), S, T, strips);
         const long tiles = lowrank_outer_tiles(counts.data(), S, T, shift);
         const auto f32 = p.options().dtype(at::kFloat);
-        auto part = at::empty({tiles * rp * strips * (u ? 1024l : 256l)}, f32);
+        auto part = at::empty({tiles * rp * strips * columns}, f32);
         Tensor partv;
         if (u) partv = at::empty({strips * N * rp}, f32);
         auto out = rcont ? at::empty({L, np, R}, p.options()) : at::empty({L, R, np}, p.options());
-        launch_outer(type, rcont, p.data_ptr(), row_stride(p), np, q.data_ptr(),
-                     (float*)part.data_ptr(), u ? w.data_ptr() : nullptr,
+        launch_outer(type, rcont, p.data_ptr(), row_stride(p), room(p), np, q.data_ptr(),
+                     (float*)part.data_ptr(), u ? w.data_ptr() : nullptr, u ? room(w) : 8,
                      u ? (float*)partv.data_ptr() : nullptr, ip(order), ip(segs), ip(adapter),
-                     counts.data(), S, Bn, T, shift, out.data_ptr(), R, L, st);
+                     counts.data(), S, Bn, T, shift, columns, out.data_ptr(), R, L, st);
         if (u) {
             *u = at::empty({N, (long)rp}, p.options());
             sum(*u, partv, strips, st);
