@@ -920,12 +920,25 @@ void launch_expand_few(int type, const void* base, long bs, void* out, long os, 
 int lowrank_outer_columns(const long* counts, int S, long T, int NP, int R, int with_u) {
     return outer_columns(R, with_u, tiles_of(counts, S, T, 6), NP);
 }
-// log2 of the rows that one partial gradient sums: about four workgroups a CU over the strips,
-// never fewer than 64 rows (a step) nor more than 4096.
-int lowrank_outer_shift(const long* counts, int S, long T, int strips) {
-    int shift = 12;
-    while (shift > 6 && (long)tiles_of(counts, S, T, shift) * strips < 1024) --shift;
-    return shift;
+// log2 of the rows that one partial gradient sums, 64 (a step) to 4096: the fewest bytes, counting
+// rounds of the workgroups that fit the chip (a last round counts whole) and the partial
+// gradients, written and read again.  65536 rows of 4096 columns, rank 16: 512 rows (604 MB; 256:
+// 671); 8192 of 50000, rank 32, in four groups: 1024 (1.2 GB; 512: 1.3, 2048: 2.2).
+int lowrank_outer_shift(const long* counts, int S, long T, int strips, int columns, int R) {
+    const long fit = columns > 256 ? 512 : 1024, R16 = r16_of(R);
+    int best = 6;
+    double least = 1e300;
+    for (int shift = 12; shift >= 6; --shift) {
+        const double tiles = tiles_of(counts, S, T, shift);
+        const double rounds = (double)(long)((tiles * strips + fit - 1) / fit);
+        const double bytes = rounds * fit * (2.0 * columns * (1l << shift)) +
+                             tiles * strips * columns * R16 * 8.0;
+        if (bytes < least) {
+            least = bytes;
+            best = shift;
+        }
+    }
+    return best;
 }
 int lowrank_outer_tiles(const long* counts, int S, long T, int shift) {
     return tiles_of(counts, S, T, shift);

@@ -26,7 +26,7 @@ void launch_adjust(int, const void*, long, void*, const void*, long, int, int, c
 int lowrank_rp(int R);
 int lowrank_splits(const long* counts, int S, long T, int K);
 int lowrank_outer_columns(const long* counts, int S, long T, int NP, int R, int with_u);
-int lowrank_outer_shift(const long* counts, int S, long T, int strips);
+int lowrank_outer_shift(const long* counts, int S, long T, int strips, int columns, int R);
 int lowrank_few(const long* counts, int S, long T);
 void launch_expand_few(int, const void*, long, void*, long, const float*, const void*, int, int,
                        const int*, const int*, const int*, const long*, int, int, long,
@@ -210,7 +210,8 @@ Tensor adjust(Tensor logits, OptTensor history, OptTensor lengths, OptTensor pro
               OptTensor bias_index, OptTensor bias, OptTensor allowed) {
     TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be (B, V) on GPU");
     const long B = logits.size(0), V = logits.size(1);
-    TORCH_CHECK(V <= (1 << 30), "logits: V must be at most 2^30");
+    TORCH_CHECK(V <= (1 << 30) && B * ((V + 2047) / 2048) < (1l << 24),
+                "logits: V at most 2^30, and fewer than 2^24 parts of 2048 columns");
     const c10::DeviceGuard guard(logits.device());
     const int type = type_of(logits, "logits");
     const Tensor z = rows_of(logits);
@@ -391,7 +392,7 @@ struct Grouped {
         const int np = (int)p.size(1), rp = lowrank_rp(R);
         const int columns = lowrank_outer_columns(counts.data(), S, T, np, R, u != nullptr);
         const int strips = (np + columns - 1) / columns;
-        const int shift = lowrank_outer_shift(counts.data(), S, T, strips);
+        const int shift = lowrank_outer_shift(counts.data(), S, T, strips, columns, R);
         const long tiles = lowrank_outer_tiles(counts.data(), S, T, shift);
         const auto f32 = p.options().dtype(at::kFloat);
         auto part = at::empty({tiles * rp * strips * columns}, f32);
