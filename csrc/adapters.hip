@@ -892,11 +892,11 @@ void launch_expand(int type, int rcont, const void* base, long bs, long blimit, 
               : expand<f16_t, false>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows, tiles, shift, st);
 }
 
-// A decode step: no adapter has so many rows that W would pass more than four times.
+// A decode step: W passes twice on the average at most, four rows a pass.  16 adapters at the
+// head (50000 columns, rank 16): 4 rows each 22 us, 29 through shrink, its sum and expand; 8 rows
+// 33 and 31, 16 rows 49 and 33.  A row alone takes as long either way, with a launch less here.
 int lowrank_few(const long* counts, int S, long T) {
-    for (int s = 0; s < S; ++s)
-        if (T * counts[s] > 4 << FEW) return 0;
-    return 1;
+    return tiles_of(counts, S, T, FEW) <= 2 * S;
 }
 
 void launch_expand_few(int type, const void* base, long bs, void* out, long os, const float* part,

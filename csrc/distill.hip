@@ -122,36 +122,47 @@ __global__ __launch_bounds__(1024) void k_distill_lists(Lists l, Stats* __restri
     }
 }
 
+DEVINL double sum1024(double s, double* lds) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = lds[0];
+    for (int w = 1; w < 16; ++w) s += lds[w];
+    return s;
+}
+
 // One workgroup in a fixed order (no atomics), 64-bit sums: a hundred thousand rows.
 __global__ __launch_bounds__(1024) void k_distill_count(const Stats* __restrict__ stats,
                                                         float weight, float* __restrict__ inv,
                                                         long N) {
-    __shared__ double ls[16];
+    __shared__ double lds[16];
     double c = 0;
+#pragma unroll 4
     for (long i = threadIdx.x; i < N; i += 1024) c += stats[i].counts;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) c += __shfl_xor(c, off, 64);
-    if ((threadIdx.x & 63) == 0) ls[threadIdx.x >> 6] = c;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) c += ls[w];
-        *inv = (float)(weight / (c > 1 ? c : 1));
-    }
+    c = sum1024(c, lds);
+    if (threadIdx.x == 0) *inv = (float)(weight / (c > 1 ? c : 1));
 }
 
+// `counted`: inv is there; otherwise the rows are counted with their losses.
 __global__ __launch_bounds__(1024) void k_distill_mean(const float* __restrict__ rows,
-                                                       const float* __restrict__ inv,
+                                                       const Stats* __restrict__ stats,
+                                                       int counted, float weight,
+                                                       float* __restrict__ inv,
                                                        float* __restrict__ loss, long N) {
-    __shared__ double ls[16];
-    double s = 0;
-    for (long i = threadIdx.x; i < N; i += 1024) s += rows[i];
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-    if ((threadIdx.x & 63) == 0) ls[threadIdx.x >> 6] = s;
-    __syncthreads();
+    __shared__ double ls[16], lc[16];
+    double s = 0, c = 0;
+#pragma unroll 4
+    for (long i = threadIdx.x; i < N; i += 1024) {
+        s += rows[i];
+        if (!counted) c += stats[i].counts;
+    }
+    s = sum1024(s, ls);
+    if (!counted) c = sum1024(c, lc);
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) s += ls[w];
-        *loss = N > 0 ? (float)(s * *inv) : 0.f;
+        const float f = counted ? *inv : (float)(weight / (c > 1 ? c : 1));
+        if (!counted) *inv = f;
+        *loss = N > 0 ? (float)(s * f) : 0.f;
     }
 }
 
@@ -525,11 +536,12 @@ void launch_distill_fwd(int type, const void* z, long zs, const void* index, lon
     const float c1 = LOG2E, ct = LOG2E / tau;
     Stats* s = (Stats*)stats;
     if (N > 0) {
-        // one workgroup up to four rows a wave; the count of more is a launch of its own
+        // one workgroup up to four rows a wave; the count of more is a launch of its own where
+        // gradients wait for it
         const long wanted = N <= 64 ? 1 : (N + 15) / 16;
         k_distill_lists<<<(unsigned)(wanted < (1 << 20) ? wanted : (1 << 20)), 1024, 0, st>>>(
             l, s, N, V, ct, weight, inv);
-        if (wanted > 1) k_distill_count<<<1, 1024, 0, st>>>(s, weight, inv, N);
+        if (wanted > 1 && dz) k_distill_count<<<1, 1024, 0, st>>>(s, weight, inv, N);
 #define MODES(T)                                                                                 \
     switch (mode_of(l, alpha, tau)) {                                                            \
         case ONE: fwd<T, ONE>(z, zs, l, s, rows, inv, dz, N, V, c1, ct, alpha, tau, st); break;  \
@@ -550,7 +562,7 @@ void launch_distill_fwd(int type, const void* z, long zs, const void* index, lon
         }
 #undef MODES
     }
-    k_distill_mean<<<1, 1024, 0, st>>>(rows, inv, loss, N);
+    k_distill_mean<<<1, 1024, 0, st>>>(rows, s, N > 0 && (N <= 64 || dz), weight, inv, loss, N);
 }
 
 void launch_distill_bwd(int type, const void* z, long zs, const void* index, long is, int index64,

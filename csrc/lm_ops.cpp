@@ -493,6 +493,8 @@ Tensor lowrank_add(Tensor y, Tensor x, Tensor a, Tensor b, Tensor order, Tensor 
     const Tensor ac = a.contiguous(), bc = b.contiguous();
     const Grouped g(x, y, ac, bc, order, segs, adapter, counts, scale, scale_all);
     TORCH_CHECK(!inplace || y.is_contiguous(), "lowrank: y must be contiguous");
+    // autograd has to see that y is another one now
+    if (inplace && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
     return lowrank_forward(g, y, x, ac, bc, inplace, nullptr);
 }
 

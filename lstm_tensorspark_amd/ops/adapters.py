@@ -33,7 +33,7 @@ class AdapterRows:
     index: an adapter in [0, num_adapters) or -1 (none) for each column; a
     host list, or a tensor (a GPU tensor is copied to the host).  The
     grouping is fixed: a captured graph replays with the rows it was
-    captured with.
+    captured with, which have to live as long as the graph.
     """
 
     def __init__(self, index: Union[Sequence[int], torch.Tensor],

@@ -98,6 +98,12 @@ class ContinuousBatcher:
         self._decode_steps = 0      # batched decode steps executed
         self._slot_steps = 0        # sum of active slots over those steps
         self._cancelled: set = set()  # rids retired by cancel()
+        if adapters is not None:
+            own = next(iter(model.weight_dict().values()))
+            if any(p.device != own.device or p.dtype != own.dtype
+                   for p in adapters.parameters()):
+                raise ValueError(f"adapters must be {own.dtype} on "
+                                 f"{own.device}, as the model is")
         self.adapters = adapters
         # of the live slots, made anew when one joins or leaves
         self._bound = None          # their adapters

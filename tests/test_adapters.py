@@ -346,6 +346,27 @@ def test_kernel_captured_and_replayed(T):
 
 
 @pytest.mark.gpu
+def test_kernel_in_place_is_seen_by_autograd():
+    t, rows, scale = make(1, 3, 16, 24, 4, 2, dtype=torch.bfloat16, dev="cuda",
+                          index=[0, 1, -1])
+    w = torch.randn(24, device="cuda").bfloat16().requires_grad_()
+    out = (t["y"] * w).sum()            # keeps y for its backward pass
+    lowrank_add_(t["y"], t["x"], t["a"], t["b"], rows, scale)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.backward()
+
+
+@pytest.mark.gpu
+def test_kernel_input_and_output_are_one_tensor():
+    t, rows, scale = make(2, 5, 48, 48, 6, 2, dtype=torch.bfloat16, dev="cuda")
+    t["x"] = t["y"].clone()
+    want, err = bounds(t, torch.zeros_like(t["y"]), rows, scale)
+    y = t["y"].clone()
+    lowrank_add_(y, y, t["a"], t["b"], rows, scale)
+    assert ((y.double().cpu() - want["out"]).abs() <= err["out"]).all()
+
+
+@pytest.mark.gpu
 def test_kernel_is_what_runs(monkeypatch):
     t, rows, scale = make(1, 4, 16, 16, 4, 2, dtype=torch.bfloat16, dev="cuda")
     monkeypatch.setattr(mod, "_ref_lowrank", None)

@@ -251,6 +251,8 @@ def test_workflow_refusals():
             eng.submit([1], 3, **kw)
     with pytest.raises(ValueError):
         ContinuousBatcher(m).submit([1], 3, adapter=0)
+    with pytest.raises(ValueError):
+        ContinuousBatcher(m, adapters=make_set(cfg).double())
     with pytest.raises(AssertionError):
         m.generate(torch.zeros(1, 1).long(), 2, use_graph=True,
                    rules=LogitRules())
