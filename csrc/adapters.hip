@@ -262,23 +262,34 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
         }
 }
 
-// The shares summed in their order, scaled and rounded; four of a row's R a thread.
-template <typename T>
+// The shares summed in a fixed order, scaled and rounded; four of a row's R a thread.  GR groups of
+// threads take every GR-th share where there are many (98 of 8192 rows, rank 32).
+template <typename T, int GR>
 __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ part, long N, int R16,
                                                     int splits, Rows rows, Scale scale,
                                                     T* __restrict__ V, int RP) {
     typedef T out4 __attribute__((ext_vector_type(4)));
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= N * (RP / 4)) return;
+    constexpr int TH = 256 / GR;
+    __shared__ f32x4 sums[GR > 1 ? 256 : 1];
+    const int group = threadIdx.x / TH;
+    const long i = (long)blockIdx.x * TH + threadIdx.x % TH;
     const long row = i / (RP / 4);
-    const int r = (int)(i % (RP / 4)) * 4, l = rows.adapter[(unsigned)row % (unsigned)rows.Bn];
-    if (l < 0) return;
+    const int r = (int)(i % (RP / 4)) * 4;
+    const int l = row < N ? rows.adapter[(unsigned)row % (unsigned)rows.Bn] : -1;
     f32x4 s = f32x4{0, 0, 0, 0};
-    if (r < R16) {
+    if (l >= 0 && r < R16) {
         const float* p = part + row * R16 + r;
 #pragma unroll 8
-        for (int k = 0; k < splits; ++k) s += *(const f32x4*)(p + (long)k * N * R16);
+        for (int k = group; k < splits; k += GR) s += *(const f32x4*)(p + (long)k * N * R16);
     }
+    if (GR > 1) {
+        sums[threadIdx.x] = s;
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int k = 1; k < GR; ++k) s += sums[k * TH + threadIdx.x];
+    }
+    if (l < 0) return;
     const float sc = scale(l);
     *(out4*)(V + row * RP + r) = out4{(T)(s[0] * sc), (T)(s[1] * sc), (T)(s[2] * sc),
                                       (T)(s[3] * sc)};
@@ -864,13 +875,18 @@ void launch_shrink_sum(int type, int R, const int* order, const int* segs, const
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const Scale sc{scale, scale_all};
     const int RP = lowrank_rp(R), R16 = r16_of(R);
-    const long N = T * Bn, blocks = (N * (RP / 4) + 255) / 256;
-    if (type == LM_BF16)
-        k_shrink_sum<bf16_t><<<(unsigned)blocks, 256, 0, st>>>(part, N, R16, splits, rows, sc,
-                                                               (bf16_t*)V, RP);
-    else
-        k_shrink_sum<f16_t><<<(unsigned)blocks, 256, 0, st>>>(part, N, R16, splits, rows, sc,
-                                                              (f16_t*)V, RP);
+    const long N = T * Bn, threads = N * (RP / 4);
+#define GO(T, GR)                                                                                \
+    k_shrink_sum<T, GR><<<(unsigned)((threads + 256 / GR - 1) / (256 / GR)), 256, 0, st>>>(      \
+        part, N, R16, splits, rows, sc, (T*)V, RP)
+    if (type == LM_BF16) {
+        if (splits < 32) GO(bf16_t, 1);
+        else GO(bf16_t, 8);
+    } else {
+        if (splits < 32) GO(f16_t, 1);
+        else GO(f16_t, 8);
+    }
+#undef GO
 }
 
 void launch_expand(int type, int rcont, const void* base, long bs, long blimit, void* out,
