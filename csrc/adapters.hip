@@ -42,6 +42,15 @@ template <typename T> DEVINL typename Frag<T>::type eight(const T* p, long e, lo
     return __builtin_bit_cast(typename Frag<T>::type,
                               *(const typename Vec8<T>::type*)(p + min(e, limit - 8)));
 }
+// The same of a matrix that is read once in whole lines and need not stay in the caches: outer's
+// P (65536 rows of 4096: 139 -> 103 us).  Not of base or x, whose lines several loads share, nor
+// of the distilled logits, which are written next (all three slower).
+template <typename T>
+DEVINL typename Frag<T>::type eight_once(const T* p, long e, long limit) {
+    return __builtin_bit_cast(
+        typename Frag<T>::type,
+        __builtin_nontemporal_load((const typename Vec8<T>::type*)(p + min(e, limit - 8))));
+}
 // What `eight` gave for element e, with zeros for all but the first `left`.
 template <typename F> DEVINL F trim(F v, long e, long limit, int left) {
     typedef unsigned long long u2 __attribute__((ext_vector_type(2)));
@@ -604,7 +613,7 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
 #pragma unroll
         for (int i = 0; i < PV; ++i) {
             const int n = i * (256 / PW) + tid / PW, c = first + tid % PW * 8;
-            x[i] = eight(P, at[slot][n] * ps + c, plimit);
+            x[i] = eight_once(P, at[slot][n] * ps + c, plimit);
         }
     };
     auto load_q = [&](long j0, int slot) {
