@@ -10,7 +10,8 @@ see README "Serving / decode") behind a FastAPI endpoint:
 
 With --demo (no checkpoint) it serves a random-init model -- useful for
 latency/throughput testing of the serving stack itself.  Endpoints:
-POST /generate (greedy/temperature/top-k/top-p/beam/EOS), POST
+POST /generate (greedy/temperature/top-k/top-p/beam/EOS, penalties for
+repeated tokens and logit biases), POST
 /generate_stream (SSE token stream; needs --continuous), GET /health,
 GET /metrics (Prometheus).  --continuous turns on the continuous
 batcher (lstm_tensorspark_amd/serving.py): concurrent requests share
@@ -31,6 +32,7 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 from lstm_tensorspark_amd.config import Config, ModelConfig
 from lstm_tensorspark_amd.models.lstm import LSTMModel
+from lstm_tensorspark_amd.ops.logits import LogitRules
 
 
 def build_app(model: LSTMModel, device: torch.device, batcher=None):
@@ -48,6 +50,22 @@ def build_app(model: LSTMModel, device: torch.device, batcher=None):
         beam_size: int = 1
         eos_token: int = -1
         seed: int | None = None
+        repetition_penalty: float = 1.0
+        presence_penalty: float = 0.0
+        frequency_penalty: float = 0.0
+        logit_bias: dict[int, float] | None = None
+
+        def rules(self):
+            """What the request wants done to its logits, None for nothing."""
+            r = LogitRules(self.repetition_penalty, self.presence_penalty,
+                           self.frequency_penalty, self.logit_bias)
+            try:
+                r.check(model.cfg.vocab_size)
+            except ValueError as e:
+                raise HTTPException(400, str(e))
+            if self.beam_size > 1 and (r.penalizes or r.bias):
+                raise HTTPException(400, "beam search takes no penalties")
+            return r if r.penalizes or r.bias else None
 
     app = FastAPI(title="lstm_tensorspark_amd serving")
 
@@ -93,11 +111,12 @@ def build_app(model: LSTMModel, device: torch.device, batcher=None):
             raise HTTPException(400, f"tokens must be in [0, {V})")
         if req.steps < 1 or req.steps > 4096:
             raise HTTPException(400, "steps must be in [1, 4096]")
+        rules = req.rules()
         rid = batcher.submit(req.tokens, req.steps,
                              eos_token=req.eos_token,
                              temperature=req.temperature,
                              top_k=req.top_k, top_p=req.top_p,
-                             seed=req.seed)
+                             seed=req.seed, rules=rules)
 
         def events():
             sent = len(req.tokens)
@@ -143,6 +162,12 @@ def build_app(model: LSTMModel, device: torch.device, batcher=None):
             if m_reqs:
                 m_reqs.labels(status="bad_request").inc()
             raise HTTPException(400, "steps must be in [1, 4096]")
+        try:
+            rules = req.rules()
+        except HTTPException:
+            if m_reqs:
+                m_reqs.labels(status="bad_request").inc()
+            raise
         score = None
         if batcher is not None and req.beam_size <= 1:
             # continuous batching: greedy AND sampled requests share
@@ -151,7 +176,7 @@ def build_app(model: LSTMModel, device: torch.device, batcher=None):
                                  eos_token=req.eos_token,
                                  temperature=req.temperature,
                                  top_k=req.top_k, top_p=req.top_p,
-                                 seed=req.seed)
+                                 seed=req.seed, rules=rules)
             toks = batcher.result(rid, timeout=120.0)
             if m_reqs:
                 m_reqs.labels(status="ok").inc()
@@ -169,7 +194,7 @@ def build_app(model: LSTMModel, device: torch.device, batcher=None):
                 out = model.generate(prompt, steps=req.steps,
                                      temperature=req.temperature,
                                      top_k=req.top_k, top_p=req.top_p,
-                                     eos_token=req.eos_token)
+                                     eos_token=req.eos_token, rules=rules)
         if m_reqs:
             m_reqs.labels(status="ok").inc()
             m_toks.inc(out.shape[0] - len(req.tokens))

@@ -350,6 +350,35 @@ def test_distil_into_adapters_and_serve_them():
     serve_them(base, s)
 
 
+@pytest.mark.parametrize("batched", [False, True])
+def test_served_requests_have_penalties(batched, monkeypatch):
+    import os
+    monkeypatch.syspath_prepend(os.path.join(os.path.dirname(
+        os.path.dirname(os.path.abspath(__file__))), "examples"))
+    import serve
+    from starlette.testclient import TestClient
+    torch.manual_seed(9)
+    m = LSTMModel(make_cfg()).eval()
+    eng = ContinuousBatcher(m) if batched else None
+    if eng:
+        eng.start()
+    try:
+        c = TestClient(serve.build_app(m, torch.device("cpu"), batcher=eng))
+        ask = {"tokens": [1, 2], "steps": 9}
+        plain = c.post("/generate", json=ask).json()["generated"]
+        assert plain == solo(m, [1, 2], 9)[2:]
+        got = c.post("/generate", json={**ask, "presence_penalty": 1e4})
+        assert len(set(got.json()["generated"])) == 9
+        got = c.post("/generate", json={**ask, "logit_bias": {"7": 1e4}})
+        assert got.json()["generated"] == [7] * 9
+        for bad in ({"repetition_penalty": 0.0}, {"logit_bias": {"30": 1.0}},
+                    {"presence_penalty": 1.0, "beam_size": 2}):
+            assert c.post("/generate", json={**ask, **bad}).status_code == 400
+    finally:
+        if eng:
+            eng.stop()
+
+
 # ------------------------------------------------------------------- GPU
 @gpu
 @pytest.mark.parametrize("head,bidi", [("lm", False), ("seq_classifier", True)])
