@@ -155,7 +155,9 @@ DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 @pytest.mark.parametrize("B,V,L,K", [(1, 1, 1, 1), (1, 7, 3, 2),
                                      (2, 2047, 100, 5), (3, 2049, 1, 40),
                                      (1, 50000, 300, 8), (17, 4097, 700, 0),
-                                     (300, 1000, 20, 3), (5, 70001, 4096, 300)])
+                                     (300, 1000, 20, 3), (5, 70001, 4096, 300),
+                                     (3, 8193, 5001, 9), (2, 100, 4100, 2),
+                                     (1, 20000, 40000, 0)])
 def test_kernel_sizes(dtype, B, V, L, K):
     for masked in (True, False):
         z, h, a = make(B, V, L, K, seed=V + B, dtype=dtype, dev="cuda",
