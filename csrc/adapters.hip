@@ -563,7 +563,8 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
                                                int NP, const T* __restrict__ Q, int RP,
                                                float* __restrict__ part,
                                                const T* __restrict__ W, long wlimit, int R,
-                                               float* __restrict__ partv, long N, Rows rows,
+                                               float* __restrict__ partv, long N,
+                                               T* __restrict__ whole, int rcont, Rows rows,
                                                int shares, int shift) {
     typedef typename Frag<T>::type F;
     constexpr bool DV = NS > 0;
@@ -695,6 +696,23 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
         find_rows(j0 + 128, behind);
         slot = next;
     }
+    if (whole) {                // the adapter's only tile: its gradient, rounded here
+        T* o = whole + (long)f.adapter * NP * R;
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int p = p0 + k * PC + (wave * CT + c) * 16 + g * 4 + i;
+                        const int r = t * 16 + (lane & 15);
+                        if (p < NP && r < R)
+                            o[rcont ? (long)p * R + r : (long)r * NP + p] = (T)acc[k][c][t][i];
+                    }
+        return;
+    }
     const int LO = shares * C * PC;
 #pragma unroll
     for (int k = 0; k < C; ++k)
@@ -807,15 +825,16 @@ int outer_columns(int R, int with_u, long row_tiles, int NP) {
     return with_u && row_tiles * ((NP + wide - 1) / wide) >= 512 ? wide : 256;
 }
 
+// `whole`: every adapter's rows are one tile, and out holds zeros for those without rows.
 template <typename T, bool RCONT>
 void outer(const void* P, long ps, long plimit, int NP, const void* Q, int RP, float* part,
-           const void* W, long wlimit, float* partv, long N, const Rows& rows, int tiles, int shift, int columns, void* out,
-           int R, int L, hipStream_t st) {
+           const void* W, long wlimit, float* partv, long N, const Rows& rows, int tiles, int shift, int columns, int whole,
+           void* out, int R, int L, hipStream_t st) {
     const int PC = columns, strips = (NP + PC - 1) / PC, R16 = r16_of(R);
 #define GO(RT, CT, NS)                                                                           \
     k_outer<T, RT, CT, NS><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
         (const T*)P, ps, plimit, NP, (const T*)Q, RP, part, (const T*)W, wlimit, R, partv, N,    \
-        rows, strips, shift)
+        whole ? (T*)out : nullptr, RCONT, rows, strips, shift)
     if (tiles == 0) {           // no row has an adapter: the sum below writes zeros
     } else if (R16 == 16) {
         if (!W) GO(1, 4, 0);
@@ -828,6 +847,7 @@ void outer(const void* P, long ps, long plimit, int NP, const void* Q, int RP, f
     } else if (R16 == 64) GO(4, 4, 0);
     else GO(8, 2, 0);
 #undef GO
+    if (whole) return;
     if (tiles > 16 * L) {           // many tiles an adapter
         const int blocks = (NP + 127) / 128 * R;
         k_outer_sum<T, RCONT, 8><<<(unsigned)L * blocks, 256, 0, st>>>(
@@ -945,21 +965,30 @@ void launch_expand_few(int type, const void* base, long bs, void* out, long os, 
 int lowrank_outer_columns(const long* counts, int S, long T, int NP, int R, int with_u) {
     return outer_columns(R, with_u, tiles_of(counts, S, T, 6), NP);
 }
-// log2 of the rows that one partial gradient sums, 64 (a step) to 4096: the fewest bytes, counting
-// rounds of the workgroups that fit the chip (a last round counts whole) and the partial
-// gradients, written and read again.  65536 rows of 4096 columns, rank 16: 512 rows (604 MB; 256:
-// 671); 8192 of 50000, rank 32, in four groups: 1024 (1.2 GB; 512: 1.3, 2048: 2.2).
+// Whether every group of rows is one tile: its gradient is written without a sum of partial ones.
+int lowrank_outer_whole(const long* counts, int S, long T, int shift) {
+    return tiles_of(counts, S, T, shift) == S;
+}
+// log2 of the rows that one partial gradient sums, 64 (a step) to 4096: the least time by what
+// was measured, in us.  A workgroup takes 6 to come and go, and a step of 64 rows 1.2, or what it
+// reads at 25 GB/s by itself, or at its share of 5 TB/s; rounds of the workgroups that fit the chip count whole; the partial gradients are
+// written and read again by a launch of 4, which one tile an adapter does without.  65536 rows of
+// 4096 columns, rank 16: 512 rows; 8192 of 50000, rank 32, in four groups: 1024; 1073 of 2049 in
+// seven: one tile each.
 int lowrank_outer_shift(const long* counts, int S, long T, int strips, int columns, int R) {
-    const long fit = columns > 256 ? 512 : 1024, R16 = r16_of(R);
+    const double fit = columns > 256 ? 512 : 1024, R16 = r16_of(R);
     int best = 6;
     double least = 1e300;
     for (int shift = 12; shift >= 6; --shift) {
-        const double tiles = tiles_of(counts, S, T, shift);
-        const double rounds = (double)(long)((tiles * strips + fit - 1) / fit);
-        const double bytes = rounds * fit * (2.0 * columns * (1l << shift)) +
-                             tiles * strips * columns * R16 * 8.0;
-        if (bytes < least) {
-            least = bytes;
+        const double blocks = (double)tiles_of(counts, S, T, shift) * strips;
+        const double at_once = blocks < fit ? blocks : fit;
+        const double alone = columns * 128 / 2.5e4 > 1.2 ? columns * 128 / 2.5e4 : 1.2;
+        const double step = columns * 128 * at_once / 5e6;
+        double us = (double)(long)((blocks + fit - 1) / fit) *
+                    (6 + (1 << (shift - 6)) * (step > alone ? step : alone));
+        if (!lowrank_outer_whole(counts, S, T, shift)) us += 4 + blocks * columns * R16 * 8 / 5e6;
+        if (us < least) {
+            least = us;
             best = shift;
         }
     }
@@ -975,20 +1004,20 @@ int lowrank_one_reading(int R) { return R <= 32; }
 void launch_outer(int type, int rcont, const void* P, long ps, long plimit, int NP,
                   const void* Q, float* part, const void* W, long wlimit, float* partv, const int* order, const int* segs,
                   const int* adapter, const long* counts, int S, int Bn, long T, int shift,
-                  int columns, void* out, int R, int L, hipStream_t st) {
+                  int columns, int whole, void* out, int R, int L, hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const int tiles = tiles_of(counts, S, T, shift), RP = lowrank_rp(R);
     const long N = T * Bn;
     if (type == LM_BF16)
         rcont ? outer<bf16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
-                                    columns, out, R, L, st)
+                                    columns, whole, out, R, L, st)
               : outer<bf16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
-                                     columns, out, R, L, st);
+                                     columns, whole, out, R, L, st);
     else
         rcont ? outer<f16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
-                                   columns, out, R, L, st)
+                                   columns, whole, out, R, L, st)
               : outer<f16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
-                                    columns, out, R, L, st);
+                                    columns, whole, out, R, L, st);
 }
 
 }  // extern "C"

@@ -31,6 +31,7 @@ int lowrank_few(const long* counts, int S, long T);
 void launch_expand_few(int, const void*, long, void*, long, const float*, const void*, int, int,
                        const int*, const int*, const int*, const long*, int, int, long,
                        const float*, float, int, hipStream_t);
+int lowrank_outer_whole(const long* counts, int S, long T, int shift);
 int lowrank_outer_tiles(const long* counts, int S, long T, int shift);
 int lowrank_one_reading(int R);
 void launch_shrink(int, int, const void*, long, long, const void*, long, int, int, const int*,
@@ -42,7 +43,7 @@ void launch_expand(int, int, const void*, long, long, void*, long, const void*, 
                    int, int, const int*, const int*, const int*, const long*, int, int, long,
                    hipStream_t);
 void launch_outer(int, int, const void*, long, long, int, const void*, float*, const void*, long,
-                  float*, const int*, const int*, const int*, const long*, int, int, long, int, int,
+                  float*, const int*, const int*, const int*, const long*, int, int, long, int, int, int,
                   void*, int, int, hipStream_t);
 }
 
@@ -277,13 +278,14 @@ struct Grouped {
     std::vector<long> counts;
     int S, Bn, L, K, M, R, type;
     long T, N;
+    int groups;         // adapters that have rows
     float scale_all;
 
     Grouped(const Tensor& x, const Tensor& y, const Tensor& a, const Tensor& b, Tensor order_,
-            Tensor segs_, Tensor adapter_, std::vector<int64_t> counts_, const OptTensor& scale_,
-            double all)
+            Tensor segs_, Tensor adapter_, std::vector<int64_t> counts_, int64_t groups_,
+            const OptTensor& scale_, double all)
         : order(order_), segs(segs_), adapter(adapter_), counts(counts_.begin(), counts_.end()),
-          scale_all((float)all) {
+          groups((int)groups_), scale_all((float)all) {
         TORCH_CHECK(x.is_cuda() && x.dim() >= 2 && x.dim() == y.dim() &&
                         x.sizes().slice(0, x.dim() - 1) == y.sizes().slice(0, y.dim() - 1),
                     "lowrank: x (..., Bn, K) and y (..., Bn, M) on GPU");
@@ -317,6 +319,7 @@ struct Grouped {
         T = N / Bn;
         long sum = 0;
         for (long c : counts) sum += c;
+        TORCH_CHECK(groups <= S && groups >= S - 1, "lowrank: groups");
         TORCH_CHECK(sum == Bn && N < (1l << 31) && N / 64 * ((std::max(K, M) + 127) / 128) <
                         (1l << 31), "lowrank: too many rows");
         if (scale_.has_value()) {
@@ -349,13 +352,13 @@ struct Grouped {
                       k, R, ip(order),
                       ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
                       v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, st);
-        if (splits > 1) sum(v, part, splits, st);
+        if (splits > 1) sum(v, (const float*)part.data_ptr(), splits, st);
         check_launch("lowrank shrink");
         return v;
     }
-    void sum(Tensor& v, const Tensor& part, int splits, hipStream_t st) const {
+    void sum(Tensor& v, const float* part, int splits, hipStream_t st) const {
         launch_shrink_sum(type, R, ip(order), ip(segs), ip(adapter), S, Bn, T, float_ptr(scale),
-                          scale_all, v.data_ptr(), (const float*)part.data_ptr(), splits, st);
+                          scale_all, v.data_ptr(), part, splits, st);
     }
     // out = base + s x A B of a few rows an adapter, in two launches
     void few(const Tensor& base, Tensor& out, const Tensor& x_, const Tensor& a_, const Tensor& b,
@@ -394,18 +397,21 @@ struct Grouped {
         const int strips = (np + columns - 1) / columns;
         const int shift = lowrank_outer_shift(counts.data(), S, T, strips, columns, R);
         const long tiles = lowrank_outer_tiles(counts.data(), S, T, shift);
-        const auto f32 = p.options().dtype(at::kFloat);
-        auto part = at::empty({tiles * rp * strips * columns}, f32);
-        Tensor partv;
-        if (u) partv = at::empty({strips * N * rp}, f32);
-        auto out = rcont ? at::empty({L, np, R}, p.options()) : at::empty({L, R, np}, p.options());
+        const bool whole = lowrank_outer_whole(counts.data(), S, T, shift);
+        // one workspace: the gradient's parts, u's shares
+        const long parts = whole ? 0 : tiles * rp * strips * columns;
+        auto work = at::empty({parts + (u ? strips * N * rp : 0)}, p.options().dtype(at::kFloat));
+        float* part = (float*)work.data_ptr();
+        const std::vector<int64_t> size = rcont ? std::vector<int64_t>{L, np, R}
+                                                : std::vector<int64_t>{L, R, np};
+        // an adapter without rows has no tile to write its zeros
+        auto out = whole && groups < L ? at::zeros(size, p.options()) : at::empty(size, p.options());
         launch_outer(type, rcont, p.data_ptr(), row_stride(p), room(p), np, q.data_ptr(),
-                     (float*)part.data_ptr(), u ? w.data_ptr() : nullptr, u ? room(w) : 8,
-                     u ? (float*)partv.data_ptr() : nullptr, ip(order), ip(segs), ip(adapter),
-                     counts.data(), S, Bn, T, shift, columns, out.data_ptr(), R, L, st);
+                     part, u ? w.data_ptr() : nullptr, u ? room(w) : 8, u ? part + parts : nullptr, ip(order), ip(segs), ip(adapter),
+                     counts.data(), S, Bn, T, shift, columns, whole, out.data_ptr(), R, L, st);
         if (u) {
             *u = at::empty({N, (long)rp}, p.options());
-            sum(*u, partv, strips, st);
+            sum(*u, part + parts, strips, st);
         }
         check_launch("lowrank outer");
         return out;
@@ -434,12 +440,14 @@ Tensor lowrank_forward(const Grouped& g, const Tensor& y, const Tensor& x, const
 struct LowRankAdd : public torch::autograd::Function<LowRankAdd> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor y, Tensor x, Tensor a,
                           Tensor b, Tensor order, Tensor segs, Tensor adapter,
-                          std::vector<int64_t> counts, OptTensor scale, double scale_all) {
+                          std::vector<int64_t> counts, int64_t groups, OptTensor scale,
+                          double scale_all) {
         const c10::DeviceGuard guard(x.device());
-        const Grouped g(x, y, a, b, order, segs, adapter, counts, scale, scale_all);
+        const Grouped g(x, y, a, b, order, segs, adapter, counts, groups, scale, scale_all);
         Tensor v, out = lowrank_forward(g, y, x, a, b, false, &v);
         ctx->save_for_backward({x, a, b, v, order, segs, adapter, scale.value_or(Tensor())});
         ctx->saved_data["counts"] = counts;
+        ctx->saved_data["groups"] = groups;
         ctx->saved_data["scale"] = scale_all;
         ctx->saved_data["need"] = std::vector<bool>{y.requires_grad(), x.requires_grad(),
                                                     a.requires_grad(), b.requires_grad()};
@@ -449,13 +457,14 @@ struct LowRankAdd : public torch::autograd::Function<LowRankAdd> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "lowrank_add is differentiable once");
-        torch::autograd::variable_list out(10);
+        torch::autograd::variable_list out(11);
         const Tensor& dy = grads[0];
         if (!dy.defined()) return out;
         const auto s = ctx->get_saved_variables();
         const Tensor &x = s[0], &a = s[1], &b = s[2], &v = s[3];
         const c10::DeviceGuard guard(x.device());
         const Grouped g(x, dy, a, b, s[4], s[5], s[6], ctx->saved_data["counts"].toIntVector(),
+                        ctx->saved_data["groups"].toInt(),
                         s[7].defined() ? OptTensor(s[7]) : OptTensor(),
                         ctx->saved_data["scale"].toDouble());
         const hipStream_t st = stream_of(x);
@@ -482,16 +491,16 @@ struct LowRankAdd : public torch::autograd::Function<LowRankAdd> {
 };
 
 Tensor lowrank_add(Tensor y, Tensor x, Tensor a, Tensor b, Tensor order, Tensor segs,
-                   Tensor adapter, std::vector<int64_t> counts, OptTensor scale, double scale_all,
-                   bool inplace) {
+                   Tensor adapter, std::vector<int64_t> counts, int64_t groups, OptTensor scale,
+                   double scale_all, bool inplace) {
     if (!inplace && at::GradMode::is_enabled() &&
         (y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad()))
         return LowRankAdd::apply(y, x, a.contiguous(), b.contiguous(), order, segs, adapter,
-                                 counts, scale, scale_all);
+                                 counts, groups, scale, scale_all);
     const at::NoGradGuard off;
     const c10::DeviceGuard guard(x.device());
     const Tensor ac = a.contiguous(), bc = b.contiguous();
-    const Grouped g(x, y, ac, bc, order, segs, adapter, counts, scale, scale_all);
+    const Grouped g(x, y, ac, bc, order, segs, adapter, counts, groups, scale, scale_all);
     TORCH_CHECK(!inplace || y.is_contiguous(), "lowrank: y must be contiguous");
     // autograd has to see that y is another one now
     if (inplace && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
@@ -512,6 +521,6 @@ void register_lm_ops(pybind11::module_& m) {
           py::arg("bias_index"), py::arg("bias"), py::arg("allowed"));
     m.def("lowrank_add", &lowrank_add, "y + s x A B by rows' adapters", py::arg("y"),
           py::arg("x"), py::arg("a"), py::arg("b"), py::arg("order"), py::arg("segs"),
-          py::arg("adapter"), py::arg("counts"), py::arg("scale") = py::none(),
-          py::arg("scale_all") = 1.0, py::arg("inplace") = false);
+          py::arg("adapter"), py::arg("counts"), py::arg("groups"),
+          py::arg("scale") = py::none(), py::arg("scale_all") = 1.0, py::arg("inplace") = false);
 }

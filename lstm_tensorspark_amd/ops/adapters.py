@@ -61,6 +61,7 @@ class AdapterRows:
         for i in order:
             groups[index[i]] = groups.get(index[i], 0) + 1
         self.counts = list(groups.values())
+        self.groups = len(groups) - (-1 in groups)  # adapters with rows
         segs, start = [], 0
         for adapter, count in groups.items():
             segs += [adapter, start, count, 0]
@@ -95,11 +96,13 @@ def _ref_lowrank(y, x, a, b, rows: AdapterRows, scale):
 
 
 def _launch_args(rows: AdapterRows, scale):
+    args = dict(order=rows.order, segs=rows.segs, adapter=rows.adapter,
+                counts=rows.counts, groups=rows.groups)
     if isinstance(scale, torch.Tensor):
-        return dict(order=rows.order, segs=rows.segs, adapter=rows.adapter,
-                    counts=rows.counts, scale=scale)
-    return dict(order=rows.order, segs=rows.segs, adapter=rows.adapter,
-                counts=rows.counts, scale_all=float(scale))
+        args["scale"] = scale
+    else:
+        args["scale_all"] = float(scale)
+    return args
 
 
 def _check(y, x, a, b, rows, scale):

@@ -190,6 +190,8 @@ SHAPES = [
     (64, 3, 128, 513, 16, 2), (37, 29, 101, 259, 12, 6), (130, 9, 65, 70, 128, 2),
     (300, 1, 520, 136, 64, 1), (3, 200, 300, 90, 32, 100), (1, 1, 9000, 9001, 24, 1),
     (1, 5, 2050, 50, 3, 5),
+    # u in wide shares of columns, few and many of them
+    (64, 70, 40, 8001, 16, 2), (20, 53, 33, 16901, 20, 2),
 ]
 
 
