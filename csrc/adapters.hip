@@ -150,13 +150,13 @@ DEVINL long row_of(const Rows& r, const Tile& f, long j) {
 }
 
 // ---------------------------------------------------------------------------
-// shrink: V[row] = s_l X[row] W_l.  A workgroup takes 128 rows of one adapter and `kper` of the
-// contraction; its four waves hold 32 rows each, straight from memory in the operand's layout,
-// and share W's 128-step panel in LDS.  The next step's rows and panel are on their way while
-// this one is multiplied.
+// shrink: V[row] = s_l X[row] W_l.  A workgroup takes 64 rows of one adapter and `kper` of the
+// contraction, 256 a step: rows come in 512 neighbouring bytes each (in the operand's own layout,
+// 64 at a time, 65536 rows of 1024 took 48 us from memory, now 26) and pass through LDS with W's
+// panel, the next step's on their way meanwhile; a wave multiplies 16 of the rows.
 // ---------------------------------------------------------------------------
-constexpr int S_TM = 7;     // log2 rows a workgroup
-constexpr int S_KC = 128;   // contraction a step
+constexpr int S_TM = 6;     // log2 rows a workgroup
+constexpr int S_KC = 256;   // contraction a step
 
 template <typename T, int RT, bool KCONT>
 __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs, long xlimit,
@@ -165,30 +165,25 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
                                                 float* __restrict__ part, long N, int splits,
                                                 int kper) {
     typedef typename Frag<T>::type F;
-    // rows of the panel: R of the contraction each (KCONT), or 128 of R each
-    constexpr int LD = KCONT ? S_KC + 8 : RT * 16 + (RT >= 4 ? 16 : 0);
+    // rows of the panel: R of the contraction each (KCONT), or 256 of R each
+    constexpr int LX = S_KC + 8, LD = KCONT ? S_KC + 8 : RT * 16 + (RT >= 4 ? 16 : 0);
+    __shared__ __attribute__((aligned(16))) T xt[64 * LX];
     __shared__ __attribute__((aligned(16))) T w[(KCONT ? RT * 16 : S_KC) * LD];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ int at[64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
     const int split = blockIdx.x % splits;
     const Tile f = find_tile(rows, blockIdx.x / splits, S_TM);
     if (f.adapter < 0) return;
+    if (tid < 64) at[tid] = (int)row_of(rows, f, min(f.j0 + tid, f.n - 1));
     const long wl = (long)f.adapter * K * R;
     const int kend = min(K, (split + 1) * kper);
-    long row[2];
-    bool ok[2];
+    f32x4 acc[RT];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const long j = f.j0 + wave * 32 + m * 16 + (lane & 15);
-        ok[m] = j < f.n;
-        row[m] = row_of(rows, f, ok[m] ? j : f.n - 1);
-    }
-    f32x4 acc[2][RT];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int t = 0; t < RT; ++t) acc[m][t] = f32x4{0, 0, 0, 0};
+    for (int t = 0; t < RT; ++t) acc[t] = f32x4{0, 0, 0, 0};
+    __syncthreads();
 
-    F x[2][4], wv[RT];      // RT * 16 * 128 elements of the panel: RT vectors a thread
+    constexpr int XV = 64 * S_KC / 8 / 256, WV = RT * 2;    // vectors a thread
+    F x[XV], wv[WV];
     // element of W that vector i starts with, and how many of it belong to the panel
     auto of_panel = [&](int i, int k0, int& left) {
         const int u = i * 256 + tid;
@@ -201,14 +196,12 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
         left = k < kend ? R - r : 0;
         return wl + (long)k * R + r;
     };
+    auto of_rows = [&](int i, int k0) { return at[i * 8 + tid / 32] * xs + k0 + tid % 32 * 8; };
     auto load = [&](int k0) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int i = 0; i < XV; ++i) x[i] = eight_once(X, of_rows(i, k0), xlimit);
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-                x[m][s] = eight(X, row[m] * xs + k0 + s * 32 + (lane >> 4) * 8, xlimit);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
+        for (int i = 0; i < WV; ++i) {
             int left;
             wv[i] = eight(W, of_panel(i, k0, left), wlimit);
         }
@@ -219,7 +212,12 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
         const bool tail = k0 + S_KC > kend;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
+        for (int i = 0; i < XV; ++i) {
+            if (tail) x[i] = trim(x[i], of_rows(i, k0), xlimit, kend - k0 - tid % 32 * 8);
+            *(F*)(xt + (i * 8 + tid / 32) * LX + tid % 32 * 8) = x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < WV; ++i) {
             const int u = i * 256 + tid, n = KCONT ? S_KC / 8 : RT * 2;
             if (tail || R != RT * 16) {
                 int left;
@@ -228,47 +226,35 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
             }
             *(F*)(w + u / n * LD + u % n * 8) = wv[i];
         }
-        F now[2][4];
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int k = k0 + s * 32 + (lane >> 4) * 8;
-                now[m][s] = tail ? trim(x[m][s], row[m] * xs + k, xlimit, kend - k) : x[m][s];
-            }
         __syncthreads();
         if (k0 + S_KC < kend) load(k0 + S_KC);
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int s = 0; s < S_KC / 32; ++s) {
+            const F a = *(const F*)(xt + (wave * 16 + (lane & 15)) * LX + s * 32 + g * 8);
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                const F b = KCONT ? *(const F*)(w + (t * 16 + (lane & 15)) * LD + s * 32 +
-                                                (lane >> 4) * 8)
-                                  : column_frag(w, LD, s * 32, t * 16 + own_columns());
-#pragma unroll
-                for (int m = 0; m < 2; ++m) acc[m][t] = mfma(now[m][s], b, acc[m][t]);
-            }
+            for (int t = 0; t < RT; ++t)
+                acc[t] = mfma(a, KCONT ? *(const F*)(w + (t * 16 + (lane & 15)) * LD + s * 32 + g * 8)
+                                       : column_frag(w, LD, s * 32, t * 16 + own_columns()),
+                              acc[t]);
+        }
     }
     const float sc = scale(f.adapter);
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int i = 0; i < 4; ++i) {
+        const int n = wave * 16 + g * 4 + i;
+        if (f.j0 + n >= f.n) continue;
+        const long r = at[n];
+        if (part) {
+            float* p = part + ((long)split * N + r) * (RT * 16) + (lane & 15);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int src = (lane >> 4) * 4 + i;
-            const long r = __shfl(row[m], src, 64);
-            const int good = __shfl((int)ok[m], src, 64);
-            if (!good) continue;
-            if (part) {
-                float* p = part + ((long)split * N + r) * (RT * 16) + (lane & 15);
+            for (int t = 0; t < RT; ++t) p[t * 16] = acc[t][i];
+        } else {
+            T* v = V + r * RP + (lane & 15);
 #pragma unroll
-                for (int t = 0; t < RT; ++t) p[t * 16] = acc[m][t][i];
-            } else {
-                T* v = V + r * RP + (lane & 15);
-#pragma unroll
-                for (int t = 0; t < RT; ++t) v[t * 16] = (T)(acc[m][t][i] * sc);
-                if (RT == 1) v[16] = (T)0.f;        // expand contracts 32 at a time
-            }
+            for (int t = 0; t < RT; ++t) v[t * 16] = (T)(acc[t][i] * sc);
+            if (RT == 1) v[16] = (T)0.f;        // expand contracts 32 at a time
         }
+    }
 }
 
 // The shares summed in a fixed order, scaled and rounded; four of a row's R a thread.  GR groups of
@@ -866,9 +852,9 @@ extern "C" {
 // Row length of v and u: the contraction of expand, in steps of 32.
 int lowrank_rp(int R) { return R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
-// Workgroups that share a row tile's contraction: about two a CU, no share below two steps.
+// Workgroups that share a row tile's contraction: about two a CU, no share below a step.
 int lowrank_splits(const long* counts, int S, long T, int K) {
-    const int tiles = tiles_of(counts, S, T, S_TM), most = (K + 2 * S_KC - 1) / (2 * S_KC);
+    const int tiles = tiles_of(counts, S, T, S_TM), most = (K + S_KC - 1) / S_KC;
     int want = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
     return want < 1 ? 1 : want > most ? most : want;
 }
