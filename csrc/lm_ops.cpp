@@ -57,6 +57,17 @@ hipStream_t stream_of(const Tensor& t) {
     return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
+// The capture that the stream is in, 0 for none.
+int64_t capture_of(hipStream_t st) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(st, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();        // the default stream, while another one is captured
+        return 0;
+    }
+    return status == hipStreamCaptureStatusActive ? (int64_t)id : 0;
+}
+
 int type_of(const Tensor& t, const char* name) {
     switch (t.scalar_type()) {
         case at::kBFloat16: return 0;
@@ -153,7 +164,10 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
                                     inv});
             ctx->saved_data["alpha"] = alpha;
             ctx->saved_data["tau"] = tau;
-            if (dz.defined()) ctx->saved_data["dz"] = dz;
+            if (dz.defined()) {
+                ctx->saved_data["dz"] = dz;
+                ctx->saved_data["capture"] = capture_of(stream_of(logits));
+            }
         }
         return loss;
     }
@@ -167,9 +181,11 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
         if (!g.defined()) return out;
         const Distill d(logits, v[1], v[2], v[3].defined() ? OptTensor(v[3]) : OptTensor());
         const c10::DeviceGuard guard(logits.device());
-        // handed out once: a second backward pass over a kept graph computes its own
+        // Handed out once: a second backward pass over a kept graph computes its own.  So does a
+        // captured one whose forward is not in the same capture: it is replayed without it.
         const auto had = ctx->saved_data.find("dz");
-        const bool done = had != ctx->saved_data.end();
+        const bool done = had != ctx->saved_data.end() &&
+                          ctx->saved_data["capture"].toInt() == capture_of(stream_of(logits));
         if (done) {
             out[0] = had->second.toTensor();
             ctx->saved_data.erase(had);

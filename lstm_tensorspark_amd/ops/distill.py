@@ -99,8 +99,9 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
         raise ValueError("teacher_logits must be floating")
     if not 0.0 <= alpha <= 1.0:
         raise ValueError(f"alpha must be in [0, 1], got {alpha}")
-    if not (temperature > 0.0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be positive, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:      # its square and inverse in fp32
+        raise ValueError("temperature must be in [1e-6, 1e6], got "
+                         f"{temperature}")
     if not math.isfinite(weight):
         raise ValueError(f"weight must be finite, got {weight}")
     if targets is None and alpha != 1.0:

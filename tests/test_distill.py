@@ -135,6 +135,8 @@ def test_refusals():
             ((z, i, t, y), dict(alpha=math.nan)),
             ((z, i, t, y), dict(temperature=0.0)),
             ((z, i, t, y), dict(temperature=math.inf)),
+            ((z, i, t, y), dict(temperature=1e-39)),
+            ((z, i, t, y), dict(temperature=1e20)),
             ((z, i, t, y), dict(weight=math.nan)),
             ((z[:, :0], i, t, y), ok)]:
         with pytest.raises(ValueError):
@@ -346,6 +348,39 @@ def test_kernel_captured_and_replayed():
         torch.cuda.synchronize()
         want = check_on_gpu(z2, i2, t2, y2, 0.5, 2.0)
         assert torch.equal(loss.detach(), want[0]) and torch.equal(g, want[1])
+
+
+@pytest.mark.gpu
+def test_kernel_backward_captured_apart():
+    """A backward pass in a graph of its own writes its gradient at every
+    replay, also where the forward in another graph had left it."""
+    z, i, t, y = make(40, 3000, 8, seed=15, dtype=torch.bfloat16, dev="cuda")
+    zs = z.clone().requires_grad_()
+    step = lambda: distill_loss(zs, i, t, y, alpha=0.5, temperature=2.0)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(step(), zs)
+    torch.cuda.current_stream().wait_stream(s)
+    fwd, bwd = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(fwd, stream=s):
+        loss = step()
+    with torch.cuda.graph(bwd, stream=s, pool=fwd.pool()):
+        g, = torch.autograd.grad(loss, zs)
+    for seed in (16, 17):
+        z2 = make(40, 3000, 8, seed=seed, dtype=torch.bfloat16, dev="cuda")[0]
+        with torch.no_grad():
+            zs.copy_(z2)
+        fwd.replay()
+        want = check_on_gpu(z2, i, t, y, 0.5, 2.0)
+        for _ in range(3):
+            g.zero_()
+            bwd.replay()
+            torch.cuda.synchronize()
+            # from the logits again: the same numbers, in another kernel
+            assert torch.equal(loss.detach(), want[0])
+            off = (g.double() - want[1].double()).abs()
+            assert (off <= 2.0 ** -7 * want[1].double().abs()).all()
 
 
 @pytest.mark.gpu
