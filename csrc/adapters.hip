@@ -251,7 +251,8 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
         } else {
             T* v = V + r * RP + (lane & 15);
 #pragma unroll
-            for (int t = 0; t < RT; ++t) v[t * 16] = (T)(acc[t][i] * sc);
+            for (int t = 0; t < RT; ++t)        // zeros behind R, where an infinity left NaN
+                v[t * 16] = (T)(t * 16 + (lane & 15) < R ? acc[t][i] * sc : 0.f);
             if (RT == 1) v[16] = (T)0.f;        // expand contracts 32 at a time
         }
     }
@@ -260,8 +261,8 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
 // The shares summed in a fixed order, scaled and rounded; four of a row's R a thread.  GR groups of
 // threads take every GR-th share where there are many (98 of 8192 rows, rank 32).
 template <typename T, int GR>
-__global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ part, long N, int R16,
-                                                    int splits, Rows rows, Scale scale,
+__global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ part, long N, int R,
+                                                    int R16, int splits, Rows rows, Scale scale,
                                                     T* __restrict__ V, int RP) {
     typedef T out4 __attribute__((ext_vector_type(4)));
     constexpr int TH = 256 / GR;
@@ -286,8 +287,10 @@ __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ pa
     }
     if (l < 0) return;
     const float sc = scale(l);
-    *(out4*)(V + row * RP + r) = out4{(T)(s[0] * sc), (T)(s[1] * sc), (T)(s[2] * sc),
-                                      (T)(s[3] * sc)};
+    out4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (T)(r + j < R ? s[j] * sc : 0.f);
+    *(out4*)(V + row * RP + r) = v;
 }
 
 // ---------------------------------------------------------------------------
@@ -893,7 +896,7 @@ void launch_shrink_sum(int type, int R, const int* order, const int* segs, const
     const long N = T * Bn, threads = N * (RP / 4);
 #define GO(T, GR)                                                                                \
     k_shrink_sum<T, GR><<<(unsigned)((threads + 256 / GR - 1) / (256 / GR)), 256, 0, st>>>(      \
-        part, N, R16, splits, rows, sc, (T*)V, RP)
+        part, N, R, R16, splits, rows, sc, (T*)V, RP)
     if (type == LM_BF16) {
         if (splits < 32) GO(bf16_t, 1);
         else GO(bf16_t, 8);

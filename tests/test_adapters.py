@@ -252,6 +252,30 @@ def test_kernel_other_rows_do_not_leak():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("R", [1, 5, 16, 31, 33, 100])
+@pytest.mark.parametrize("K", [40, 2000])
+def test_kernel_an_infinity_stays_one(K, R):
+    """An overflow is not turned into NaN by ranks that fill no tile."""
+    t, rows, _ = make(1, 70, K, 90, R, 2, dtype=torch.bfloat16, dev="cuda",
+                      index=[0] * 70)
+    t = {n: p.abs() + 0.01 for n, p in t.items()}
+    t["x"][0, 3, 1] = float("inf")
+    with torch.no_grad():
+        few = lowrank_add(t["y"][:, :4], t["x"][:, :4], t["a"], t["b"],
+                          AdapterRows([0] * 4, 2, device="cuda"))
+    assert (few[0, 3] == float("inf")).all()
+    v = {n: p.clone().requires_grad_() for n, p in t.items()}
+    out = lowrank_add(**v, rows=rows)
+    dy = torch.ones_like(out)
+    dy[0, 5, 7] = float("inf")
+    dx, = torch.autograd.grad(out, [v["x"]], dy)
+    assert (out[0, 3] == float("inf")).all()
+    assert (dx[0, 5] == float("inf")).all()
+    rest = [i for i in range(70) if i not in (3, 5)]
+    assert out[0, rest].isfinite().all() and dx[0, rest].isfinite().all()
+
+
+@pytest.mark.gpu
 def test_kernel_strides():
     t, rows, scale = make(1, 9, 50, 70, 6, 3, dtype=torch.bfloat16, dev="cuda")
     want = check_on_gpu(t, rows, scale)["out"]
