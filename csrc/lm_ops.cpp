@@ -5,6 +5,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
@@ -317,6 +318,16 @@ struct Grouped {
         for (const Tensor* t : {&order, &segs, &adapter}) {
             check_on(*t, x, "lowrank: the grouped rows");
             TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous(), "lowrank: rows int32");
+        }
+        // The rows may end with the call, or with the backward pass, and with a stream that is not
+        // theirs still at work: their memory waits for it.
+        const c10::impl::VirtualGuardImpl device(x.device().type());
+        const auto stream = device.getStream(x.device());
+        const Tensor* last = nullptr;
+        for (const Tensor* t : {&order, &segs, &adapter}) {     // parts of one storage, as a rule
+            if (!last || !t->is_alias_of(*last))
+                device.recordDataPtrOnStream(t->storage().data_ptr(), stream);
+            last = t;
         }
         type = type_of(x, "x");
         TORCH_CHECK(type != 2, "lowrank: bf16 or fp16");

@@ -338,6 +338,37 @@ def test_kernel_repeats_bitwise_on_another_stream():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_kernel_rows_may_end_before_another_stream_does(grad):
+    """Rows that nobody keeps, used on a stream that is not theirs: their
+    memory is not given away while that stream has work to do."""
+    t, rows, _ = make(4, 40, 64, 300, 8, 3, dtype=torch.bfloat16, dev="cuda")
+    index = list(rows.index)
+    want = lowrank_add(**t, rows=rows)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    if grad:
+        t["x"].requires_grad_()
+    dy = torch.ones_like(want)
+    for _ in range(3):
+        rows = AdapterRows(index, 3, device="cuda")
+        at = rows.segs.data_ptr()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(20_000_000)
+            out = lowrank_add(**t, rows=rows)
+            if grad:
+                torch.cuda._sleep(20_000_000)
+                torch.autograd.grad(out, t["x"], dy)
+        del rows
+        out = out.detach()
+        again = [AdapterRows(index, 3, device="cuda") for _ in range(4)]
+        assert all(r.segs.data_ptr() != at for r in again)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 30])
 def test_kernel_captured_and_replayed(T):
     shape = (T, 12, 200, 330, 16, 5)
