@@ -385,12 +385,17 @@ class LSTMModel(nn.Module):
                                device=prompt.device)
             seen[:, :Tp] = prompt.t()
 
+        done = None
+
         def ruled(logits, length):
             if rules is None:
                 return logits
             past = seen[:, :length]
-            allowed = [rules.allows(t, logits.shape[1])
-                       for t in past.tolist()] if rules.grammar else ()
+            allowed = ()
+            if rules.grammar:       # not asked about a finished column
+                ended = [False] * B if done is None else done.tolist()
+                allowed = [None if e else rules.allows(t, logits.shape[1])
+                           for t, e in zip(past.tolist(), ended)]
             return every.apply(logits, past, None, allowed)
 
         try:

@@ -67,6 +67,8 @@ class Trainer:
             self.model = self.model.to(self.dtype)
         self.teacher = teacher
         if teacher is not None:
+            if teacher is self.model:
+                raise ValueError("a model cannot be its own teacher")
             t, own = teacher.cfg, self.model.cfg
             if own.head == "none" or t.head != own.head or (
                     t.vocab_size if t.head == "lm" else t.num_classes) != (

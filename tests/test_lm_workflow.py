@@ -223,6 +223,25 @@ def test_grammars_that_fail_end_their_request_only():
         solo(m, [1, 2], 6, LogitRules(grammar=later))
 
 
+def test_grammar_is_not_asked_about_finished_columns():
+    """Columns of one batch end at different steps."""
+    m = LSTMModel(make_cfg())
+    ends = 7
+
+    def grammar(tokens):
+        if ends in tokens:
+            raise KeyError("asked behind the end")
+        ok = torch.zeros(30, dtype=torch.bool)
+        ok[ends if len(tokens) > tokens[0] else 1] = True
+        return ok
+
+    out = m.generate(torch.tensor([[2, 4, 3]]), 6, eos_token=ends,
+                     rules=LogitRules(grammar=grammar))
+    # the token behind as many as the first one says is the end
+    assert out[:6].t().tolist() == [[2, 1, 1, 7, 7, 7], [4, 1, 1, 1, 1, 7],
+                                    [3, 1, 1, 1, 7, 7]]
+
+
 def test_workflow_refusals():
     cfg = make_cfg()
     m, s = LSTMModel(cfg), make_set(cfg)
@@ -260,6 +279,8 @@ def test_workflow_refusals():
         m.distill_loss(torch.zeros(2, 3, 30), torch.zeros(2, 3, 31), None)
     with pytest.raises(ValueError):
         Trainer(Config(model=cfg), teacher=LSTMModel(make_cfg(vocab=31)))
+    with pytest.raises(ValueError):
+        Trainer(Config(model=cfg), model=m, teacher=m)
 
 
 def distill_config(dtype="fp32", bptt=4):
