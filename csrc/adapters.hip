@@ -17,6 +17,8 @@
 // `order[start, start + count)`, and its T * count rows are enumerated time-major.
 #include "lm_common.h"
 
+#include <algorithm>
+
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -43,7 +45,7 @@ template <typename T> DEVINL typename Frag<T>::type eight(const T* p, long e, lo
                               *(const typename Vec8<T>::type*)(p + min(e, limit - 8)));
 }
 // The same of a matrix that is read once in whole lines and need not stay in the caches: outer's
-// P (65536 rows of 4096: 139 -> 103 us).  Not of base or x, whose lines several loads share, nor
+// P (65536 rows of 4096: 129 -> 104 us).  Not of base or x, whose lines several loads share, nor
 // of the distilled logits, which are written next (all three slower).
 template <typename T>
 DEVINL typename Frag<T>::type eight_once(const T* p, long e, long limit) {
@@ -63,6 +65,19 @@ template <typename F> DEVINL F trim(F v, long e, long limit, int left) {
     if (keep < 64) u = u2{u[0] & ((1ull << keep) - 1), 0};
     else if (keep < 128) u = u2{u[0], u[1] & ((1ull << (keep - 64)) - 1)};
     return __builtin_bit_cast(F, u);
+}
+
+// The bits of a vector's first `left` elements, and the vector without the others.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+DEVINL u32x4 first_bits(int left) {
+    u32x4 m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        m[i] = left >= 2 * i + 2 ? ~0u : left == 2 * i + 1 ? 0xffffu : 0u;
+    return m;
+}
+template <typename F> DEVINL F keep(F v, u32x4 m) {
+    return __builtin_bit_cast(F, __builtin_bit_cast(u32x4, v) & m);
 }
 
 // An operand whose contraction runs down the rows of an LDS tile: column c (lane & 15) of rows
@@ -233,7 +248,8 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
             const F a = *(const F*)(xt + (wave * 16 + (lane & 15)) * LX + s * 32 + g * 8);
 #pragma unroll
             for (int t = 0; t < RT; ++t)
-                acc[t] = mfma(a, KCONT ? *(const F*)(w + (t * 16 + (lane & 15)) * LD + s * 32 + g * 8)
+                acc[t] = mfma(a,
+                              KCONT ? *(const F*)(w + (t * 16 + (lane & 15)) * LD + s * 32 + g * 8)
                                        : column_frag(w, LD, s * 32, t * 16 + own_columns()),
                               acc[t]);
         }
@@ -354,7 +370,7 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
     // a lane's share of base and out: eight columns of every eighth row
     const int m = strip + (tid & 31) * 8;
     const bool whole = m + 8 <= M;
-    F y[4];
+    F y[4], v[2][RK];
     auto load_base = [&](long j0) {
         if (!base) return;
 #pragma unroll
@@ -363,7 +379,6 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
             y[i] = eight(base, at[(j < jend ? j : jend - 1) - f.j0] * bs + m, blimit);
         }
     };
-    F v[2][RK];
     auto load_rows = [&](long j0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -382,34 +397,56 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
             for (int t = 0; t < 4; ++t)
                 w[k][t] = column_frag(wt, LD, k * 32, wave * 64 + t * 16 + own_columns());
     }
-    for (long j0 = f.j0; j0 < jend; j0 += 32) {
-        f32x4 acc[2][4];
-        F b[4];
+    auto multiply = [&](f32x4 (&acc)[2][4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = y[i];
-        if (mine) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int t = 0; t < 4; ++t) {
+                acc[h][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    acc[h][t] = f32x4{0, 0, 0, 0};
+                for (int k = 0; k < RK; ++k) acc[h][t] = mfma(w[k][t], v[h][k], acc[h][t]);
+            }
+    };
+    auto to_lds = [&](const f32x4 (&acc)[2][4]) {
 #pragma unroll
-                    for (int k = 0; k < RK; ++k) acc[h][t] = mfma(w[k][t], v[h][k], acc[h][t]);
-                }
-        }
-        if (j0 + 32 < jend) {
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                *(f32x4*)(sums + (h * 16 + (lane & 15)) * LS + wave * 64 + t * 16 + g * 4) =
+                    acc[h][t];
+    };
+    long j0 = f.j0;
+    // Whole steps: loads and stores without a condition, so that a wait for a load counts exactly
+    // the younger ones and does not drain the stores.
+    if (mine && strip + 256 <= M) {
+        for (; j0 + 32 <= jend; j0 += 32) {
+            f32x4 acc[2][4];
+            multiply(acc);
+            __syncthreads();                    // W, or the last step's products, are read
+            to_lds(acc);
+            load_rows(j0 + 32);
+            __syncthreads();
+            U8 o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int n = i * 8 + (tid >> 5);
+                const f32x4 lo = *(const f32x4*)(sums + n * LS + (tid & 31) * 8);
+                const f32x4 hi = *(const f32x4*)(sums + n * LS + (tid & 31) * 8 + 4);
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    o[i][q] = (T)((base ? (float)y[i][q] : 0.f) + (q < 4 ? lo[q & 3] : hi[q & 3]));
+            }
             load_base(j0 + 32);
-            if (mine) load_rows(j0 + 32);
-        }
-        __syncthreads();                        // W, or the last step's products, are read
-        if (mine) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    *(f32x4*)(sums + (h * 16 + (lane & 15)) * LS + wave * 64 + t * 16 + g * 4) =
-                        acc[h][t];
+            for (int i = 0; i < 4; ++i)
+                *(U8*)(out + at[j0 + i * 8 + (tid >> 5) - f.j0] * os + m) = o[i];
         }
+    }
+    for (; j0 < jend; j0 += 32) {
+        f32x4 acc[2][4];
+        if (mine) multiply(acc);
+        __syncthreads();
+        if (mine) to_lds(acc);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -425,16 +462,20 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
                 U8 o;
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    o[q] = (T)((base ? (float)b[i][q] : 0.f) + (q < 4 ? lo[q & 3] : hi[q & 3]));
+                    o[q] = (T)((base ? (float)y[i][q] : 0.f) + (q < 4 ? lo[q & 3] : hi[q & 3]));
                 *(U8*)(out + row * os + m) = o;
             } else {
-                const F was = trim(b[i], row * bs + m, blimit, M - m);
+                const F was = trim(y[i], row * bs + m, blimit, M - m);
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
                     if (m + q < M)
                         out[row * os + m + q] =
                             (T)((base ? (float)was[q] : 0.f) + (q < 4 ? lo[q & 3] : hi[q & 3]));
             }
+        }
+        if (j0 + 32 < jend) {
+            load_base(j0 + 32);
+            if (mine) load_rows(j0 + 32);
         }
     }
 }
@@ -588,14 +629,24 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
     constexpr int PV = 64 * PC / 8 / 256, PW = PC / 8;  // of P; a row's
     constexpr int D = C > 1 ? 2 : 1;                    // strips of P ahead
     F x[D][PV], q[QV];
-    // Rows of this step (for u), the next (loading) and the one behind it, divided out by one wave.
+    // Loads and stores end in the order they went out, and a wait for a load has to know how many
+    // are younger: so nothing in the loop goes out on a condition (rows behind the last are the
+    // last again), or the wait would drain all of them (8192 rows of 50000 in one group, a
+    // workgroup a CU: 280 us, now 215).
+    // Rows of this step (for u), the next (loading) and the one behind it: row t Bn + column.
     __shared__ int at[3][64];
-    auto find_rows = [&](long j0, int slot) {
+    auto find_row = [&](long j0, int& tb) {
         const long k = j0 + lane;
-        if (wave == 3) at[slot][lane] = (int)row_of(rows, f, k < jend ? k : jend - 1);
+        const unsigned j = (unsigned)(k < jend ? k : jend - 1), c = f.count, t = j / c;
+        tb = t * rows.Bn;
+        return rows.order[f.start + (j - t * c)];
     };
-    find_rows(f.j0, 0);
-    find_rows(f.j0 + 64, 1);
+    int tb, column;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        column = find_row(f.j0 + i * 64, tb);
+        if (wave == 3) at[i][lane] = tb + column;
+    }
     __syncthreads();
     int slot = 0;
     // a row's columns side by side over the lanes: rows of an odd width straddle few lines
@@ -614,25 +665,47 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
             q[i] = *(const F*)(Q + (long)at[slot][n] * RP + u % (RT * 2) * 8);
         }
     };
-    load(x[0], f.j0, 0, p0);
-    if (D > 1) load(x[D - 1], f.j0, 0, p0 + PC);
+    // u of a step goes out in the next one, before its loads; rows behind the last, and the first
+    // time all, to a row behind the shares that nobody reads.
+    f32x4 u[RT];
+    long to[4];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) u[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = (long)shares * N;
+    auto store_u = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float* v = partv + to[i] * (RT * 16) + (lane & 15);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                v[t * 16] = u[t][i];
+                u[t][i] = 0.f;
+            }
+        }
+    };
     load_q(f.j0, 0);
+    load(x[0], f.j0, 0, p0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (D > 1) load(x[D - 1], f.j0, 0, p0 + PC);
     for (long j0 = f.j0; j0 < jend; j0 += 64) {
         const int next = slot == 2 ? 0 : slot + 1, behind = next == 2 ? 0 : next + 1;
-        const bool more = j0 + 64 < jend;
-        f32x4 u[RT];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) u[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < C; ++k) {
             __syncthreads();
-            // columns behind the last and rows behind the tile's are zero on both sides
-            const bool edge = p0 + (k + 1) * PC > NP || !(j0 + 64 <= jend);
+            // Columns behind the last and rows behind the tile's are zero.  A strip that ends early
+            // masks its columns (trimming them held its workgroups, and with them the launch, up by
+            // half); the last rows of the tile, and of the matrix, are trimmed.
+            const bool tail = j0 + 64 > jend;
+            const bool close = tail || __builtin_amdgcn_readfirstlane(at[slot][63]) * ps + p0 +
+                                               (k + 1) * PC > plimit;
+            const u32x4 mask = first_bits(NP - p0 - k * PC - tid % PW * 8);
 #pragma unroll
             for (int i = 0; i < PV; ++i) {
                 const int n = i * (256 / PW) + tid / PW, c = p0 + k * PC + tid % PW * 8;
                 F v = x[k % D][i];
-                if (edge) v = trim(v, at[slot][n] * ps + c, plimit, j0 + n < jend ? NP - c : 0);
+                if (close) v = trim(v, at[slot][n] * ps + c, plimit, j0 + n < jend ? NP - c : 0);
+                else if (p0 + (k + 1) * PC > NP) v = keep(v, mask);
                 *(F*)(pt + n * LP + tid % PW * 8) = v;
             }
             if (k == 0)
@@ -641,13 +714,17 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
                     const int u = i * 256 + tid, n = u / (RT * 2);
                     if (n >= 64) continue;
                     F v = q[i];
-                    if (edge) v = trim(v, 0, 8, j0 + n < jend ? 8 : 0);
+                    if (tail) v = trim(v, 0, 8, j0 + n < jend ? 8 : 0);
                     *(F*)(qt + n * LQ + u % (RT * 2) * 8) = v;
                 }
             __syncthreads();
+            if (k == 0) {
+                if (DV) store_u();
+                column = find_row(j0 + 128, tb);
+                load_q(j0 + 64, next);
+            }
             if (k + D < C) load(x[k % D], j0, slot, p0 + (k + D) * PC);
-            else if (more) load(x[k % D], j0 + 64, next, p0 + (k + D - C) * PC);
-            if (k + 1 == C && more) load_q(j0 + 64, next);
+            else load(x[k % D], j0 + 64, next, p0 + (k + D - C) * PC);
             if (DV) {           // a wave takes 16 of the rows
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
@@ -676,15 +753,13 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int n = wave * 16 + g * 4 + i;
-                if (j0 + n >= jend) continue;
-                float* v = partv + ((long)share * N + at[slot][n]) * (RT * 16) + (lane & 15);
-#pragma unroll
-                for (int t = 0; t < RT; ++t) v[t * 16] = u[t][i];
+                to[i] = j0 + n < jend ? (long)share * N + at[slot][n] : (long)shares * N;
             }
         }
-        find_rows(j0 + 128, behind);
+        if (wave == 3) at[behind][lane] = tb + column;
         slot = next;
     }
+    if (DV) store_u();
     if (whole) {                // the adapter's only tile: its gradient, rounded here
         T* o = whole + (long)f.adapter * NP * R;
 #pragma unroll
@@ -692,14 +767,21 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int t = 0; t < RT; ++t)
+                for (int t = 0; t < RT; ++t) {
+                    typedef T out4 __attribute__((ext_vector_type(4), aligned(2)));
+                    const int p = p0 + k * PC + (wave * CT + c) * 16 + g * 4;
+                    const int r = t * 16 + (lane & 15);
+                    const f32x4 v = acc[k][c][t];
+                    if (r >= R) continue;
+                    if (!rcont && p + 4 <= NP) {
+                        *(out4*)(o + (long)r * NP + p) = out4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int p = p0 + k * PC + (wave * CT + c) * 16 + g * 4 + i;
-                        const int r = t * 16 + (lane & 15);
-                        if (p < NP && r < R)
-                            o[rcont ? (long)p * R + r : (long)r * NP + p] = (T)acc[k][c][t][i];
+                        for (int i = 0; i < 4; ++i)
+                            if (p + i < NP)
+                                o[rcont ? (long)(p + i) * R + r : (long)r * NP + p + i] = (T)v[i];
                     }
+                }
         return;
     }
     const int LO = shares * C * PC;
@@ -775,7 +857,8 @@ int tiles_of(const long* counts, int S, long T, int shift) {
 int r16_of(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
 template <typename T, bool KCONT>
-void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int K, int R, const Rows& rows, int tiles,
+void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int K, int R,
+            const Rows& rows, int tiles,
             const Scale& scale, void* V, int RP, float* part, long N, int splits, int kper,
             hipStream_t st) {
 #define GO(RT)                                                                                   \
@@ -792,7 +875,8 @@ void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int
 
 template <typename T, bool RCONT>
 void expand(const void* base, long bs, long blimit, void* out, long os, const void* V, int RP,
-            const void* W, long wlimit, int M, int R, const Rows& rows, int tiles, int shift, hipStream_t st) {
+            const void* W, long wlimit, int M, int R, const Rows& rows, int tiles, int shift,
+                hipStream_t st) {
     const int strips = (M + 255) / 256;
 #define GO(RK)                                                                                   \
     k_expand<T, RK, RCONT><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
@@ -817,7 +901,8 @@ int outer_columns(int R, int with_u, long row_tiles, int NP) {
 // `whole`: every adapter's rows are one tile, and out holds zeros for those without rows.
 template <typename T, bool RCONT>
 void outer(const void* P, long ps, long plimit, int NP, const void* Q, int RP, float* part,
-           const void* W, long wlimit, float* partv, long N, const Rows& rows, int tiles, int shift, int columns, int whole,
+           const void* W, long wlimit, float* partv, long N, const Rows& rows, int tiles,
+               int shift, int columns, int whole,
            void* out, int R, int L, hipStream_t st) {
     const int PC = columns, strips = (NP + PC - 1) / PC, R16 = r16_of(R);
 #define GO(RT, CT, NS)                                                                           \
@@ -876,14 +961,18 @@ void launch_shrink(int type, int kcont, const void* X, long xs, long xlimit, con
     const long N = T * Bn;
     const int RP = lowrank_rp(R);
     if (type == LM_BF16)
-        kcont ? shrink<bf16_t, true>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part, N, splits,
+        kcont ? shrink<bf16_t, true>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part,
+                                     N, splits,
                                      kper, st)
-              : shrink<bf16_t, false>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part, N, splits,
+              : shrink<bf16_t, false>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP,
+                                      part, N, splits,
                                       kper, st);
     else
-        kcont ? shrink<f16_t, true>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part, N, splits, kper,
+        kcont ? shrink<f16_t, true>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part,
+                                    N, splits, kper,
                                     st)
-              : shrink<f16_t, false>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part, N, splits,
+              : shrink<f16_t, false>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part,
+                                     N, splits,
                                      kper, st);
 }
 
@@ -908,7 +997,8 @@ void launch_shrink_sum(int type, int R, const int* order, const int* segs, const
 }
 
 void launch_expand(int type, int rcont, const void* base, long bs, long blimit, void* out,
-                   long os, const void* V, const void* W, long wlimit, int M, int R, const int* order, const int* segs,
+                   long os, const void* V, const void* W, long wlimit, int M, int R,
+                       const int* order, const int* segs,
                    const int* adapter, const long* counts, int S, int Bn, long T,
                    hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
@@ -919,11 +1009,15 @@ void launch_expand(int type, int rcont, const void* base, long bs, long blimit, 
     const int tiles = tiles_of(counts, S, T, shift), RP = lowrank_rp(R);
     if (tiles == 0) return;
     if (type == LM_BF16)
-        rcont ? expand<bf16_t, true>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows, tiles, shift, st)
-              : expand<bf16_t, false>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows, tiles, shift, st);
+        rcont ? expand<bf16_t, true>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows,
+                                     tiles, shift, st)
+              : expand<bf16_t, false>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows,
+                                      tiles, shift, st);
     else
-        rcont ? expand<f16_t, true>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows, tiles, shift, st)
-              : expand<f16_t, false>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows, tiles, shift, st);
+        rcont ? expand<f16_t, true>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows,
+                                    tiles, shift, st)
+              : expand<f16_t, false>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows,
+                                     tiles, shift, st);
 }
 
 // A decode step: W passes twice on the average at most, four rows a pass.  16 adapters at the
@@ -960,21 +1054,24 @@ int lowrank_outer_whole(const long* counts, int S, long T, int shift) {
 }
 // log2 of the rows that one partial gradient sums, 64 (a step) to 4096: the least time by what
 // was measured, in us.  A workgroup takes 6 to come and go, and a step of 64 rows 1.2, or what it
-// reads at 25 GB/s by itself, or at its share of 5 TB/s; rounds of the workgroups that fit the chip count whole; the partial gradients are
-// written and read again by a launch of 4, which one tile an adapter does without.  65536 rows of
-// 4096 columns, rank 16: 512 rows; 8192 of 50000, rank 32, in four groups: 1024; 1073 of 2049 in
-// seven: one tile each.
+// reads at 25 GB/s by itself, or at its share of 5 TB/s; rounds of the workgroups that fit the
+// chip count whole; the partial gradients are written and read again by a launch of 4, which one
+// tile an adapter does without.  65536 rows of 4096 columns, rank 16: 1024 rows; 8192 of 50000,
+// rank 32, in four groups, and 1073 of 2049 in seven: one tile each.
 int lowrank_outer_shift(const long* counts, int S, long T, int strips, int columns, int R) {
     const double fit = columns > 256 ? 512 : 1024, R16 = r16_of(R);
     int best = 6;
     double least = 1e300;
+    long most = 0;              // rows of an adapter
+    for (int s = 0; s < S; ++s) most = std::max(most, T * counts[s]);
     for (int shift = 12; shift >= 6; --shift) {
         const double blocks = (double)tiles_of(counts, S, T, shift) * strips;
         const double at_once = blocks < fit ? blocks : fit;
         const double alone = columns * 128 / 2.5e4 > 1.2 ? columns * 128 / 2.5e4 : 1.2;
+        const double steps = (double)((std::min(1l << shift, most) + 63) >> 6);
         const double step = columns * 128 * at_once / 5e6;
         double us = (double)(long)((blocks + fit - 1) / fit) *
-                    (6 + (1 << (shift - 6)) * (step > alone ? step : alone));
+                    (6 + steps * (step > alone ? step : alone));
         if (!lowrank_outer_whole(counts, S, T, shift)) us += 4 + blocks * columns * R16 * 8 / 5e6;
         if (us < least) {
             least = us;
@@ -991,21 +1088,26 @@ int lowrank_outer_tiles(const long* counts, int S, long T, int shift) {
 int lowrank_one_reading(int R) { return R <= 32; }
 
 void launch_outer(int type, int rcont, const void* P, long ps, long plimit, int NP,
-                  const void* Q, float* part, const void* W, long wlimit, float* partv, const int* order, const int* segs,
+                  const void* Q, float* part, const void* W, long wlimit, float* partv,
+                      const int* order, const int* segs,
                   const int* adapter, const long* counts, int S, int Bn, long T, int shift,
                   int columns, int whole, void* out, int R, int L, hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const int tiles = tiles_of(counts, S, T, shift), RP = lowrank_rp(R);
     const long N = T * Bn;
     if (type == LM_BF16)
-        rcont ? outer<bf16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
+        rcont ? outer<bf16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows,
+                                    tiles, shift,
                                     columns, whole, out, R, L, st)
-              : outer<bf16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
+              : outer<bf16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows,
+                                     tiles, shift,
                                      columns, whole, out, R, L, st);
     else
-        rcont ? outer<f16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
+        rcont ? outer<f16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows,
+                                   tiles, shift,
                                    columns, whole, out, R, L, st)
-              : outer<f16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows, tiles, shift,
+              : outer<f16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows,
+                                    tiles, shift,
                                     columns, whole, out, R, L, st);
 }
 

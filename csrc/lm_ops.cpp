@@ -44,8 +44,8 @@ void launch_expand(int, int, const void*, long, long, void*, long, const void*, 
                    int, int, const int*, const int*, const int*, const long*, int, int, long,
                    hipStream_t);
 void launch_outer(int, int, const void*, long, long, int, const void*, float*, const void*, long,
-                  float*, const int*, const int*, const int*, const long*, int, int, long, int, int, int,
-                  void*, int, int, hipStream_t);
+                  float*, const int*, const int*, const int*, const long*, int, int, long, int,
+                  int, int, void*, int, int, hipStream_t);
 }
 
 namespace {
@@ -220,7 +220,9 @@ Tensor per_row(const OptTensor& t, const Tensor& logits, const char* name) {
     check_on(*t, logits, name);
     return t->to(at::kFloat).contiguous();
 }
-const float* float_ptr(const Tensor& t) { return t.defined() ? (const float*)t.data_ptr() : nullptr; }
+const float* float_ptr(const Tensor& t) {
+    return t.defined() ? (const float*)t.data_ptr() : nullptr;
+}
 
 Tensor adjust(Tensor logits, OptTensor history, OptTensor lengths, OptTensor prompts,
               OptTensor repetition, double repetition_all, OptTensor presence,
@@ -362,7 +364,8 @@ struct Grouped {
     }
     static Tensor readable(const Tensor& t) {
         if (!t.defined() || room(t) >= 8) return t;
-        Tensor copy = at::zeros({t.numel() + 8}, t.options()).narrow(0, 0, t.numel()).view(t.sizes());
+        Tensor copy =
+            at::zeros({t.numel() + 8}, t.options()).narrow(0, 0, t.numel()).view(t.sizes());
         return copy.copy_(t);
     }
     const int* ip(const Tensor& t) const { return (const int*)t.data_ptr(); }
@@ -425,16 +428,19 @@ struct Grouped {
         const int shift = lowrank_outer_shift(counts.data(), S, T, strips, columns, R);
         const long tiles = lowrank_outer_tiles(counts.data(), S, T, shift);
         const bool whole = lowrank_outer_whole(counts.data(), S, T, shift);
-        // one workspace: the gradient's parts, u's shares
+        // one workspace: the gradient's parts, u's shares and a row for what belongs to no row
         const long parts = whole ? 0 : tiles * rp * strips * columns;
-        auto work = at::empty({parts + (u ? strips * N * rp : 0)}, p.options().dtype(at::kFloat));
+        auto work = at::empty({parts + (u ? (strips * N + 1) * rp : 0)},
+                              p.options().dtype(at::kFloat));
         float* part = (float*)work.data_ptr();
         const std::vector<int64_t> size = rcont ? std::vector<int64_t>{L, np, R}
                                                 : std::vector<int64_t>{L, R, np};
         // an adapter without rows has no tile to write its zeros
-        auto out = whole && groups < L ? at::zeros(size, p.options()) : at::empty(size, p.options());
+        auto out = whole && groups < L ? at::zeros(size, p.options())
+                                       : at::empty(size, p.options());
         launch_outer(type, rcont, p.data_ptr(), row_stride(p), room(p), np, q.data_ptr(),
-                     part, u ? w.data_ptr() : nullptr, u ? room(w) : 8, u ? part + parts : nullptr, ip(order), ip(segs), ip(adapter),
+                     part, u ? w.data_ptr() : nullptr, u ? room(w) : 8,
+                     u ? part + parts : nullptr, ip(order), ip(segs), ip(adapter),
                      counts.data(), S, Bn, T, shift, columns, whole, out.data_ptr(), R, L, st);
         if (u) {
             *u = at::empty({N, (long)rp}, p.options());

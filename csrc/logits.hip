@@ -7,9 +7,9 @@
 //   z3 = z2 + sum of the biases that the row lists for the token
 //   out = allowed ? z3 : -inf
 //
-// ONE launch without state between steps: a workgroup owns 2048 (8192) neighbouring columns of a row,
-// counts the history's tokens that fall into them in LDS (whole-number atomics, so the order
-// does not matter), and streams its columns once.  Each workgroup of a row reads the row's
+// ONE launch without state between steps: a workgroup owns 2048 (8192) neighbouring columns of a
+// row, counts the history's tokens that fall into them in LDS (whole-number atomics, so the
+// order does not matter), and streams its columns once.  Each workgroup of a row reads the row's
 // history again, from L2: a few KB beside its own columns.
 #include "lm_common.h"
 
