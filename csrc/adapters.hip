@@ -488,6 +488,21 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
 // ---------------------------------------------------------------------------
 constexpr int FEW = 2;      // log2 rows a wave
 
+// v = s x A of the rows `at`, rounded to the type, from the shares of x A.
+template <typename T>
+DEVINL void sum_shares(const float* __restrict__ part, const int* at, int n, long N, int R16,
+                       int splits, float scale, float* v, T) {
+    for (int u = threadIdx.x; u < n * R16; u += 64) {
+        const int i = u / R16, r = u - i * R16;
+        const float* p = part + (long)at[i] * R16 + r;
+        float s = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < splits; ++k) s += p[(long)k * N * R16];
+        v[i * 128 + r] = (float)(T)(s * scale);
+    }
+    __syncthreads();
+}
+
 template <typename T>
 __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* out, long os,
                                                    const float* __restrict__ part, long N, int R16,
@@ -497,6 +512,7 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
     constexpr int NR = 1 << FEW, U = 16;
     typedef typename Vec8<T>::type U8;
     __shared__ float v[NR * 128];
+    __shared__ int at[NR];
     const int lane = threadIdx.x;
     const Tile f = find_tile(rows, blockIdx.x / strips, FEW);
     const bool mine = f.adapter >= 0;
@@ -506,34 +522,30 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
     // own; lanes behind it take them too and store nothing.
     const bool whole = M >= 8;
     const int m = whole && own > M - 8 ? M - 8 : own;
-    long row[NR];
+    // What is read goes out without conditions (a row behind the last is the first again), the
+    // rows' numbers first: W is on its way while they come, base and V while W does.
+    const unsigned j = (unsigned)f.j0 + (lane < n ? lane : 0), c = f.count, t = j / c;
+    const int column = rows.order[f.start + (j - t * c)];
+    const T* Wl = W + (long)(mine ? f.adapter : 0) * M * R + m;
+    U8 w[U];
+    auto load = [&](int r0) {
 #pragma unroll
-    for (int i = 0; i < NR; ++i) row[i] = row_of(rows, f, f.j0 + (i < n ? i : 0));
-    float acc[NR][8] = {};
-    U8 y[NR], w[U];
-    // base and the first of W are on their way before V is known
-#pragma unroll
-    for (int i = 0; i < NR; ++i)
-        if (whole && i < n) y[i] = *(const U8*)(base + row[i] * bs + m);
-    if (mine) {
-        const T* Wl = W + (long)f.adapter * M * R + m;
-        auto load = [&](int r0) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (whole && r0 + u < R) w[u] = *(const U8*)(Wl + (long)(r0 + u) * M);
-        };
+        for (int u = 0; u < U; ++u) w[u] = *(const U8*)(Wl + (long)min(r0 + u, R - 1) * M);
+    };
+    if (whole) {
         load(0);
-        const float sc = scale(f.adapter);
-        for (int u = lane; u < n * R16; u += 64) {
-            const int i = u / R16, r = u - i * R16;
-            const float* p = part + row_of(rows, f, f.j0 + i) * R16 + r;
-            float s = 0.f;
-#pragma unroll 8
-            for (int k = 0; k < splits; ++k) s += p[(long)k * N * R16];
-            v[i * 128 + r] = (float)(T)(s * sc);
-        }
+        if (lane < NR) at[lane] = (int)t * rows.Bn + column;
         __syncthreads();
-        if (whole) {
+        long row[NR];
+        U8 y[NR];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            row[i] = at[i];
+            y[i] = *(const U8*)(base + row[i] * bs + m);
+        }
+        float acc[NR][8] = {};
+        if (mine) {
+            sum_shares(part, at, n, N, R16, splits, scale(f.adapter), v, T());
             for (int r0 = 0; r0 < R; r0 += U) {
                 if (r0) load(r0);
 #pragma unroll
@@ -546,21 +558,10 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
                                 for (int q = 0; q < 8; ++q)
                                     acc[i][q] += v[i * 128 + r0 + u] * (float)w[u][q];
             }
-        } else if (m < M) {
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const float x = m + q < M ? (float)Wl[(long)r * M + q] : 0.f;
-#pragma unroll
-                    for (int i = 0; i < NR; ++i)
-                        if (i < n) acc[i][q] += v[i * 128 + r] * x;
-                }
         }
-    }
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-        if (i >= n) continue;
-        if (whole) {
+        for (int i = 0; i < NR; ++i) {
+            if (i >= n) continue;
             float o[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) o[q] = (float)y[i][q] + acc[i][q];
@@ -569,13 +570,19 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
                     if (m + q >= own) out[row[i] * os + m + q] = (T)o[q];
-        } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                if (m + q < M)
-                    out[row[i] * os + m + q] = (T)((float)base[row[i] * bs + m + q] + acc[i][q]);
         }
+        return;
     }
+    if (lane < NR) at[lane] = (int)t * rows.Bn + column;
+    __syncthreads();
+    if (mine) sum_shares(part, at, n, N, R16, splits, scale(f.adapter), v, T());
+    for (int i = 0; i < n; ++i)
+        for (int q = lane; q < M; q += 64) {            // fewer than eight columns
+            float s = (float)base[at[i] * bs + q];
+            if (mine)
+                for (int r = 0; r < R; ++r) s += v[i * 128 + r] * (float)Wl[(long)r * M + q - m];
+            out[at[i] * os + q] = (T)s;
+        }
 }
 
 // ---------------------------------------------------------------------------
