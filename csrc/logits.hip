@@ -137,8 +137,9 @@ __global__ __launch_bounds__(TH) void k_adjust(const T* __restrict__ logits, lon
 
 template <typename T>
 void go(const void* z, long zs, void* out, const Adjust& a, long B, int V, hipStream_t stream) {
-    // Every workgroup of a row reads its whole history: a long one by a quarter as many (64 rows
-    // with 16384 tokens 27 -> 16 us; with 1024 tokens 9.8 and 10.2, with 64 on 257 rows 20 and 17).
+    // Every workgroup of a row reads its whole history: a long one by a quarter as many (columns of
+    // 2048 and of 8192, 64 rows of 50000: 16384 tokens 27 and 16 us, 4096 12.7 and 10.4, 1024 10.3
+    // and 10.0; 1024 rows: 4096 tokens 105 and 97, 1024 75 and 92).
     const int small = (V + 2047) / 2048, large = (V + 8191) / 8192;
     if (a.L >= 4096)
         k_adjust<T, 1024><<<(unsigned)(B * large), 1024, 0, stream>>>((const T*)z, zs, (T*)out, a,
