@@ -300,6 +300,35 @@ def test_kernel_strides():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,K,M,R", [(64, 70, 300, 16), (128, 257, 257, 5),
+                                     (100, 33, 1031, 40), (65, 9, 511, 128),
+                                     (3, 300, 1025, 16)])
+def test_kernel_what_lies_behind_the_rows_is_not_used(B, K, M, R):
+    """Rows inside wider ones whose other columns hold NaN: the same bits."""
+    t, rows, scale = make(1, B, K, M, R, 3, dtype=torch.bfloat16, dev="cuda")
+    g = torch.Generator().manual_seed(5)
+    t["dy"] = torch.randn(1, B, M, generator=g).to(t["y"])
+
+    def inside(p):
+        wide = torch.full((1, B, p.shape[-1] + 19), float("nan"),
+                          device="cuda", dtype=p.dtype)
+        wide[..., 6:6 + p.shape[-1]] = p
+        return wide[..., 6:6 + p.shape[-1]]
+
+    got = []
+    for put in (lambda p: p, inside):
+        v = {n: put(t[n]).detach().requires_grad_() for n in "yx"}
+        v.update({n: t[n].clone().requires_grad_() for n in "ab"})
+        out = lowrank_add(**v, rows=rows, scale=scale)
+        got.append((out, *torch.autograd.grad(out, list(v.values()),
+                                              put(t["dy"]))))
+        with torch.no_grad():
+            got[-1] += (lowrank_add(**v, rows=rows, scale=scale),)
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+    assert all(p.isfinite().all() for p in got[0])
+
+
+@pytest.mark.gpu
 def test_kernel_some_gradients_only():
     for R in (8, 40):
         t, rows, scale = make(20, 6, 80, 90, R, 3, dtype=torch.bfloat16,
