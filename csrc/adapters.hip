@@ -947,22 +947,24 @@ extern "C" {
 // Row length of v and u: the contraction of expand, in steps of 32.
 int lowrank_rp(int R) { return R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
-// Workgroups that share a row tile's contraction: about two a CU, no share below a step.
-int lowrank_splits(const long* counts, int S, long T, int K) {
-    const int tiles = tiles_of(counts, S, T, S_TM), most = (K + S_KC - 1) / S_KC;
-    int want = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
-    return want < 1 ? 1 : want > most ? most : want;
+// Workgroups that share a row tile's contraction: about two a CU, no share below a step.  Up to
+// `alone` steps stay with one: where the sum is a launch of its own, four do (8192 rows of 1024,
+// rank 32: 10.4 us, 8.2 + 5.2 in four shares; eight take 11.9, and 6.4 + 3.8 in eight).
+int lowrank_splits(const long* counts, int S, long T, int K, int alone) {
+    const int tiles = tiles_of(counts, S, T, S_TM), steps = (K + S_KC - 1) / S_KC;
+    const int want = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
+    return steps <= alone ? 1 : want > steps ? steps : want;
 }
 
 // With `part` (splits, N, R16) the shares are left there unscaled and V is not written.
 void launch_shrink(int type, int kcont, const void* X, long xs, long xlimit, const void* W,
-                   long wlimit, int K, int R,
-                   const int* order, const int* segs, const int* adapter, const long* counts,
-                   int S, int Bn, long T, const float* scale, float scale_all, void* V,
-                   float* part, hipStream_t st) {
+                   long wlimit, int K, int R, const int* order, const int* segs,
+                   const int* adapter, const long* counts, int S, int Bn, long T,
+                   const float* scale, float scale_all, void* V, float* part, int splits,
+                   hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const Scale sc{scale, scale_all};
-    const int tiles = tiles_of(counts, S, T, S_TM), splits = lowrank_splits(counts, S, T, K);
+    const int tiles = tiles_of(counts, S, T, S_TM);
     if (tiles == 0) return;
     const int kper = ((K + splits - 1) / splits + S_KC - 1) / S_KC * S_KC;
     const long N = T * Bn;

@@ -25,7 +25,7 @@ void launch_adjust(int, const void*, long, void*, const void*, long, int, int, c
                    float, const void*, long, int, const float*, long, int, const unsigned*, long,
                    long, int, hipStream_t);
 int lowrank_rp(int R);
-int lowrank_splits(const long* counts, int S, long T, int K);
+int lowrank_splits(const long* counts, int S, long T, int K, int alone);
 int lowrank_outer_columns(const long* counts, int S, long T, int NP, int R, int with_u);
 int lowrank_outer_shift(const long* counts, int S, long T, int strips, int columns, int R);
 int lowrank_few(const long* counts, int S, long T);
@@ -37,7 +37,7 @@ int lowrank_outer_tiles(const long* counts, int S, long T, int shift);
 int lowrank_one_reading(int R);
 void launch_shrink(int, int, const void*, long, long, const void*, long, int, int, const int*,
                    const int*, const int*, const long*, int, int, long, const float*, float,
-                   void*, float*, hipStream_t);
+                   void*, float*, int, hipStream_t);
 void launch_shrink_sum(int, int, const int*, const int*, const int*, int, int, long, const float*,
                        float, void*, const float*, int, hipStream_t);
 void launch_expand(int, int, const void*, long, long, void*, long, const void*, const void*, long,
@@ -373,7 +373,7 @@ struct Grouped {
     // v (N, RP) = s x W, W (L, K, R) or, contraction contiguous, (L, R, K)
     Tensor shrink(const Tensor& x_, const Tensor& w_, bool kcont, hipStream_t st) const {
         const Tensor x = readable(x_), w = readable(w_);
-        const int k = (int)x.size(1), splits = lowrank_splits(counts.data(), S, T, k);
+        const int k = (int)x.size(1), splits = lowrank_splits(counts.data(), S, T, k, 4);
         auto v = at::empty({N, (long)lowrank_rp(R)}, x.options());
         Tensor part;
         if (splits > 1)
@@ -381,7 +381,7 @@ struct Grouped {
         launch_shrink(type, kcont, x.data_ptr(), row_stride(x), room(x), w.data_ptr(), room(w),
                       k, R, ip(order),
                       ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
-                      v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, st);
+                      v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, splits, st);
         if (splits > 1) sum(v, (const float*)part.data_ptr(), splits, st);
         check_launch("lowrank shrink");
         return v;
@@ -394,12 +394,12 @@ struct Grouped {
     void few(const Tensor& base, Tensor& out, const Tensor& x_, const Tensor& a_, const Tensor& b,
              hipStream_t st) const {
         const Tensor x = readable(x_), a = readable(a_);
-        const int splits = lowrank_splits(counts.data(), S, T, K);
+        const int splits = lowrank_splits(counts.data(), S, T, K, 0);
         auto part = at::empty({(long)splits * N * lowrank_rp(R)}, x.options().dtype(at::kFloat));
         launch_shrink(type, 0, x.data_ptr(), row_stride(x), room(x), a.data_ptr(), room(a), K,
                       R, ip(order),
                       ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
-                      nullptr, (float*)part.data_ptr(), st);
+                      nullptr, (float*)part.data_ptr(), splits, st);
         launch_expand_few(type, base.data_ptr(), row_stride(base), out.data_ptr(),
                           row_stride(out), (const float*)part.data_ptr(), b.data_ptr(), M, R,
                           ip(order), ip(segs), ip(adapter), counts.data(), S, Bn, T,
