@@ -1,6 +1,7 @@
 // Host side of the operators around the language-model head: argument checks, workspaces and
-// launches of distill.hip, adapters.hip and logits.hip.  Python (ops/distill.py and its
-// neighbours) checks shapes with errors of its own; what a kernel relies on is checked here again.
+// launches of distill.hip, adapters.hip and logits.hip.  What a decode step calls checks its
+// tensors here alone, with the errors that Python (ops/logits.py, ops/adapters.py) raises for the
+// reference: a check there costs as much as a launch.
 #include "lm_ops.h"
 
 #include <ATen/ATen.h>
@@ -53,6 +54,10 @@ namespace {
 using at::Tensor;
 using OptTensor = c10::optional<Tensor>;
 
+// A refusal of an argument, Python's ValueError.
+#define REQUIRE(cond, ...) \
+    if (!(cond)) throw pybind11::value_error(c10::str(__VA_ARGS__))
+
 // The current stream of the tensors' own device (the caller holds a DeviceGuard on it).
 hipStream_t stream_of(const Tensor& t) {
     return c10::hip::getCurrentHIPStream(t.device().index()).stream();
@@ -76,18 +81,18 @@ int type_of(const Tensor& t, const char* name) {
         case at::kFloat: return 2;
         default: break;
     }
-    TORCH_CHECK(false, name, " must be bf16, fp16 or fp32, got ", t.scalar_type());
+    REQUIRE(false, name, " must be bf16, fp16 or fp32, got ", t.scalar_type());
+    return -1;
 }
 
 bool wide_index(const Tensor& t, const char* name) {
-    TORCH_CHECK(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, name,
-                " must be int32 or int64");
+    REQUIRE(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, name,
+            " must be int32 or int64");
     return t.scalar_type() == at::kLong;
 }
 
 void check_on(const Tensor& t, const Tensor& ref, const char* name) {
-    TORCH_CHECK(t.device() == ref.device(), name, " must be on ", ref.device(), ", got ",
-                t.device());
+    REQUIRE(t.device() == ref.device(), name, " must be on ", ref.device(), ", got ", t.device());
 }
 
 void check_launch(const char* name) {
@@ -216,7 +221,8 @@ Tensor distill_loss(Tensor logits, Tensor index, Tensor teacher, OptTensor targe
 // A per-request number as a (B,) tensor; the scalar beside it is used where there is none.
 Tensor per_row(const OptTensor& t, const Tensor& logits, const char* name) {
     if (!t.has_value()) return Tensor();
-    TORCH_CHECK(t->dim() == 1 && t->size(0) == logits.size(0), name, " must be (B,)");
+    REQUIRE(t->dim() == 1 && t->size(0) == logits.size(0) && t->is_floating_point(), name,
+            " must be a number or (B=", logits.size(0), ",) floating");
     check_on(*t, logits, name);
     return t->to(at::kFloat).contiguous();
 }
@@ -228,25 +234,26 @@ Tensor adjust(Tensor logits, OptTensor history, OptTensor lengths, OptTensor pro
               OptTensor repetition, double repetition_all, OptTensor presence,
               double presence_all, OptTensor frequency, double frequency_all,
               OptTensor bias_index, OptTensor bias, OptTensor allowed) {
-    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be (B, V) on GPU");
+    REQUIRE(logits.is_cuda() && logits.dim() == 2, "logits must be (B, V) on GPU, got ",
+            logits.sizes());
     const long B = logits.size(0), V = logits.size(1);
-    TORCH_CHECK(V <= (1 << 30) && B * ((V + 2047) / 2048) < (1l << 24),
-                "logits: V at most 2^30, and fewer than 2^24 parts of 2048 columns");
+    REQUIRE(V <= (1 << 30) && B * ((V + 2047) / 2048) < (1l << 24),
+            "logits: V at most 2^30, and fewer than 2^24 parts of 2048 columns");
+    const at::NoGradGuard off;
     const c10::DeviceGuard guard(logits.device());
     const int type = type_of(logits, "logits");
     const Tensor z = rows_of(logits);
     Tensor h, len, pre, bi, bv, ok;
     int h64 = 0, l64 = 0, p64 = 0, i64 = 0;
     if (history.has_value()) {
-        TORCH_CHECK(history->dim() == 2 && history->size(0) == B &&
-                        history->size(1) <= (1 << 30),
-                    "history must be (B, L)");
+        REQUIRE(history->dim() == 2 && history->size(0) == B && history->size(1) <= (1 << 30),
+                "history must be (B=", B, ", L), got ", history->sizes());
         check_on(*history, logits, "history");
         h64 = wide_index(*history, "history");
         h = rows_of(*history);
         auto per_request = [&](const OptTensor& t, Tensor& to, int& wide, const char* name) {
             if (!t.has_value()) return;
-            TORCH_CHECK(t->dim() == 1 && t->size(0) == B, name, " must be (B,)");
+            REQUIRE(t->dim() == 1 && t->size(0) == B, name, " must be (B=", B, ",)");
             check_on(*t, logits, name);
             wide = wide_index(*t, name);
             to = t->contiguous();
@@ -258,9 +265,10 @@ Tensor adjust(Tensor logits, OptTensor history, OptTensor lengths, OptTensor pro
                  pres = per_row(presence, logits, "presence"),
                  freq = per_row(frequency, logits, "frequency");
     if (bias_index.has_value()) {
-        TORCH_CHECK(bias.has_value() && bias_index->dim() == 2 && bias_index->size(0) == B &&
-                        bias->sizes() == bias_index->sizes() && bias->size(1) <= (1 << 30),
-                    "bias_index and bias must be (B, K)");
+        REQUIRE(bias.has_value() && bias_index->dim() == 2 && bias_index->size(0) == B &&
+                    bias->sizes() == bias_index->sizes() && bias->size(1) <= (1 << 30) &&
+                    bias->is_floating_point(),
+                "bias_index must be (B=", B, ", K) and bias floating of the same shape");
         check_on(*bias_index, logits, "bias_index");
         check_on(*bias, logits, "bias");
         i64 = wide_index(*bias_index, "bias_index");
@@ -268,9 +276,9 @@ Tensor adjust(Tensor logits, OptTensor history, OptTensor lengths, OptTensor pro
         bv = rows_of(bias->to(at::kFloat));
     }
     if (allowed.has_value()) {
-        TORCH_CHECK(allowed->dim() == 2 && allowed->size(0) == B &&
-                        allowed->size(1) == (V + 31) / 32 && allowed->scalar_type() == at::kInt,
-                    "allowed must be (B, ceil(V / 32)) int32");
+        REQUIRE(allowed->dim() == 2 && allowed->size(0) == B &&
+                    allowed->size(1) == (V + 31) / 32 && allowed->scalar_type() == at::kInt,
+                "allowed must be (B=", B, ", ", (V + 31) / 32, ") int32");
         check_on(*allowed, logits, "allowed");
         ok = rows_of(*allowed);
     }
@@ -305,20 +313,37 @@ struct Grouped {
             const OptTensor& scale_, double all)
         : order(order_), segs(segs_), adapter(adapter_), counts(counts_.begin(), counts_.end()),
           groups((int)groups_), scale_all((float)all) {
-        TORCH_CHECK(x.is_cuda() && x.dim() >= 2 && x.dim() == y.dim() &&
-                        x.sizes().slice(0, x.dim() - 1) == y.sizes().slice(0, y.dim() - 1),
-                    "lowrank: x (..., Bn, K) and y (..., Bn, M) on GPU");
-        TORCH_CHECK(a.dim() == 3 && b.dim() == 3 && a.size(0) == b.size(0) &&
-                        a.size(2) == b.size(1) && a.size(1) == x.size(-1) &&
-                        b.size(2) == y.size(-1),
-                    "lowrank: a (L, K, R), b (L, R, M)");
-        TORCH_CHECK(a.is_contiguous() && b.is_contiguous(), "lowrank: a and b contiguous");
+        REQUIRE(a.dim() == 3 && b.dim() == 3 && a.size(0) == b.size(0) && a.size(2) == b.size(1),
+                "a must be (L, K, R) and b (L, R, M), got ", a.sizes(), ", ", b.sizes());
+        REQUIRE(a.size(2) >= 1 && a.size(2) <= 128, "rank must be in [1, 128], got ", a.size(2));
+        REQUIRE(x.is_cuda() && x.dim() >= 2 && x.dim() == y.dim() &&
+                    x.sizes().slice(0, x.dim() - 1) == y.sizes().slice(0, y.dim() - 1) &&
+                    a.size(1) == x.size(-1) && b.size(2) == y.size(-1),
+                "x must be (..., B, ", a.size(1), ") and y (..., B, ", b.size(2), "), got ",
+                x.sizes(), ", ", y.sizes());
         for (const Tensor* t : {&y, &a, &b}) {
-            check_on(*t, x, "lowrank: every tensor");
-            TORCH_CHECK(t->scalar_type() == x.scalar_type(), "lowrank: one type for all");
+            check_on(*t, x, "every tensor");
+            REQUIRE(t->scalar_type() == x.scalar_type(),
+                    "y, x, a and b must have one floating type");
         }
+        type = type_of(x, "x");
+        REQUIRE(type != 2, "x must be bf16 or fp16");
+        L = (int)a.size(0);
+        K = (int)a.size(1);
+        R = (int)a.size(2);
+        M = (int)b.size(2);
+        if (scale_.has_value()) {
+            REQUIRE(scale_->dim() == 1 && scale_->size(0) == L && scale_->is_floating_point(),
+                    "scale must be a number or (L=", L, ",) floating");
+            REQUIRE(!scale_->requires_grad(), "scale gets no gradient: detach it");
+            check_on(*scale_, x, "scale");
+            scale = scale_->to(at::kFloat).contiguous();
+        }
+        Bn = (int)order.numel();
+        S = (int)counts.size();
+        REQUIRE(Bn == x.size(-2), "rows must be AdapterRows of ", x.size(-2), " columns");
         for (const Tensor* t : {&order, &segs, &adapter}) {
-            check_on(*t, x, "lowrank: the grouped rows");
+            check_on(*t, x, "rows");
             TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous(), "lowrank: rows int32");
         }
         // The rows may end with the call, or with the backward pass, and with a stream that is not
@@ -331,31 +356,18 @@ struct Grouped {
                 device.recordDataPtrOnStream(t->storage().data_ptr(), stream);
             last = t;
         }
-        type = type_of(x, "x");
-        TORCH_CHECK(type != 2, "lowrank: bf16 or fp16");
-        L = (int)a.size(0);
-        K = (int)a.size(1);
-        R = (int)a.size(2);
-        M = (int)b.size(2);
+        TORCH_CHECK(a.is_contiguous() && b.is_contiguous(), "lowrank: a and b contiguous");
         TORCH_CHECK(x.numel() > 0 && y.numel() > 0, "lowrank: no rows");
         N = x.numel() / K;
-        Bn = (int)order.numel();
-        S = (int)counts.size();
-        TORCH_CHECK(R >= 1 && R <= 128 && K >= 1 && M >= 1 && K < (1 << 30) && M < (1 << 30),
-                    "lowrank: a rank of 1 to 128");
-        TORCH_CHECK(segs.numel() == 4l * S && adapter.numel() == Bn && Bn > 0 && N % Bn == 0,
+        REQUIRE(K < (1 << 30) && M < (1 << 30), "rows of fewer than 2^30 elements");
+        TORCH_CHECK(segs.numel() == 4l * S && adapter.numel() == Bn && N % Bn == 0,
                     "lowrank: N rows of Bn columns");
         T = N / Bn;
         long sum = 0;
         for (long c : counts) sum += c;
-        TORCH_CHECK(groups <= S && groups >= S - 1, "lowrank: groups");
-        TORCH_CHECK(sum == Bn && N < (1l << 31) && N / 64 * ((std::max(K, M) + 127) / 128) <
-                        (1l << 31), "lowrank: too many rows");
-        if (scale_.has_value()) {
-            TORCH_CHECK(scale_->numel() == L && scale_->dim() == 1, "lowrank: scale (L,)");
-            check_on(*scale_, x, "scale");
-            scale = scale_->to(at::kFloat).contiguous();
-        }
+        TORCH_CHECK(groups <= S && groups >= S - 1 && sum == Bn, "lowrank: groups");
+        REQUIRE(N < (1l << 31) && N / 64 * ((std::max(K, M) + 127) / 128) < (1l << 31),
+                "too many rows");
     }
     // Elements of the storage from the tensor's first on: the kernels read eight at a time, past a
     // row's end if need be but never past this.  Where there are not even eight, in a copy.
@@ -525,7 +537,9 @@ struct LowRankAdd : public torch::autograd::Function<LowRankAdd> {
 
 Tensor lowrank_add(Tensor y, Tensor x, Tensor a, Tensor b, Tensor order, Tensor segs,
                    Tensor adapter, std::vector<int64_t> counts, int64_t groups, OptTensor scale,
-                   double scale_all, bool inplace) {
+                   double scale_all, bool inplace, int64_t adapters) {
+    REQUIRE(a.dim() >= 1 && a.size(0) == adapters, "rows are of ", adapters, " adapters, a is ",
+            a.sizes());
     if (!inplace && at::GradMode::is_enabled() &&
         (y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad()))
         return LowRankAdd::apply(y, x, a.contiguous(), b.contiguous(), order, segs, adapter,
@@ -534,7 +548,7 @@ Tensor lowrank_add(Tensor y, Tensor x, Tensor a, Tensor b, Tensor order, Tensor 
     const c10::DeviceGuard guard(x.device());
     const Tensor ac = a.contiguous(), bc = b.contiguous();
     const Grouped g(x, y, ac, bc, order, segs, adapter, counts, groups, scale, scale_all);
-    TORCH_CHECK(!inplace || y.is_contiguous(), "lowrank: y must be contiguous");
+    REQUIRE(!inplace || y.is_contiguous(), "y must be contiguous");
     // autograd has to see that y is another one now
     if (inplace && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
     return lowrank_forward(g, y, x, ac, bc, inplace, nullptr);
@@ -555,5 +569,5 @@ void register_lm_ops(pybind11::module_& m) {
     m.def("lowrank_add", &lowrank_add, "y + s x A B by rows' adapters", py::arg("y"),
           py::arg("x"), py::arg("a"), py::arg("b"), py::arg("order"), py::arg("segs"),
           py::arg("adapter"), py::arg("counts"), py::arg("groups"),
-          py::arg("scale") = py::none(), py::arg("scale_all") = 1.0, py::arg("inplace") = false);
+          py::arg("scale"), py::arg("scale_all"), py::arg("inplace"), py::arg("adapters"));
 }

@@ -95,17 +95,8 @@ def _ref_lowrank(y, x, a, b, rows: AdapterRows, scale):
     return out.to(y.dtype)
 
 
-def _launch_args(rows: AdapterRows, scale):
-    args = dict(order=rows.order, segs=rows.segs, adapter=rows.adapter,
-                counts=rows.counts, groups=rows.groups)
-    if isinstance(scale, torch.Tensor):
-        args["scale"] = scale
-    else:
-        args["scale_all"] = float(scale)
-    return args
-
-
 def _check(y, x, a, b, rows, scale):
+    """What the kernels' path refuses in csrc/lm_ops.cpp."""
     if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] \
             or a.shape[2] != b.shape[1]:
         raise ValueError("a must be (L, K, R) and b (L, R, M), got "
@@ -140,8 +131,22 @@ def _check(y, x, a, b, rows, scale):
         raise ValueError(f"rows are on {rows.device}, the tensors on {dev}")
 
 
-def _kernels(x: torch.Tensor) -> bool:
-    return extension.use_hip_lm(x) and x.dtype != torch.float32
+def _kernels(y, x) -> bool:
+    return extension.use_hip_lm(x) and x.dtype != torch.float32 \
+        and x.numel() > 0 and y.numel() > 0
+
+
+def _launch(y, x, a, b, rows, scale, inplace: bool):
+    if not isinstance(rows, AdapterRows):
+        raise ValueError("rows must be AdapterRows")
+    each = None
+    if isinstance(scale, torch.Tensor):
+        each, scale = scale, 1.0
+    elif not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    return extension.get_extension().lowrank_add(
+        y, x, a, b, rows.order, rows.segs, rows.adapter, rows.counts,
+        rows.groups, each, float(scale), inplace, rows.num_adapters)
 
 
 def lowrank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
@@ -153,24 +158,22 @@ def lowrank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
     y (..., B, M), x (..., B, K); a (L, K, R), b (L, R, M), R <= 128; rows of
     the B columns; scale a number or one for each adapter (L,), a constant.
     """
+    if _kernels(y, x):
+        return _launch(y, x, a, b, rows, scale, False)
     _check(y, x, a, b, rows, scale)
-    if not _kernels(x) or x.numel() == 0 or y.numel() == 0:
-        return _ref_lowrank(y, x, a, b, rows, scale)
-    return extension.get_extension().lowrank_add(
-        y, x, a, b, **_launch_args(rows, scale))
+    return _ref_lowrank(y, x, a, b, rows, scale)
 
 
-@torch.no_grad()
 def lowrank_add_(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
                  b: torch.Tensor, rows: AdapterRows,
                  scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
     """`lowrank_add` into a contiguous y itself, the serving form: rows
     without an adapter are not touched.  No gradient."""
+    if _kernels(y, x):
+        _launch(y, x, a, b, rows, scale, True)
+        return y
     _check(y, x, a, b, rows, scale)
     if not y.is_contiguous():
         raise ValueError("y must be contiguous")
-    if not _kernels(x) or x.numel() == 0 or y.numel() == 0:
+    with torch.no_grad():
         return y.copy_(_ref_lowrank(y, x, a, b, rows, scale))
-    extension.get_extension().lowrank_add(
-        y, x, a, b, inplace=True, **_launch_args(rows, scale))
-    return y

@@ -71,9 +71,11 @@ def use_hip(device: torch.device | str,
     return True
 
 
+_LM_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
 def use_hip_lm(t: torch.Tensor) -> bool:
     """Backend of the operators around the language-model head (distill,
     adapters, logits): their kernels take bf16, fp16 and, where an operator
     says so, fp32 on the GPU; the CPU and fp64 run the reference."""
-    return use_hip(t.device) and t.dtype in (
-        torch.bfloat16, torch.float16, torch.float32)
+    return t.is_cuda and t.dtype in _LM_TYPES and use_hip("cuda")

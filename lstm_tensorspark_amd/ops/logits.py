@@ -76,15 +76,47 @@ def _ref_adjust(logits, history, lengths, prompt_lengths, repetition,
     return z.to(logits.dtype)
 
 
-def _per_row(x: PerRow, none: float, B: int, dev, name: str):
+def _check(logits, history, lengths, prompt_lengths, per_row, bias_index,
+           bias, allowed):
+    """What the kernel's path refuses in csrc/lm_ops.cpp."""
+    if logits.dim() != 2 or not logits.dtype.is_floating_point:
+        raise ValueError(
+            f"logits must be (B, V) floating, got {tuple(logits.shape)}")
+    B, V = logits.shape
+    index = (torch.int32, torch.int64)
+    if history is not None and (
+            history.dim() != 2 or history.shape[0] != B
+            or history.dtype not in index):
+        raise ValueError(f"history must be (B={B}, L) int32 or int64")
+    for t, name in ((lengths, "lengths"), (prompt_lengths, "prompt_lengths")):
+        if t is not None and (t.shape != (B,) or t.dtype not in index):
+            raise ValueError(f"{name} must be (B={B},) int32 or int64")
+    for t in per_row:
+        if t is not None and (t.shape != (B,)
+                              or not t.dtype.is_floating_point):
+            raise ValueError(
+                f"penalties must be numbers or (B={B},) floating")
+    if bias is not None and (
+            bias_index.dim() != 2 or bias_index.shape[0] != B
+            or bias.shape != bias_index.shape
+            or bias_index.dtype not in index
+            or not bias.dtype.is_floating_point):
+        raise ValueError(f"bias_index must be (B={B}, K) int32 or int64 and "
+                         "bias floating of the same shape")
+    if allowed is not None and (allowed.dtype != torch.int32 or allowed.shape
+                                != (B, (V + 31) // 32)):
+        raise ValueError(f"allowed must be (B={B}, {(V + 31) // 32}) int32")
+    for t in (history, lengths, prompt_lengths, *per_row, bias_index, bias,
+              allowed):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"all tensors must be on {logits.device}")
+
+
+def _per_row(x: PerRow, none: float, name: str):
     """-> (tensor or None, number used without one)."""
     if x is None:
         return None, none
     if isinstance(x, torch.Tensor):
-        if x.shape != (B,) or not x.dtype.is_floating_point:
-            raise ValueError(f"{name} must be a number or (B={B},) floating")
-        if x.device != dev:
-            raise ValueError(f"all tensors must be on {dev}")
         return x, none
     x = float(x)
     if not math.isfinite(x):
@@ -92,7 +124,6 @@ def _per_row(x: PerRow, none: float, B: int, dev, name: str):
     return None, x
 
 
-@torch.no_grad()
 def adjust_logits(logits: torch.Tensor,
                   history: Optional[torch.Tensor] = None,
                   lengths: Optional[torch.Tensor] = None,
@@ -117,51 +148,29 @@ def adjust_logits(logits: torch.Tensor,
     allows nothing comes back as -inf throughout; a masked NaN is -inf.
     Not differentiable: this is the serving path.
     """
-    if logits.dim() != 2 or not logits.dtype.is_floating_point:
-        raise ValueError(
-            f"logits must be (B, V) floating, got {tuple(logits.shape)}")
-    B, V = logits.shape
-    dev = logits.device
-    index = (torch.int32, torch.int64)
     if history is None:
-        if any(x is not None for x in (lengths, prompt_lengths, repetition,
-                                       presence, frequency)):
+        if not (lengths is prompt_lengths is repetition is presence
+                is frequency is None):
             raise ValueError("penalties and lengths need a history")
-    elif (history.dim() != 2 or history.shape[0] != B
-          or history.dtype not in index):
-        raise ValueError(f"history must be (B={B}, L) int32 or int64")
-    for t, name in ((lengths, "lengths"), (prompt_lengths, "prompt_lengths")):
-        if t is not None and (t.shape != (B,) or t.dtype not in index):
-            raise ValueError(f"{name} must be (B={B},) int32 or int64")
     if (bias_index is None) != (bias is None):
         raise ValueError("bias_index and bias come together")
-    if bias is not None and (
-            bias_index.dim() != 2 or bias_index.shape[0] != B
-            or bias.shape != bias_index.shape
-            or bias_index.dtype not in index
-            or not bias.dtype.is_floating_point):
-        raise ValueError(f"bias_index must be (B={B}, K) int32 or int64 and "
-                         "bias floating of the same shape")
-    if allowed is not None and (allowed.dtype != torch.int32 or allowed.shape
-                                != (B, (V + 31) // 32)):
-        raise ValueError(f"allowed must be (B={B}, {(V + 31) // 32}) int32")
-    for t in (history, lengths, prompt_lengths, bias_index, bias, allowed):
-        if t is not None and t.device != dev:
-            raise ValueError(f"all tensors must be on {dev}")
-    rep, rep_all = _per_row(repetition, 1.0, B, dev, "repetition")
-    if rep is None and rep_all <= 0.0:
+    rep, rep_all = _per_row(repetition, 1.0, "repetition")
+    if rep_all <= 0.0:
         raise ValueError(f"repetition must be positive, got {rep_all}")
-    pres, pres_all = _per_row(presence, 0.0, B, dev, "presence")
-    freq, freq_all = _per_row(frequency, 0.0, B, dev, "frequency")
+    pres, pres_all = _per_row(presence, 0.0, "presence")
+    freq, freq_all = _per_row(frequency, 0.0, "frequency")
     if extension.use_hip_lm(logits):
         return extension.get_extension().adjust_logits(
             logits, history, lengths, prompt_lengths, rep, rep_all, pres,
             pres_all, freq, freq_all, bias_index, bias, allowed)
-    return _ref_adjust(logits, history, lengths, prompt_lengths,
-                       rep_all if rep is None else rep,
-                       pres_all if pres is None else pres,
-                       freq_all if freq is None else freq, bias_index, bias,
-                       allowed)
+    _check(logits, history, lengths, prompt_lengths, (rep, pres, freq),
+           bias_index, bias, allowed)
+    with torch.no_grad():
+        return _ref_adjust(logits, history, lengths, prompt_lengths,
+                           rep_all if rep is None else rep,
+                           pres_all if pres is None else pres,
+                           freq_all if freq is None else freq, bias_index,
+                           bias, allowed)
 
 
 @dataclasses.dataclass

@@ -457,3 +457,12 @@ def test_kernel_is_what_runs(monkeypatch):
     t, rows, scale = make(1, 4, 16, 16, 4, 2, dtype=torch.bfloat16, dev="cuda")
     monkeypatch.setattr(mod, "_ref_lowrank", None)
     lowrank_add(**t, rows=rows, scale=scale)
+
+
+@pytest.mark.gpu
+def test_kernel_refusals(monkeypatch):
+    """The same refusals, raised before anything is launched."""
+    plain = make
+    monkeypatch.setitem(globals(), "make", lambda *a: plain(
+        *a, dtype=torch.bfloat16, dev="cuda"))
+    test_refusals()

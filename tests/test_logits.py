@@ -258,3 +258,12 @@ def test_kernel_is_what_runs(monkeypatch):
     z, h, a = make(2, 50, 4, 2, dtype=torch.bfloat16, dev="cuda")
     monkeypatch.setattr(mod, "_ref_adjust", None)
     adjust_logits(z, h, **a)
+
+
+@pytest.mark.gpu
+def test_kernel_refusals(monkeypatch):
+    """The same refusals, raised before anything is launched."""
+    plain = make
+    monkeypatch.setitem(globals(), "make", lambda *a: plain(
+        *a, dtype=torch.bfloat16, dev="cuda"))
+    test_refusals()
