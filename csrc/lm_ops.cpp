@@ -1,7 +1,7 @@
 // Host side of the operators around the language-model head: argument checks, workspaces and
-// launches of distill.hip, adapters.hip and logits.hip.  What a decode step calls checks its
-// tensors here alone, with the errors that Python (ops/logits.py, ops/adapters.py) raises for the
-// reference: a check there costs as much as a launch.
+// launches of distill.hip, adapters.hip and logits.hip.  Tensors on the GPU are checked here alone,
+// with the errors that Python (ops/distill.py and its neighbours) raises for the reference: the
+// checks there take as long as a launch (logits of one row 9.7 us a call with them, 6.7 without).
 #include "lm_ops.h"
 
 #include <ATen/ATen.h>
@@ -113,14 +113,13 @@ struct Distill {
     const long* tp;
 
     Distill(const Tensor& logits, const Tensor& idx, const Tensor& t, const OptTensor& y) {
-        TORCH_CHECK(logits.is_cuda(), "logits must be on GPU");
-        TORCH_CHECK(logits.dim() == 2 && idx.dim() == 2 && t.dim() == 2 &&
-                        idx.size(0) == logits.size(0) && t.size(0) == logits.size(0) &&
-                        idx.size(1) == t.size(1),
-                    "distill: logits (N, V), teacher_index and teacher_logits (N, K)");
-        TORCH_CHECK(logits.size(1) >= 1 && logits.size(1) <= (1 << 30) &&
-                        t.size(1) <= (1 << 30),
-                    "distill: V and K must be below 2^30, V at least 1");
+        REQUIRE(logits.is_cuda() && logits.dim() == 2, "logits must be (N, V) on GPU, got ",
+                logits.sizes());
+        REQUIRE(idx.dim() == 2 && idx.size(0) == logits.size(0) && t.sizes() == idx.sizes(),
+                "teacher_index and teacher_logits must be (N=", logits.size(0), ", K), got ",
+                idx.sizes(), ", ", t.sizes());
+        REQUIRE(logits.size(1) >= 1 && logits.size(1) <= (1 << 30) && t.size(1) <= (1 << 30),
+                "V and K must be below 2^30, V at least 1");
         check_on(idx, logits, "teacher_index");
         check_on(t, logits, "teacher_logits");
         type = type_of(logits, "logits");
@@ -132,11 +131,11 @@ struct Distill {
         N = z.size(0);
         V = (int)z.size(1);
         K = (int)t.size(1);
-        TORCH_CHECK(N < (1l << 32) / (V > 8192 ? 1024 : 256), "distill: too many rows");
+        REQUIRE(N < (1l << 32) / (V > 8192 ? 1024 : 256), "too many rows");
         tp = nullptr;
         if (y.has_value()) {
-            TORCH_CHECK(y->dim() == 1 && y->size(0) == N && y->scalar_type() == at::kLong,
-                        "distill: targets must be (N,) int64");
+            REQUIRE(y->dim() == 1 && y->size(0) == N && y->scalar_type() == at::kLong,
+                    "targets must be (N=", N, ",) int64");
             check_on(*y, logits, "targets");
             target = y->contiguous();
             tp = (const long*)target.data_ptr();
@@ -214,6 +213,8 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
 Tensor distill_loss(Tensor logits, Tensor index, Tensor teacher, OptTensor targets, double alpha,
                     double tau, double weight) {
     const bool need = at::GradMode::is_enabled() && logits.requires_grad();
+    if (teacher.scalar_type() == at::kDouble) teacher = teacher.to(at::kFloat);
+    if (teacher.requires_grad()) teacher = teacher.detach();
     return DistillLoss::apply(logits, index, teacher, targets, alpha, tau, weight, need);
 }
 

@@ -60,6 +60,30 @@ def _ref_distill(logits, index, teacher, targets, alpha, tau):
     return rows.sum() / (soft | label).sum().clamp_min(1)
 
 
+def _check(logits, teacher_index, teacher_logits, targets):
+    """What the kernels' path refuses in csrc/lm_ops.cpp."""
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be (N, V), got {tuple(logits.shape)}")
+    N, V = logits.shape
+    if V < 1 or not logits.dtype.is_floating_point:
+        raise ValueError("logits must be floating and have a vocabulary")
+    if (teacher_index.dim() != 2 or teacher_index.shape[0] != N
+            or teacher_index.shape != teacher_logits.shape):
+        raise ValueError(
+            f"teacher_index and teacher_logits must be (N={N}, K), got "
+            f"{tuple(teacher_index.shape)}, {tuple(teacher_logits.shape)}")
+    if teacher_index.dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_index must be int32 or int64")
+    if not teacher_logits.dtype.is_floating_point:
+        raise ValueError("teacher_logits must be floating")
+    if targets is not None and (targets.dtype != torch.long
+                                or targets.shape != (N,)):
+        raise ValueError(f"targets must be (N={N},) int64")
+    for t in (teacher_index, teacher_logits, targets):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"all tensors must be on {logits.device}")
+
+
 def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
                  teacher_logits: torch.Tensor,
                  targets: Optional[torch.Tensor] = None, *,
@@ -83,20 +107,6 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
     A row of padding (no entry and no label) adds nothing, is not counted
     and gets a zero gradient.
     """
-    if logits.dim() != 2:
-        raise ValueError(f"logits must be (N, V), got {tuple(logits.shape)}")
-    N, V = logits.shape
-    if V < 1 or not logits.dtype.is_floating_point:
-        raise ValueError("logits must be floating and have a vocabulary")
-    if (teacher_index.dim() != 2 or teacher_index.shape[0] != N
-            or teacher_index.shape != teacher_logits.shape):
-        raise ValueError(
-            f"teacher_index and teacher_logits must be (N={N}, K), got "
-            f"{tuple(teacher_index.shape)}, {tuple(teacher_logits.shape)}")
-    if teacher_index.dtype not in (torch.int32, torch.int64):
-        raise ValueError("teacher_index must be int32 or int64")
-    if not teacher_logits.dtype.is_floating_point:
-        raise ValueError("teacher_logits must be floating")
     if not 0.0 <= alpha <= 1.0:
         raise ValueError(f"alpha must be in [0, 1], got {alpha}")
     if not 1e-6 <= temperature <= 1e6:      # its square and inverse in fp32
@@ -106,18 +116,11 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor,
         raise ValueError(f"weight must be finite, got {weight}")
     if targets is None and alpha != 1.0:
         raise ValueError("alpha < 1 needs targets")
-    if targets is not None and (targets.dtype != torch.long
-                                or targets.shape != (N,)):
-        raise ValueError(f"targets must be (N={N},) int64")
-    for t in (teacher_index, teacher_logits, targets):
-        if t is not None and t.device != logits.device:
-            raise ValueError(f"all tensors must be on {logits.device}")
     if extension.use_hip_lm(logits):
-        if teacher_logits.dtype == torch.float64:
-            teacher_logits = teacher_logits.float()
         return extension.get_extension().distill_loss(
-            logits, teacher_index, teacher_logits.detach(), targets, alpha,
+            logits, teacher_index, teacher_logits, targets, alpha,
             temperature, weight)
+    _check(logits, teacher_index, teacher_logits, targets)
     loss = _ref_distill(logits, teacher_index, teacher_logits, targets,
                         float(alpha), float(temperature))
     return loss * weight

@@ -419,3 +419,24 @@ def test_kernel_is_what_runs(monkeypatch):
     z, i, t, y = make(4, 50, 3, dtype=torch.bfloat16, dev="cuda")
     monkeypatch.setattr(distill, "_ref_distill", None)
     distill_loss(z, i, t, y, alpha=0.5)
+
+
+@pytest.mark.gpu
+def test_kernel_refusals(monkeypatch):
+    """The same refusals, raised before anything is launched."""
+    plain = make
+    monkeypatch.setitem(globals(), "make", lambda *a: plain(
+        *a, dtype=torch.bfloat16, dev="cuda"))
+    test_refusals()
+
+
+@pytest.mark.gpu
+def test_kernel_teacher_gets_no_gradient():
+    z, i, t, y = make(6, 300, 5, dtype=torch.bfloat16, dev="cuda")
+    want = distill_loss(z, i, t.double(), y, alpha=0.5)
+    t = t.double().requires_grad_()
+    loss = distill_loss(z, i, t, y, alpha=0.5)
+    assert torch.equal(loss, want) and not loss.requires_grad
+    z.requires_grad_()
+    distill_loss(z, i, t, y, alpha=0.5).backward()
+    assert t.grad is None and z.grad is not None
