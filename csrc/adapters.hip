@@ -126,6 +126,18 @@ struct Tile {               // up to 1 << shift rows of one segment, from its ro
     int first;              // number of the segment's first tile
 };
 
+// The sum over a wave's lanes up to one's own: by shifts in rows of 16 lanes, then from the last
+// lane of a row to the next ones (every lane of the wave has to be there).
+DEVINL int running_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);     // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);     // row_shr:2
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);     // row_shr:4
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);     // row_shr:8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // row_bcast:15
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // row_bcast:31
+    return x;
+}
+
 // Which rows tile number `tile` holds.  A wave sums up the segments' tiles, 64 at a time.
 DEVINL Tile find_tile(const Rows& r, int tile, int shift) {
     const int lane = threadIdx.x & 63;
@@ -135,24 +147,19 @@ DEVINL Tile find_tile(const Rows& r, int tile, int shift) {
         const int s = s0 + lane;
         const int4 g = s < r.S ? r.segs[s] : make_int4(-1, 0, 0, 0);
         const int t = (int)((r.T * g.z + (1l << shift) - 1) >> shift);
-        int sum = t;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(sum, off, 64);
-            if (lane >= off) sum += o;
-        }
+        const int sum = running_sum(t);
         const unsigned long long hit = __ballot(base + sum > tile);
         if (hit) {
             const int at = __ffsll(hit) - 1;
-            f.adapter = __shfl(g.x, at, 64);
-            f.start = __shfl(g.y, at, 64);
-            f.count = __shfl(g.z, at, 64);
-            f.first = base + __shfl(sum - t, at, 64);
+            f.adapter = __builtin_amdgcn_readlane(g.x, at);
+            f.start = __builtin_amdgcn_readlane(g.y, at);
+            f.count = __builtin_amdgcn_readlane(g.z, at);
+            f.first = base + __builtin_amdgcn_readlane(sum - t, at);
             f.n = r.T * f.count;
             f.j0 = (long)(tile - f.first) << shift;
             return f;
         }
-        base += __shfl(sum, 63, 64);
+        base += __builtin_amdgcn_readlane(sum, 63);
     }
     return f;
 }
@@ -815,20 +822,15 @@ __global__ __launch_bounds__(256) void k_outer_sum(const float* __restrict__ par
         const int s = s0 + lane;
         const int4 g = s < rows.S ? rows.segs[s] : make_int4(-1, 0, 0, 0);
         const int t = (int)((rows.T * g.z + (1l << shift) - 1) >> shift);
-        int sum = t;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(sum, off, 64);
-            if (lane >= off) sum += o;
-        }
+        const int sum = running_sum(t);
         const unsigned long long hit = __ballot(g.x == l && t > 0);
         if (hit) {
             const int k = __ffsll(hit) - 1;
-            first = base + __shfl(sum - t, k, 64);
-            tiles = __shfl(t, k, 64);
+            first = base + __builtin_amdgcn_readlane(sum - t, k);
+            tiles = __builtin_amdgcn_readlane(t, k);
             break;
         }
-        base += __shfl(sum, 63, 64);
+        base += __builtin_amdgcn_readlane(sum, 63);
     }
     constexpr int TH = 256 / GR;
     __shared__ f32x4 sums[GR > 1 ? 256 : 1];
