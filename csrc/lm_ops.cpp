@@ -300,6 +300,44 @@ Tensor adjust(Tensor logits, OptTensor history, OptTensor lengths, OptTensor pro
 }
 
 // ------------------------------------------------------------------ low-rank adapters
+// Elements of the storage from the tensor's first on: the kernels read eight at a time, past a
+// row's end if need be but never past this.  Where there are not even eight, in a copy.
+long room_of(const Tensor& t) {
+    return (long)(t.storage().nbytes() / t.element_size()) - t.storage_offset();
+}
+Tensor readable(const Tensor& t) {
+    if (!t.defined() || room_of(t) >= 8) return t;
+    Tensor copy = at::zeros({t.numel() + 8}, t.options()).narrow(0, 0, t.numel()).view(t.sizes());
+    return copy.copy_(t);
+}
+
+// A tensor of any leading shape as rows; a contiguous one without asking for a view.
+struct Matrix {
+    Tensor t;
+    long cols = 0, stride = 0, room = 8;
+
+    Matrix() = default;         // none
+    Matrix(const Tensor& any, long rows, long n) : t(any), cols(n), stride(n) {
+        if (!any.is_contiguous()) {
+            t = rows_of(any.reshape({rows, n}));
+            stride = row_stride(t);
+        }
+        if (room_of(t) < 8) {
+            t = readable(t.reshape({rows, n}));
+            stride = n;
+        }
+        room = room_of(t);
+    }
+    // A contiguous result: written, so as it is, whatever lies behind it.
+    static Matrix result(const Tensor& out, long n) {
+        Matrix m;
+        m.t = out;
+        m.cols = m.stride = n;
+        return m;
+    }
+    void* data() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+
 // Rows grouped by adapter (ops/adapters.py: AdapterRows), and what every launch takes of them.
 struct Grouped {
     Tensor order, segs, adapter, scale;
@@ -370,30 +408,19 @@ struct Grouped {
         REQUIRE(N < (1l << 31) && N / 64 * ((std::max(K, M) + 127) / 128) < (1l << 31),
                 "too many rows");
     }
-    // Elements of the storage from the tensor's first on: the kernels read eight at a time, past a
-    // row's end if need be but never past this.  Where there are not even eight, in a copy.
-    static long room(const Tensor& t) {
-        return (long)(t.storage().nbytes() / t.element_size()) - t.storage_offset();
-    }
-    static Tensor readable(const Tensor& t) {
-        if (!t.defined() || room(t) >= 8) return t;
-        Tensor copy =
-            at::zeros({t.numel() + 8}, t.options()).narrow(0, 0, t.numel()).view(t.sizes());
-        return copy.copy_(t);
-    }
     const int* ip(const Tensor& t) const { return (const int*)t.data_ptr(); }
 
     // v (N, RP) = s x W, W (L, K, R) or, contraction contiguous, (L, R, K)
-    Tensor shrink(const Tensor& x_, const Tensor& w_, bool kcont, hipStream_t st) const {
-        const Tensor x = readable(x_), w = readable(w_);
-        const int k = (int)x.size(1), splits = lowrank_splits(counts.data(), S, T, k, 4);
-        auto v = at::empty({N, (long)lowrank_rp(R)}, x.options());
+    Tensor shrink(const Matrix& x, const Tensor& w_, bool kcont, hipStream_t st) const {
+        const Tensor w = readable(w_);
+        const int k = (int)x.cols, splits = lowrank_splits(counts.data(), S, T, k, 4);
+        auto v = at::empty({N, (long)lowrank_rp(R)}, w.options());
         Tensor part;
         if (splits > 1)
-            part = at::empty({(long)splits * N * lowrank_rp(R)}, x.options().dtype(at::kFloat));
-        launch_shrink(type, kcont, x.data_ptr(), row_stride(x), room(x), w.data_ptr(), room(w),
-                      k, R, ip(order),
-                      ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
+            part = at::empty({(long)splits * N * lowrank_rp(R)}, w.options().dtype(at::kFloat));
+        launch_shrink(type, kcont, x.data(), x.stride, x.room, w.data_ptr(), room_of(w), k, R,
+                      ip(order), ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale),
+                      scale_all,
                       v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, splits, st);
         if (splits > 1) sum(v, (const float*)part.data_ptr(), splits, st);
         check_launch("lowrank shrink");
@@ -404,38 +431,35 @@ struct Grouped {
                           scale_all, v.data_ptr(), part, splits, st);
     }
     // out = base + s x A B of a few rows an adapter, in two launches
-    void few(const Tensor& base, Tensor& out, const Tensor& x_, const Tensor& a_, const Tensor& b,
-             hipStream_t st) const {
-        const Tensor x = readable(x_), a = readable(a_);
+    void few(const Matrix& base, const Matrix& out, const Matrix& x, const Tensor& a_,
+             const Tensor& b, hipStream_t st) const {
+        const Tensor a = readable(a_);
         const int splits = lowrank_splits(counts.data(), S, T, K, 0);
-        auto part = at::empty({(long)splits * N * lowrank_rp(R)}, x.options().dtype(at::kFloat));
-        launch_shrink(type, 0, x.data_ptr(), row_stride(x), room(x), a.data_ptr(), room(a), K,
-                      R, ip(order),
-                      ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
-                      nullptr, (float*)part.data_ptr(), splits, st);
-        launch_expand_few(type, base.data_ptr(), row_stride(base), out.data_ptr(),
-                          row_stride(out), (const float*)part.data_ptr(), b.data_ptr(), M, R,
-                          ip(order), ip(segs), ip(adapter), counts.data(), S, Bn, T,
-                          float_ptr(scale), scale_all, splits, st);
+        auto part = at::empty({(long)splits * N * lowrank_rp(R)}, a.options().dtype(at::kFloat));
+        launch_shrink(type, 0, x.data(), x.stride, x.room, a.data_ptr(), room_of(a), K, R,
+                      ip(order), ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale),
+                      scale_all, nullptr, (float*)part.data_ptr(), splits, st);
+        launch_expand_few(type, base.data(), base.stride, out.data(), out.stride,
+                          (const float*)part.data_ptr(), b.data_ptr(), M, R, ip(order), ip(segs),
+                          ip(adapter), counts.data(), S, Bn, T, float_ptr(scale), scale_all,
+                          splits, st);
         check_launch("lowrank few");
     }
     // out = base + v W, W (L, R, M) or, rank contiguous, (L, M, R)
-    void expand(const Tensor& base_, Tensor& out, const Tensor& v, const Tensor& w_, bool rcont,
-                hipStream_t st) const {
-        const Tensor base = readable(base_), w = readable(w_);
-        launch_expand(type, rcont, base.defined() ? base.data_ptr() : nullptr,
-                      base.defined() ? row_stride(base) : 0, base.defined() ? room(base) : 8,
-                      out.data_ptr(), row_stride(out), v.data_ptr(), w.data_ptr(), room(w),
-                      (int)out.size(1), R, ip(order), ip(segs),
-                      ip(adapter), counts.data(), S, Bn, T, st);
+    void expand(const Matrix& base, const Matrix& out, const Tensor& v, const Tensor& w_,
+                bool rcont, hipStream_t st) const {
+        const Tensor w = readable(w_);
+        launch_expand(type, rcont, base.data(), base.stride, base.room, out.data(), out.stride,
+                      v.data_ptr(), w.data_ptr(), room_of(w), (int)out.cols, R, ip(order),
+                      ip(segs), ip(adapter), counts.data(), S, Bn, T, st);
         check_launch("lowrank expand");
     }
     // sum over an adapter's rows of p^T q: (L, R, NP) or, rank contiguous, (L, NP, R).  With w
     // (L, R, NP) also `u` (N, RP) = s p w^T, from the same reading of p.
-    Tensor outer(const Tensor& p_, const Tensor& q, bool rcont, hipStream_t st,
+    Tensor outer(const Matrix& p, const Tensor& q, bool rcont, hipStream_t st,
                  const Tensor& w_ = Tensor(), Tensor* u = nullptr) const {
-        const Tensor p = readable(p_), w = readable(w_);
-        const int np = (int)p.size(1), rp = lowrank_rp(R);
+        const Tensor w = readable(w_);
+        const int np = (int)p.cols, rp = lowrank_rp(R);
         const int columns = lowrank_outer_columns(counts.data(), S, T, np, R, u != nullptr);
         const int strips = (np + columns - 1) / columns;
         const int shift = lowrank_outer_shift(counts.data(), S, T, strips, columns, R);
@@ -444,19 +468,19 @@ struct Grouped {
         // one workspace: the gradient's parts, u's shares and a row for what belongs to no row
         const long parts = whole ? 0 : tiles * rp * strips * columns;
         auto work = at::empty({parts + (u ? (strips * N + 1) * rp : 0)},
-                              p.options().dtype(at::kFloat));
+                              q.options().dtype(at::kFloat));
         float* part = (float*)work.data_ptr();
         const std::vector<int64_t> size = rcont ? std::vector<int64_t>{L, np, R}
                                                 : std::vector<int64_t>{L, R, np};
         // an adapter without rows has no tile to write its zeros
-        auto out = whole && groups < L ? at::zeros(size, p.options())
-                                       : at::empty(size, p.options());
-        launch_outer(type, rcont, p.data_ptr(), row_stride(p), room(p), np, q.data_ptr(),
-                     part, u ? w.data_ptr() : nullptr, u ? room(w) : 8,
+        auto out = whole && groups < L ? at::zeros(size, q.options())
+                                       : at::empty(size, q.options());
+        launch_outer(type, rcont, p.data(), p.stride, p.room, np, q.data_ptr(),
+                     part, u ? w.data_ptr() : nullptr, u ? room_of(w) : 8,
                      u ? part + parts : nullptr, ip(order), ip(segs), ip(adapter),
                      counts.data(), S, Bn, T, shift, columns, whole, out.data_ptr(), R, L, st);
         if (u) {
-            *u = at::empty({N, (long)rp}, p.options());
+            *u = at::empty({N, (long)rp}, q.options());
             sum(*u, part + parts, strips, st);
         }
         check_launch("lowrank outer");
@@ -470,9 +494,8 @@ Tensor lowrank_forward(const Grouped& g, const Tensor& y, const Tensor& x, const
                        const Tensor& b, bool inplace, Tensor* v) {
     const hipStream_t st = stream_of(x);
     Tensor out = inplace ? y : at::empty(y.sizes(), y.options());
-    Tensor rows = out.view({g.N, (long)g.M});
-    const Tensor base = inplace ? rows : rows_of(y.reshape({g.N, (long)g.M}));
-    const Tensor xr = rows_of(x.reshape({g.N, (long)g.K}));
+    const Matrix base(y, g.N, g.M), xr(x, g.N, g.K);
+    const Matrix rows = Matrix::result(out, g.M);
     if (!v && lowrank_few(g.counts.data(), g.S, g.T)) {
         g.few(base, rows, xr, a, b, st);
         return out;
@@ -518,7 +541,7 @@ struct LowRankAdd : public torch::autograd::Function<LowRankAdd> {
         const bool need_u = need[1] || need[2];
         if (need[0]) out[0] = dy;
         if (!need_u && !need[3]) return out;
-        const Tensor dr = rows_of(dy.reshape({g.N, (long)g.M}));
+        const Matrix dr(dy, g.N, g.M);
         Tensor u;
         if (need[3] && need_u && lowrank_one_reading(g.R)) {
             out[3] = g.outer(dr, v, false, st, b, &u);
@@ -528,10 +551,9 @@ struct LowRankAdd : public torch::autograd::Function<LowRankAdd> {
         }
         if (need[1]) {
             out[1] = at::empty(x.sizes(), x.options());
-            Tensor rows = out[1].view({g.N, (long)g.K});
-            g.expand(Tensor(), rows, u, a, true, st);
+            g.expand(Matrix(), Matrix::result(out[1], g.K), u, a, true, st);
         }
-        if (need[2]) out[2] = g.outer(rows_of(x.reshape({g.N, (long)g.K})), u, true, st);
+        if (need[2]) out[2] = g.outer(Matrix(x, g.N, g.K), u, true, st);
         return out;
     }
 };
