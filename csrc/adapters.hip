@@ -9,8 +9,10 @@
 // R is 4 to 128 where K and M are thousands, so every product streams one wide matrix past a
 // narrow one and is bound by that stream: `shrink` reads rows (x, dy), `expand` reads and writes
 // them (y, dx), `outer` reads them again for the weights' gradients.  MFMA feeds on 32 of the
-// contraction at a time in the stream's own layout; accumulation, split sums and partial
-// gradients are fp32, v and u are rounded once to the type (they are MFMA operands).
+// contraction at a time in the stream's own layout; accumulation, split sums, partial gradients,
+// v and u are fp32.  v and u meet the matrix instructions in parts of the type that add up to them
+// (`split`): of 16-bit v the products would carry 2^-8 of error, and an fp16 v beyond 65504 is an
+// infinity where the result need not be.  Each result is rounded once.
 //
 // Rows come grouped by adapter.  Sequences are time-major, row = t * Bn + column, and an adapter
 // belongs to a column, so only the Bn columns are grouped: segment s lists its columns in
@@ -66,6 +68,53 @@ template <typename F> DEVINL F trim(F v, long e, long limit, int left) {
     else if (keep < 128) u = u2{u[0], u[1] & ((1ull << (keep - 64)) - 1)};
     return __builtin_bit_cast(F, u);
 }
+
+// fp32 numbers as a sum of a 16-bit type's, operands of as many matrix instructions.  All parts
+// have the number's sign, and none is zero unless it is: an infinity in the other operand then
+// gives that infinity, where plus and minus or zero times infinity would give NaN.
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+template <typename T> struct Split;
+// bf16 has fp32's range and a third of its digits: three parts, all but the last one's rest is
+// cut off, and the last has no more digits than fit.  Where nothing is left, 2^-30 of the first.
+template <> struct Split<bf16_t> {
+    static constexpr int N = 3;
+    bf16x8 p[N];
+    DEVINL Split(f32x8 v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            auto cut = [](float x) { return __int_as_float(__float_as_int(x) & 0xffff0000); };
+            const float a = cut(v[j]), least = a * 0x1p-30f;
+            const float r = v[j] - a, b = fabsf(r) > 0.f ? cut(r) : least;  // infinity: r is NaN
+            const float q = r - b, c = fabsf(q) > 0.f ? q : least;
+            p[0][j] = __builtin_bit_cast(bf16_t, (short)(__float_as_int(a) >> 16));
+            p[1][j] = __builtin_bit_cast(bf16_t, (short)(__float_as_int(b) >> 16));
+            p[2][j] = __builtin_bit_cast(bf16_t, (short)(__float_as_int(c) >> 16));
+        }
+    }
+};
+// fp16 has not the range: the numbers come scaled so that the largest of those that a sum holds is
+// near 2^15 (`shift_of`).  Two parts: 22 digits, and an error of 2^-40 of the largest at most.
+template <> struct Split<f16_t> {
+    static constexpr int N = 2;
+    f16x8 p[N];
+    DEVINL Split(f32x8 v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const f16_t least = (f16_t)(v[j] > 0.f ? 0x1p-24f : v[j] < 0.f ? -0x1p-24f : 0.f);
+            f16_t a = (f16_t)__builtin_amdgcn_cvt_pkrtz(v[j], 0.f)[0];
+            if (a == (f16_t)0.f) a = least;
+            const float r = v[j] - (float)a;
+            const f16_t b = (f16_t)r;
+            p[0][j] = a;
+            p[1][j] = fabsf(r) > 0.f && b != (f16_t)0.f && (r > 0.f) == (v[j] > 0.f) ? b : least;
+        }
+    }
+};
+// The power of two that brings numbers of which m is the largest to [2^14, 2^15), and its inverse
+// (m finite; both are normal numbers: of 0 or the least the shift is -120).
+DEVINL int shift_of(float m) { return max((__float_as_int(m) >> 23) - 127 - 14, -120); }
+DEVINL float two_to(int e) { return __int_as_float((127 + e) << 23); }
+DEVINL float finite_size(float x) { return fabsf(x) < __builtin_huge_valf() ? fabsf(x) : 0.f; }
 
 // The bits of a vector's first `left` elements, and the vector without the others.
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -183,7 +232,7 @@ constexpr int S_KC = 256;   // contraction a step
 template <typename T, int RT, bool KCONT>
 __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs, long xlimit,
                                                 const T* __restrict__ W, long wlimit, int K, int R,
-                                                Rows rows, Scale scale, T* __restrict__ V, int RP,
+                                                Rows rows, Scale scale, float* __restrict__ V,
                                                 float* __restrict__ part, long N, int splits,
                                                 int kper) {
     typedef typename Frag<T>::type F;
@@ -272,31 +321,29 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
 #pragma unroll
             for (int t = 0; t < RT; ++t) p[t * 16] = acc[t][i];
         } else {
-            T* v = V + r * RP + (lane & 15);
+            float* v = V + r * (RT * 16) + (lane & 15);
 #pragma unroll
             for (int t = 0; t < RT; ++t)        // zeros behind R, where an infinity left NaN
-                v[t * 16] = (T)(t * 16 + (lane & 15) < R ? acc[t][i] * sc : 0.f);
-            if (RT == 1) v[16] = (T)0.f;        // expand contracts 32 at a time
+                v[t * 16] = t * 16 + (lane & 15) < R ? acc[t][i] * sc : 0.f;
         }
     }
 }
 
-// The shares summed in a fixed order, scaled and rounded; four of a row's R a thread.  GR groups of
-// threads take every GR-th share where there are many (98 of 8192 rows, rank 32).
-template <typename T, int GR>
+// The shares summed in a fixed order and scaled; four of a row's R a thread.  GR groups of threads
+// take every GR-th share where there are many (98 of 8192 rows, rank 32).
+template <int GR>
 __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ part, long N, int R,
                                                     int R16, int splits, Rows rows, Scale scale,
-                                                    T* __restrict__ V, int RP) {
-    typedef T out4 __attribute__((ext_vector_type(4)));
+                                                    float* __restrict__ V) {
     constexpr int TH = 256 / GR;
     __shared__ f32x4 sums[GR > 1 ? 256 : 1];
     const int group = threadIdx.x / TH;
     const long i = (long)blockIdx.x * TH + threadIdx.x % TH;
-    const long row = i / (RP / 4);
-    const int r = (int)(i % (RP / 4)) * 4;
+    const long row = i / (R16 / 4);
+    const int r = (int)(i % (R16 / 4)) * 4;
     const int l = row < N ? rows.adapter[(unsigned)row % (unsigned)rows.Bn] : -1;
     f32x4 s = f32x4{0, 0, 0, 0};
-    if (l >= 0 && r < R16) {
+    if (l >= 0) {
         const float* p = part + row * R16 + r;
 #pragma unroll 8
         for (int k = group; k < splits; k += GR) s += *(const f32x4*)(p + (long)k * N * R16);
@@ -310,10 +357,10 @@ __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ pa
     }
     if (l < 0) return;
     const float sc = scale(l);
-    out4 v;
+    f32x4 v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (T)(r + j < R ? s[j] * sc : 0.f);
-    *(out4*)(V + row * RP + r) = v;
+    for (int j = 0; j < 4; ++j) v[j] = r + j < R ? s[j] * sc : 0.f;
+    *(f32x4*)(V + row * R16 + r) = v;
 }
 
 // ---------------------------------------------------------------------------
@@ -326,7 +373,7 @@ __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ pa
 // ---------------------------------------------------------------------------
 template <typename T, int RK, bool RCONT>
 __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long blimit, T* out,
-                                                long os, const T* __restrict__ V, int RP,
+                                                long os, const float* __restrict__ V, int R16,
                                                 const T* __restrict__ W, long wlimit, int M, int R,
                                                 Rows rows, int strips, int shift) {
     typedef typename Frag<T>::type F;
@@ -377,7 +424,8 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
     // a lane's share of base and out: eight columns of every eighth row
     const int m = strip + (tid & 31) * 8;
     const bool whole = m + 8 <= M;
-    F y[4], v[2][RK];
+    F y[4];
+    f32x8 v[2][RK];
     auto load_base = [&](long j0) {
         if (!base) return;
 #pragma unroll
@@ -392,7 +440,11 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
             const long j = j0 + h * 16 + (lane & 15);
             const long row = at[(j < jend ? j : jend - 1) - f.j0];
 #pragma unroll
-            for (int k = 0; k < RK; ++k) v[h][k] = *(const F*)(V + row * RP + k * 32 + g * 8);
+            for (int k = 0; k < RK; ++k) {          // a contraction of 32 is zeros behind 16
+                const bool there = RK > 1 || g * 8 < R16;
+                v[h][k] = *(const f32x8*)(V + row * R16 + (there ? k * 32 + g * 8 : 0));
+                if (!there) v[h][k] = 0.f;
+            }
         }
     };
     load_base(f.j0);
@@ -406,13 +458,31 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
     }
     auto multiply = [&](f32x4 (&acc)[2][4]) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+            int e = 0;
+            if (__is_same(T, f16_t)) {          // a row's lanes are 16 apart
+                float m = 0.f;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                acc[h][t] = f32x4{0, 0, 0, 0};
+                for (int k = 0; k < RK; ++k)
 #pragma unroll
-                for (int k = 0; k < RK; ++k) acc[h][t] = mfma(w[k][t], v[h][k], acc[h][t]);
+                    for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_size(v[h][k][j]));
+                m = fmaxf(m, __shfl_xor(m, 16, 64));
+                e = shift_of(fmaxf(m, __shfl_xor(m, 32, 64)));
             }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[h][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < RK; ++k) {
+                const Split<T> s(__is_same(T, f16_t) ? v[h][k] * two_to(-e) : v[h][k]);
+#pragma unroll
+                for (int i = 0; i < Split<T>::N; ++i)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[h][t] = mfma(w[k][t], s.p[i], acc[h][t]);
+            }
+            if (__is_same(T, f16_t))
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[h][t] *= two_to(e);
+        }
     };
     auto to_lds = [&](const f32x4 (&acc)[2][4]) {
 #pragma unroll
@@ -491,21 +561,20 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
 // The same for a decode step, where an adapter has a row or a few and its weights are most of
 // what is read: a wave takes 512 columns, eight a lane, and up to four rows, and multiplies W as
 // it comes, whole lines of one r, without staging.  The shares of V are summed here, which saves
-// the launch that does it elsewhere; V is rounded to the type all the same.
+// the launch that does it elsewhere.
 // ---------------------------------------------------------------------------
 constexpr int FEW = 2;      // log2 rows a wave
 
-// v = s x A of the rows `at`, rounded to the type, from the shares of x A.
-template <typename T>
+// v = s x A of the rows `at`, from the shares of x A.
 DEVINL void sum_shares(const float* __restrict__ part, const int* at, int n, long N, int R16,
-                       int splits, float scale, float* v, T) {
+                       int splits, float scale, float* v) {
     for (int u = threadIdx.x; u < n * R16; u += 64) {
         const int i = u / R16, r = u - i * R16;
         const float* p = part + (long)at[i] * R16 + r;
         float s = 0.f;
 #pragma unroll 8
         for (int k = 0; k < splits; ++k) s += p[(long)k * N * R16];
-        v[i * 128 + r] = (float)(T)(s * scale);
+        v[i * 128 + r] = s * scale;
     }
     __syncthreads();
 }
@@ -552,7 +621,7 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
         }
         float acc[NR][8] = {};
         if (mine) {
-            sum_shares(part, at, n, N, R16, splits, scale(f.adapter), v, T());
+            sum_shares(part, at, n, N, R16, splits, scale(f.adapter), v);
             for (int r0 = 0; r0 < R; r0 += U) {
                 if (r0) load(r0);
 #pragma unroll
@@ -582,7 +651,7 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
     }
     if (lane < NR) at[lane] = (int)t * rows.Bn + column;
     __syncthreads();
-    if (mine) sum_shares(part, at, n, N, R16, splits, scale(f.adapter), v, T());
+    if (mine) sum_shares(part, at, n, N, R16, splits, scale(f.adapter), v);
     for (int i = 0; i < n; ++i)
         for (int q = lane; q < M; q += 64) {            // fewer than eight columns
             float s = (float)base[at[i] * bs + q];
@@ -597,6 +666,11 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
 // CT columns and walks the tile's rows 64 at a time: they pass through LDS as they are, and both
 // operands are read from there with their columns' rows side by side.
 //
+// Q's numbers pass as their bf16 parts, split once on the way into LDS.  fp16's have to be scaled
+// first, by a power of two for each of Q's columns: such a column is the 16 lanes' own number in
+// B and in D, so every wave reads Q from LDS as it is, takes the largest of a column's 32 rows,
+// and, when that is larger than any before, brings the column's sums to the new scale.
+//
 // NS > 0: the rows meet W on the way too, partv[share][row][r] = sum over the workgroup's columns
 // of P[row][p] W_l[r][p] -- the backward pass's u, in shares of NS times as many columns.  dy is
 // then read once for both; a share costs 8 R bytes a row (written, read again), a second reading
@@ -604,7 +678,7 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
 // ---------------------------------------------------------------------------
 template <typename T, int RT, int CT, int NS>
 __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps, long plimit,
-                                               int NP, const T* __restrict__ Q, int RP,
+                                               int NP, const float* __restrict__ Q,
                                                float* __restrict__ part,
                                                const T* __restrict__ W, long wlimit, int R,
                                                float* __restrict__ partv, long N,
@@ -613,10 +687,12 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
     typedef typename Frag<T>::type F;
     constexpr bool DV = NS > 0;
     constexpr int C = DV ? NS : 1;                  // strips of PC columns
+    constexpr bool SCALED = __is_same(T, f16_t);
     constexpr int PC = 64 * CT, S = PC / 32, LP = PC + 16, LQ = RT * 16 + (RT >= 4 ? 16 : 0);
-    constexpr int LW = C * PC + 8;
+    constexpr int LW = C * PC + 8, LF = RT * 16 + 2, NQ = Split<T>::N;
     __shared__ __attribute__((aligned(16))) T pt[64 * LP];
-    __shared__ __attribute__((aligned(16))) T qt[64 * LQ];
+    __shared__ __attribute__((aligned(16))) T qt[SCALED ? 1 : NQ][SCALED ? 8 : 64 * LQ];
+    __shared__ __attribute__((aligned(16))) float qf[SCALED ? 64 * LF : 4];
     __shared__ __attribute__((aligned(16))) T wt[DV ? RT * 16 * LW : 8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
     const int block = by_xcd(), tile = block / shares, share = block % shares;
@@ -642,7 +718,11 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
     constexpr int QV = (64 * RT * 2 + 255) / 256;       // vectors of Q a thread
     constexpr int PV = 64 * PC / 8 / 256, PW = PC / 8;  // of P; a row's
     constexpr int D = C > 1 ? 2 : 1;                    // strips of P ahead
-    F x[D][PV], q[QV];
+    F x[D][PV];
+    f32x8 q[QV];
+    int shift_q[RT];            // a column's sums are what they stand for over two to this
+#pragma unroll
+    for (int t = 0; t < RT; ++t) shift_q[t] = -120;
     // Loads and stores end in the order they went out, and a wait for a load has to know how many
     // are younger: so nothing in the loop goes out on a condition (rows behind the last are the
     // last again), or the wait would drain all of them (8192 rows of 50000 in one group, a
@@ -676,7 +756,7 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
         for (int i = 0; i < QV; ++i) {
             const int u = i * 256 + tid, n = u / (RT * 2);
             if (n >= 64) continue;
-            q[i] = *(const F*)(Q + (long)at[slot][n] * RP + u % (RT * 2) * 8);
+            q[i] = *(const f32x8*)(Q + (long)at[slot][n] * (RT * 16) + u % (RT * 2) * 8);
         }
     };
     // u of a step goes out in the next one, before its loads; rows behind the last, and the first
@@ -727,9 +807,18 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
                 for (int i = 0; i < QV; ++i) {
                     const int u = i * 256 + tid, n = u / (RT * 2);
                     if (n >= 64) continue;
-                    F v = q[i];
-                    if (tail) v = trim(v, 0, 8, j0 + n < jend ? 8 : 0);
-                    *(F*)(qt + n * LQ + u % (RT * 2) * 8) = v;
+                    const f32x8 v = j0 + n < jend ? q[i] : (f32x8)0.f;
+                    if (SCALED) {
+                        typedef float f32x2 __attribute__((ext_vector_type(2)));
+                        f32x2* to = (f32x2*)(qf + n * LF + u % (RT * 2) * 8);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) to[j] = f32x2{v[2 * j], v[2 * j + 1]};
+                    } else {
+                        const Split<T> s(v);
+#pragma unroll
+                        for (int j = 0; j < NQ; ++j)
+                            *(F*)(qt[SCALED ? 0 : j] + n * LQ + u % (RT * 2) * 8) = s.p[j];
+                    }
                 }
             __syncthreads();
             if (k == 0) {
@@ -751,15 +840,47 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                F b[RT];
+                F a[CT];
 #pragma unroll
-                for (int t = 0; t < RT; ++t)
-                    b[t] = column_frag(qt, LQ, s * 32, t * 16 + own_columns());
+                for (int c = 0; c < CT; ++c)
+                    a[c] = column_frag(pt, LP, s * 32, (wave * CT + c) * 16 + own_columns());
 #pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    const F a = column_frag(pt, LP, s * 32, (wave * CT + c) * 16 + own_columns());
+                for (int t = 0; t < RT; ++t) {
+                    if (SCALED) {
+                        f32x8 v;
+                        float m = 0.f;
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) acc[k][c][t] = mfma(a, b[t], acc[k][c][t]);
+                        for (int j = 0; j < 8; ++j) {
+                            v[j] = qf[(s * 32 + g * 8 + j) * LF + t * 16 + (lane & 15)];
+                            m = fmaxf(m, finite_size(v[j]));
+                        }
+                        m = fmaxf(m, __shfl_xor(m, 16, 64));
+                        const int e = shift_of(fmaxf(m, __shfl_xor(m, 32, 64)));
+                        if (__any(e > shift_q[t])) {
+                            const int to = max(e, shift_q[t]);
+                            const float f = ldexpf(1.f, shift_q[t] - to);
+#pragma unroll
+                            for (int l = 0; l < C; ++l)
+#pragma unroll
+                                for (int c = 0; c < CT; ++c) acc[l][c][t] *= f;
+                            shift_q[t] = to;
+                        }
+                        const Split<T> b(v * two_to(-shift_q[t]));
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i)
+#pragma unroll
+                            for (int c = 0; c < CT; ++c)
+                                acc[k][c][t] = mfma(a[c], b.p[i], acc[k][c][t]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i) {
+                            const F b = column_frag(qt[SCALED ? 0 : i], LQ, s * 32,
+                                                    t * 16 + own_columns());
+#pragma unroll
+                            for (int c = 0; c < CT; ++c)
+                                acc[k][c][t] = mfma(a[c], b, acc[k][c][t]);
+                        }
+                    }
                 }
             }
         }
@@ -774,6 +895,13 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
         slot = next;
     }
     if (DV) store_u();
+    if (SCALED)
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int k = 0; k < C; ++k)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) acc[k][c][t] *= two_to(shift_q[t]);
     if (whole) {                // the adapter's only tile: its gradient, rounded here
         T* o = whole + (long)f.adapter * NP * R;
 #pragma unroll
@@ -868,11 +996,11 @@ int r16_of(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 template <typename T, bool KCONT>
 void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int K, int R,
             const Rows& rows, int tiles,
-            const Scale& scale, void* V, int RP, float* part, long N, int splits, int kper,
+            const Scale& scale, float* V, float* part, long N, int splits, int kper,
             hipStream_t st) {
 #define GO(RT)                                                                                   \
     k_shrink<T, RT, KCONT><<<(unsigned)(tiles * splits), 256, 0, st>>>(                          \
-        (const T*)X, xs, xlimit, (const T*)W, wlimit, K, R, rows, scale, (T*)V, RP, part, N,     \
+        (const T*)X, xs, xlimit, (const T*)W, wlimit, K, R, rows, scale, V, part, N,             \
         splits, kper)
     const int R16 = r16_of(R);
     if (R16 == 16) GO(1);
@@ -883,16 +1011,16 @@ void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int
 }
 
 template <typename T, bool RCONT>
-void expand(const void* base, long bs, long blimit, void* out, long os, const void* V, int RP,
+void expand(const void* base, long bs, long blimit, void* out, long os, const float* V,
             const void* W, long wlimit, int M, int R, const Rows& rows, int tiles, int shift,
                 hipStream_t st) {
-    const int strips = (M + 255) / 256;
+    const int strips = (M + 255) / 256, R16 = r16_of(R);
 #define GO(RK)                                                                                   \
     k_expand<T, RK, RCONT><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
-        (const T*)base, bs, blimit, (T*)out, os, (const T*)V, RP, (const T*)W, wlimit, M, R,     \
+        (const T*)base, bs, blimit, (T*)out, os, V, R16, (const T*)W, wlimit, M, R,              \
         rows, strips, shift)
-    if (RP == 32) GO(1);
-    else if (RP == 64) GO(2);
+    if (R16 <= 32) GO(1);
+    else if (R16 == 64) GO(2);
     else GO(4);
 #undef GO
 }
@@ -909,14 +1037,14 @@ int outer_columns(int R, int with_u, long row_tiles, int NP) {
 
 // `whole`: every adapter's rows are one tile, and out holds zeros for those without rows.
 template <typename T, bool RCONT>
-void outer(const void* P, long ps, long plimit, int NP, const void* Q, int RP, float* part,
+void outer(const void* P, long ps, long plimit, int NP, const float* Q, float* part,
            const void* W, long wlimit, float* partv, long N, const Rows& rows, int tiles,
                int shift, int columns, int whole,
            void* out, int R, int L, hipStream_t st) {
     const int PC = columns, strips = (NP + PC - 1) / PC, R16 = r16_of(R);
 #define GO(RT, CT, NS)                                                                           \
     k_outer<T, RT, CT, NS><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
-        (const T*)P, ps, plimit, NP, (const T*)Q, RP, part, (const T*)W, wlimit, R, partv, N,    \
+        (const T*)P, ps, plimit, NP, Q, part, (const T*)W, wlimit, R, partv, N,                  \
         whole ? (T*)out : nullptr, RCONT, rows, strips, shift)
     if (tiles == 0) {           // no row has an adapter: the sum below writes zeros
     } else if (R16 == 16) {
@@ -946,8 +1074,8 @@ void outer(const void* P, long ps, long plimit, int NP, const void* Q, int RP, f
 
 extern "C" {
 
-// Row length of v and u: the contraction of expand, in steps of 32.
-int lowrank_rp(int R) { return R <= 32 ? 32 : R <= 64 ? 64 : 128; }
+// Row length of v, u and their shares.
+int lowrank_width(int R) { return r16_of(R); }
 
 // Workgroups that share a row tile's contraction: about two a CU, no share below a step.  Up to
 // `alone` steps stay with one: where the sum is a launch of its own, four do (8192 rows of 1024,
@@ -962,7 +1090,7 @@ int lowrank_splits(const long* counts, int S, long T, int K, int alone) {
 void launch_shrink(int type, int kcont, const void* X, long xs, long xlimit, const void* W,
                    long wlimit, int K, int R, const int* order, const int* segs,
                    const int* adapter, const long* counts, int S, int Bn, long T,
-                   const float* scale, float scale_all, void* V, float* part, int splits,
+                   const float* scale, float scale_all, float* V, float* part, int splits,
                    hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const Scale sc{scale, scale_all};
@@ -970,65 +1098,54 @@ void launch_shrink(int type, int kcont, const void* X, long xs, long xlimit, con
     if (tiles == 0) return;
     const int kper = ((K + splits - 1) / splits + S_KC - 1) / S_KC * S_KC;
     const long N = T * Bn;
-    const int RP = lowrank_rp(R);
-    if (type == LM_BF16)
-        kcont ? shrink<bf16_t, true>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part,
-                                     N, splits,
-                                     kper, st)
-              : shrink<bf16_t, false>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP,
-                                      part, N, splits,
-                                      kper, st);
-    else
-        kcont ? shrink<f16_t, true>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part,
-                                    N, splits, kper,
-                                    st)
-              : shrink<f16_t, false>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, RP, part,
-                                     N, splits,
-                                     kper, st);
-}
-
-void launch_shrink_sum(int type, int R, const int* order, const int* segs, const int* adapter,
-                       int S, int Bn, long T, const float* scale, float scale_all, void* V,
-                       const float* part, int splits, hipStream_t st) {
-    const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
-    const Scale sc{scale, scale_all};
-    const int RP = lowrank_rp(R), R16 = r16_of(R);
-    const long N = T * Bn, threads = N * (RP / 4);
-#define GO(T, GR)                                                                                \
-    k_shrink_sum<T, GR><<<(unsigned)((threads + 256 / GR - 1) / (256 / GR)), 256, 0, st>>>(      \
-        part, N, R, R16, splits, rows, sc, (T*)V, RP)
+#define GO(T, KCONT)                                                                             \
+    shrink<T, KCONT>(X, xs, xlimit, W, wlimit, K, R, rows, tiles, sc, V, part, N, splits, kper, st)
     if (type == LM_BF16) {
-        if (splits < 32) GO(bf16_t, 1);
-        else GO(bf16_t, 8);
+        if (kcont) GO(bf16_t, true);
+        else GO(bf16_t, false);
     } else {
-        if (splits < 32) GO(f16_t, 1);
-        else GO(f16_t, 8);
+        if (kcont) GO(f16_t, true);
+        else GO(f16_t, false);
     }
 #undef GO
 }
 
+void launch_shrink_sum(int R, const int* order, const int* segs, const int* adapter, int S, int Bn,
+                       long T, const float* scale, float scale_all, float* V, const float* part,
+                       int splits, hipStream_t st) {
+    const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
+    const Scale sc{scale, scale_all};
+    const int R16 = r16_of(R);
+    const long N = T * Bn, threads = N * (R16 / 4);
+#define GO(GR)                                                                                   \
+    k_shrink_sum<GR><<<(unsigned)((threads + 256 / GR - 1) / (256 / GR)), 256, 0, st>>>(         \
+        part, N, R, R16, splits, rows, sc, V)
+    if (splits < 32) GO(1);
+    else GO(8);
+#undef GO
+}
+
 void launch_expand(int type, int rcont, const void* base, long bs, long blimit, void* out,
-                   long os, const void* V, const void* W, long wlimit, int M, int R,
-                       const int* order, const int* segs,
-                   const int* adapter, const long* counts, int S, int Bn, long T,
-                   hipStream_t st) {
+                   long os, const float* V, const void* W, long wlimit, int M, int R,
+                   const int* order, const int* segs, const int* adapter, const long* counts,
+                   int S, int Bn, long T, hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     // rows a workgroup: as many as leave four workgroups a CU, 256 at most, 32 at least
     const long strips = (M + 255) / 256;
     int shift = 8;
     while (shift > 5 && tiles_of(counts, S, T, shift) * strips < 1024) --shift;
-    const int tiles = tiles_of(counts, S, T, shift), RP = lowrank_rp(R);
+    const int tiles = tiles_of(counts, S, T, shift);
     if (tiles == 0) return;
-    if (type == LM_BF16)
-        rcont ? expand<bf16_t, true>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows,
-                                     tiles, shift, st)
-              : expand<bf16_t, false>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows,
-                                      tiles, shift, st);
-    else
-        rcont ? expand<f16_t, true>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows,
-                                    tiles, shift, st)
-              : expand<f16_t, false>(base, bs, blimit, out, os, V, RP, W, wlimit, M, R, rows,
-                                     tiles, shift, st);
+#define GO(T, RCONT)                                                                             \
+    expand<T, RCONT>(base, bs, blimit, out, os, V, W, wlimit, M, R, rows, tiles, shift, st)
+    if (type == LM_BF16) {
+        if (rcont) GO(bf16_t, true);
+        else GO(bf16_t, false);
+    } else {
+        if (rcont) GO(f16_t, true);
+        else GO(f16_t, false);
+    }
+#undef GO
 }
 
 // A decode step: W passes twice on the average at most, four rows a pass.  16 adapters at the
@@ -1099,27 +1216,24 @@ int lowrank_outer_tiles(const long* counts, int S, long T, int shift) {
 int lowrank_one_reading(int R) { return R <= 32; }
 
 void launch_outer(int type, int rcont, const void* P, long ps, long plimit, int NP,
-                  const void* Q, float* part, const void* W, long wlimit, float* partv,
-                      const int* order, const int* segs,
-                  const int* adapter, const long* counts, int S, int Bn, long T, int shift,
-                  int columns, int whole, void* out, int R, int L, hipStream_t st) {
+                  const float* Q, float* part, const void* W, long wlimit, float* partv,
+                  const int* order, const int* segs, const int* adapter, const long* counts, int S,
+                  int Bn, long T, int shift, int columns, int whole, void* out, int R, int L,
+                  hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
-    const int tiles = tiles_of(counts, S, T, shift), RP = lowrank_rp(R);
+    const int tiles = tiles_of(counts, S, T, shift);
     const long N = T * Bn;
-    if (type == LM_BF16)
-        rcont ? outer<bf16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows,
-                                    tiles, shift,
-                                    columns, whole, out, R, L, st)
-              : outer<bf16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows,
-                                     tiles, shift,
-                                     columns, whole, out, R, L, st);
-    else
-        rcont ? outer<f16_t, true>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows,
-                                   tiles, shift,
-                                   columns, whole, out, R, L, st)
-              : outer<f16_t, false>(P, ps, plimit, NP, Q, RP, part, W, wlimit, partv, N, rows,
-                                    tiles, shift,
-                                    columns, whole, out, R, L, st);
+#define GO(T, RCONT)                                                                             \
+    outer<T, RCONT>(P, ps, plimit, NP, Q, part, W, wlimit, partv, N, rows, tiles, shift, columns,\
+                    whole, out, R, L, st)
+    if (type == LM_BF16) {
+        if (rcont) GO(bf16_t, true);
+        else GO(bf16_t, false);
+    } else {
+        if (rcont) GO(f16_t, true);
+        else GO(f16_t, false);
+    }
+#undef GO
 }
 
 }  // extern "C"

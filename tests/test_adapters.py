@@ -466,3 +466,133 @@ def test_kernel_refusals(monkeypatch):
     monkeypatch.setitem(globals(), "make", lambda *a: plain(
         *a, dtype=torch.bfloat16, dev="cuda"))
     test_refusals()
+
+
+def bounds32(t, dy, rows, scale):
+    """As `bounds`, of kernels that hold v = s x A and u = s dy B^T in fp32.
+
+    What they multiply is off from v by 2^-22 of it at most and 2^-37 of the
+    largest v (two fp16 parts of 11 digits, of numbers scaled to at most 2^15
+    and rounded or raised by 2^-24 + 2^-25; three bf16 parts are better than
+    both), and the sums have three times as many products.
+
+    A matrix instruction adds eight products at 2^-24 of the largest, in which
+    a subnormal operand counts with the exponent of the smallest normal number
+    (fp16: 2^-24 * 2^14 beside 2^-25 loses the latter).  So n products are off
+    by at most n 2^-24 of the sum of magnitudes, none taken below that number;
+    v's parts, scaled to 2^14, none below 2^-28 of the largest."""
+    dt = t["x"].dtype
+    eps, w = torch.finfo(dt).eps / 2, 2.0 ** -24
+    tiny = torch.finfo(dt).smallest_normal * eps * 2
+    y, x, a, b = (t[n].double().cpu() for n in ("y", "x", "a", "b"))
+    dy = dy.double().cpu()
+    K, M, R = x.shape[2], b.shape[2], b.shape[1]
+    r = dict(out=y.clone(), x=torch.zeros_like(x), a=torch.zeros_like(a),
+             b=torch.zeros_like(b))
+    e = {n: torch.zeros_like(v) for n, v in r.items()}
+
+    def size(p):
+        return p.abs().clamp_min(torch.finfo(dt).smallest_normal)
+
+    def inner(n, left, right, s):
+        v = s * left @ right
+        off = (n + 8) * w * abs(s) * size(left) @ size(right)
+        off += 2.0 ** -22 * v.abs() + 2.0 ** -37 * v.abs().max()
+        return v, off, v.abs().clamp_min(2.0 ** -28 * float(v.abs().max()))
+
+    for l in sorted(set(rows.index) - {-1}):
+        c = [i for i, k in enumerate(rows.index) if k == l]
+        s = float(scale[l]) if isinstance(scale, torch.Tensor) else scale
+        xs, ds = x[:, c].reshape(-1, K), dy[:, c].reshape(-1, M)
+        n = xs.shape[0]
+        v, ev, av = inner(K, xs, a[l], s)
+        u, eu, au = inner(M, ds, b[l].t(), s)
+        for name, value, err in (
+                ("out", v @ b[l],
+                 (ev + (3 * R + 8) * w * (av + ev)) @ size(b[l])),
+                ("x", u @ a[l].t(),
+                 (eu + (3 * R + 8) * w * (au + eu)) @ size(a[l]).t())):
+            r[name][:, c] += value.reshape(x.shape[0], len(c), -1)
+            e[name][:, c] += err.reshape(x.shape[0], len(c), -1)
+        r["a"][l] = xs.t() @ u
+        e["a"][l] = size(xs).t() @ (eu + (3 * n + 8) * w * (au + eu))
+        r["b"][l] = v.t() @ ds
+        e["b"][l] = (ev + (3 * n + 8) * w * (av + ev)).t() @ size(ds)
+    for k in r:
+        e[k] = e[k] * (1 + eps) + (eps + 2 * w) * r[k].abs() + tiny
+    return r, e
+
+
+def held_in_32_bits(t, rows, scale, dy):
+    want, err = bounds32(t, dy, rows, scale)
+    v = {n: p.detach().clone().requires_grad_() for n, p in t.items()}
+    out = lowrank_add(**v, rows=rows, scale=scale)
+    got = [("out", out), *zip("xab", torch.autograd.grad(
+        out, [v[n] for n in "xab"], dy))]
+    with torch.no_grad():
+        got.append(("out", lowrank_add(**t, rows=rows, scale=scale)))
+    for n, p in got:
+        off = (p.detach().double().cpu() - want[n]).abs()
+        assert (off <= err[n]).all(), (n, float((off / err[n]).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_kernel_intermediates_are_32_bits(shape, dtype):
+    t, rows, scale = make(*shape, seed=3, dtype=dtype, dev="cuda")
+    g = torch.Generator().manual_seed(4)
+    held_in_32_bits(t, rows, scale,
+                    torch.randn(t["y"].shape, generator=g).to(t["y"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [3, 16, 32, 60, 128])
+@pytest.mark.parametrize("T,B", [(1, 3), (50, 7)])
+def test_kernel_intermediates_past_fp16(T, B, R):
+    """x A beyond 65504 and dy B^T below 2^-24, results within the type."""
+    t, rows, scale = make(T, B, 90, 300, R, 2, seed=R, dtype=torch.float16,
+                          dev="cuda")
+    t["x"] *= 300
+    t["a"] *= 1000
+    t["b"] *= 1e-4
+    g = torch.Generator().manual_seed(4)
+    dy = (1e-3 * torch.randn(t["y"].shape, generator=g)).to(t["y"])
+    assert (t["x"].float()[:, :, None].abs().amax(0) * 1000).max() > 65504
+    held_in_32_bits(t, rows, scale, dy)
+    # columns of one gradient far apart: the large one takes no digits
+    t["a"][..., 0] *= 30
+    t["a"][..., 1:] /= 1000
+    held_in_32_bits(t, rows, scale, dy / 30)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R", [2, 16, 40, 128])
+def test_kernel_infinite_weights_and_gradients(R, dtype):
+    """Infinities where the sums in 64 bits have them, of the same sign."""
+    t, rows, _ = make(9, 6, 70, 90, R, 2, dtype=dtype, dev="cuda",
+                      index=[0, 1, -1, 0, 1, 0])
+    g = torch.Generator().manual_seed(4)
+    dy = torch.randn(t["y"].shape, generator=g).to(t["y"])
+    inf = float("inf")
+    for n, at, f in (("b", (0, 1, 5), inf), ("b", (1, 0, 88), -inf),
+                     ("a", (1, 60, 1), inf), ("dy", (2, 3, 7), -inf),
+                     ("x", (4, 4, 8), inf)):
+        c = {m: p.clone() for m, p in t.items()}
+        d = dy.clone()
+        (d if n == "dy" else c[n])[at] = f
+        both = []
+        for dev, to in (("cuda", dtype), ("cpu", torch.float64)):
+            v = {m: p.to(dev, to).requires_grad_() for m, p in c.items()}
+            out = lowrank_add(**v, rows=AdapterRows(rows.index, 2, device=dev))
+            both.append([out.detach(), *torch.autograd.grad(
+                out, [v[m] for m in "xab"], d.to(dev, to))])
+            with torch.no_grad():
+                both[-1].append(lowrank_add(**v, rows=AdapterRows(
+                    rows.index, 2, device=dev)))
+        for p, q in zip(*both):
+            p = p.double().cpu()
+            assert torch.equal(p.isnan(), q.isnan())
+            assert torch.equal(p == inf, q == inf)
+            assert torch.equal(p == -inf, q == -inf)
