@@ -11,7 +11,7 @@
 // them (y, dx), `outer` reads them again for the weights' gradients.  MFMA feeds on 32 of the
 // contraction at a time in the stream's own layout; accumulation, split sums, partial gradients,
 // v and u are fp32.  v and u meet the matrix instructions in parts of the type that add up to them
-// (`split`): of 16-bit v the products would carry 2^-8 of error, and an fp16 v beyond 65504 is an
+// (`in_parts`): of 16-bit v the products would carry 2^-8 of error, and an fp16 v beyond 65504 is an
 // infinity where the result need not be.  Each result is rounded once.
 //
 // Rows come grouped by adapter.  Sequences are time-major, row = t * Bn + column, and an adapter
@@ -69,52 +69,59 @@ template <typename F> DEVINL F trim(F v, long e, long limit, int left) {
     return __builtin_bit_cast(F, u);
 }
 
-// fp32 numbers as a sum of a 16-bit type's, operands of as many matrix instructions.  All parts
+// An fp32 number as the sum of a 16-bit type's, operands of as many matrix instructions.  All parts
 // have the number's sign, and none is zero unless it is: an infinity in the other operand then
 // gives that infinity, where plus and minus or zero times infinity would give NaN.
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-template <typename T> struct Split;
-// bf16 has fp32's range and a third of its digits: three parts, all but the last one's rest is
-// cut off, and the last has no more digits than fit.  Where nothing is left, 2^-30 of the first.
-template <> struct Split<bf16_t> {
-    static constexpr int N = 3;
-    bf16x8 p[N];
-    DEVINL Split(f32x8 v) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            auto cut = [](float x) { return __int_as_float(__float_as_int(x) & 0xffff0000); };
-            const float a = cut(v[j]), least = a * 0x1p-30f;
-            const float r = v[j] - a, b = fabsf(r) > 0.f ? cut(r) : least;  // infinity: r is NaN
-            const float q = r - b, c = fabsf(q) > 0.f ? q : least;
-            p[0][j] = __builtin_bit_cast(bf16_t, (short)(__float_as_int(a) >> 16));
-            p[1][j] = __builtin_bit_cast(bf16_t, (short)(__float_as_int(b) >> 16));
-            p[2][j] = __builtin_bit_cast(bf16_t, (short)(__float_as_int(c) >> 16));
-        }
-    }
-};
-// fp16 has not the range: the numbers come scaled so that the largest of those that a sum holds is
-// near 2^15 (`shift_of`).  Two parts: 22 digits, and an error of 2^-40 of the largest at most.
-template <> struct Split<f16_t> {
-    static constexpr int N = 2;
-    f16x8 p[N];
-    DEVINL Split(f32x8 v) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const f16_t least = (f16_t)(v[j] > 0.f ? 0x1p-24f : v[j] < 0.f ? -0x1p-24f : 0.f);
-            f16_t a = (f16_t)__builtin_amdgcn_cvt_pkrtz(v[j], 0.f)[0];
-            if (a == (f16_t)0.f) a = least;
-            const float r = v[j] - (float)a;
-            const f16_t b = (f16_t)r;
-            p[0][j] = a;
-            p[1][j] = fabsf(r) > 0.f && b != (f16_t)0.f && (r > 0.f) == (v[j] > 0.f) ? b : least;
-        }
-    }
-};
-// The power of two that brings numbers of which m is the largest to [2^14, 2^15), and its inverse
-// (m finite; both are normal numbers: of 0 or the least the shift is -120).
+//
+// bf16 has fp32's range and a third of its digits: three parts, each but the last cut off, and the
+// last one's digits fit.  Where nothing is left, 2^-30 of the first.
+constexpr int parts_of(bool fp16) { return fp16 ? 2 : 3; }
+DEVINL void in_parts(float v, bf16_t (&p)[3]) {
+    auto cut = [](float x) { return __int_as_float(__float_as_int(x) & 0xffff0000); };
+    const float a = cut(v), least = a * 0x1p-30f;
+    const float r = v - a, b = fabsf(r) > 0.f ? cut(r) : least;         // of infinity r is NaN
+    const float q = r - b, c = fabsf(q) > 0.f ? q : least;
+    p[0] = __builtin_bit_cast(bf16_t, (short)(__float_as_int(a) >> 16));
+    p[1] = __builtin_bit_cast(bf16_t, (short)(__float_as_int(b) >> 16));
+    p[2] = __builtin_bit_cast(bf16_t, (short)(__float_as_int(c) >> 16));
+}
+// fp16 has not the range: a row's numbers come scaled by a power of two that brings the largest to
+// [2^14, 2^15).  Two parts: 22 digits, and an error of 2^-37 of the largest at most.
+DEVINL void in_parts(float v, f16_t (&p)[2]) {
+    const f16_t least = (f16_t)(v > 0.f ? 0x1p-24f : v < 0.f ? -0x1p-24f : 0.f);
+    f16_t a = (f16_t)__builtin_amdgcn_cvt_pkrtz(v, 0.f)[0];
+    if (a == (f16_t)0.f) a = least;
+    const float r = v - (float)a;
+    const f16_t b = (f16_t)r;
+    p[0] = a;
+    p[1] = fabsf(r) > 0.f && b != (f16_t)0.f && (r > 0.f) == (v > 0.f) ? b : least;
+}
+// The exponent of that power's inverse for numbers of which m is the largest finite one; of zeros
+// alone -120, so that both powers are normal numbers.
 DEVINL int shift_of(float m) { return max((__float_as_int(m) >> 23) - 127 - 14, -120); }
 DEVINL float two_to(int e) { return __int_as_float((127 + e) << 23); }
 DEVINL float finite_size(float x) { return fabsf(x) < __builtin_huge_valf() ? fabsf(x) : 0.f; }
+
+// Eight parts times two to e <= 0, none of them zero that was not: 1, as bits, is 2^-24.
+DEVINL bf16x8 shifted(bf16x8 v, int) { return v; }
+DEVINL f16x8 shifted(f16x8 v, int e) {
+    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+    const u16x8 was = __builtin_bit_cast(u16x8, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __builtin_amdgcn_ldexph(v[j], (short)e);
+    const u16x8 least = __builtin_elementwise_min(was & (unsigned short)0x7fff, (u16x8)1);
+    const u16x8 size = __builtin_bit_cast(u16x8, v) & (unsigned short)0x7fff;
+    return __builtin_bit_cast(f16x8, __builtin_elementwise_max(size, least) |
+                                         was & (unsigned short)0x8000);
+}
+
+// A row of v or u in memory: its parts one behind the other, R16 numbers each, and fp16's shift.
+__host__ __device__ constexpr int row_length(bool fp16, int R16) {
+    return fp16 ? 2 * R16 + 8 : 3 * R16;
+}
+template <typename T> DEVINL int row_shift(const T* row, int R16) {
+    return *(const int*)(row + 2 * R16);
+}
 
 // The bits of a vector's first `left` elements, and the vector without the others.
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -187,6 +194,17 @@ DEVINL int running_sum(int x) {
     return x;
 }
 
+// The largest of a wave's numbers, none below `least`, the same way.
+DEVINL int wave_largest(int x, int least) {
+    x = max(x, __builtin_amdgcn_update_dpp(least, x, 0x111, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(least, x, 0x112, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(least, x, 0x114, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(least, x, 0x118, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(least, x, 0x142, 0xa, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(least, x, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
 // Which rows tile number `tile` holds.  A wave sums up the segments' tiles, 64 at a time.
 DEVINL Tile find_tile(const Rows& r, int tile, int shift) {
     const int lane = threadIdx.x & 63;
@@ -232,7 +250,7 @@ constexpr int S_KC = 256;   // contraction a step
 template <typename T, int RT, bool KCONT>
 __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs, long xlimit,
                                                 const T* __restrict__ W, long wlimit, int K, int R,
-                                                Rows rows, Scale scale, float* __restrict__ V,
+                                                Rows rows, Scale scale, T* __restrict__ V,
                                                 float* __restrict__ part, long N, int splits,
                                                 int kper) {
     typedef typename Frag<T>::type F;
@@ -321,21 +339,42 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long xs
 #pragma unroll
             for (int t = 0; t < RT; ++t) p[t * 16] = acc[t][i];
         } else {
-            float* v = V + r * (RT * 16) + (lane & 15);
+            constexpr bool SCALED = __is_same(T, f16_t);
+            constexpr int NQ = parts_of(SCALED);
+            float x[RT], m = 0.f;
 #pragma unroll
-            for (int t = 0; t < RT; ++t)        // zeros behind R, where an infinity left NaN
-                v[t * 16] = t * 16 + (lane & 15) < R ? acc[t][i] * sc : 0.f;
+            for (int t = 0; t < RT; ++t) {      // zeros behind R, where an infinity left NaN
+                x[t] = t * 16 + (lane & 15) < R ? acc[t][i] * sc : 0.f;
+                m = fmaxf(m, finite_size(x[t]));
+            }
+            T* v = V + r * row_length(SCALED, RT * 16);
+            int e = 0;
+            if (SCALED) {
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+                e = shift_of(m);
+                if ((lane & 15) == 0) *(int*)(v + 2 * RT * 16) = e;
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                T p[NQ];
+                in_parts(SCALED ? x[t] * two_to(-e) : x[t], p);
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) v[(j * RT + t) * 16 + (lane & 15)] = p[j];
+            }
         }
     }
 }
 
 // The shares summed in a fixed order and scaled; four of a row's R a thread.  GR groups of threads
 // take every GR-th share where there are many (98 of 8192 rows, rank 32).
-template <int GR>
+template <typename T, int GR>
 __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ part, long N, int R,
                                                     int R16, int splits, Rows rows, Scale scale,
-                                                    float* __restrict__ V) {
-    constexpr int TH = 256 / GR;
+                                                    T* __restrict__ V) {
+    typedef T out4 __attribute__((ext_vector_type(4)));
+    constexpr bool SCALED = __is_same(T, f16_t);
+    constexpr int TH = 256 / GR, NQ = parts_of(SCALED);
     __shared__ f32x4 sums[GR > 1 ? 256 : 1];
     const int group = threadIdx.x / TH;
     const long i = (long)blockIdx.x * TH + threadIdx.x % TH;
@@ -357,10 +396,29 @@ __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ pa
     }
     if (l < 0) return;
     const float sc = scale(l);
-    f32x4 v;
+    T* v = V + row * row_length(SCALED, R16);
+    float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = r + j < R ? s[j] * sc : 0.f;
-    *(f32x4*)(V + row * R16 + r) = v;
+    for (int j = 0; j < 4; ++j) {
+        s[j] = r + j < R ? s[j] * sc : 0.f;
+        m = fmaxf(m, finite_size(s[j]));
+    }
+    if (SCALED) {               // a row's threads are neighbours in a wave
+        for (int off = R16 / 8; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        const int e = shift_of(m);
+        if (r == 0) *(int*)(v + 2 * R16) = e;
+        s *= two_to(-e);
+    }
+    out4 o[NQ];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        T p[NQ];
+        in_parts(s[j], p);
+#pragma unroll
+        for (int k = 0; k < NQ; ++k) o[k][j] = p[k];
+    }
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) *(out4*)(v + k * R16 + r) = o[k];
 }
 
 // ---------------------------------------------------------------------------
@@ -369,25 +427,32 @@ __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ pa
 // the A operand and the rows are B's columns, so that a lane holds four neighbouring columns of
 // one row; the products pass through LDS in fp32 to the lanes that hold base for whole rows of
 // 256 columns: read and written as 512 neighbouring bytes (in the operand's layout, 64 at a time,
-// rows of 50000 ran at 3.5 TB/s), loaded one step ahead.
+// rows of 50000 ran at 3.5 TB/s), loaded one step ahead.  V's parts pass through LDS too, a step
+// ahead and read once a workgroup: every wave needs all of them, and in registers they cost rank
+// 128 half of its waves (16384 rows of 4096: 137 us).
 // ---------------------------------------------------------------------------
 template <typename T, int RK, bool RCONT>
 __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long blimit, T* out,
-                                                long os, const float* __restrict__ V, int R16,
+                                                long os, const T* __restrict__ V, int R16,
                                                 const T* __restrict__ W, long wlimit, int M, int R,
                                                 Rows rows, int strips, int shift) {
     typedef typename Frag<T>::type F;
     typedef typename Vec8<T>::type U8;
-    constexpr int LD = 256 + 16, LS = 256 + 4;
-    constexpr int BYTES = RCONT || RK * 32 * LD * 2 < 32 * LS * 4 ? 32 * LS * 4 : RK * 32 * LD * 2;
-    __shared__ __attribute__((aligned(16))) char lds[BYTES];
+    constexpr bool SCALED = __is_same(T, f16_t);
+    constexpr int LD = 256 + 16, LS = 256 + 4, NQ = parts_of(SCALED);
+    // V's rows of a step, part by part; eight more keep neighbouring rows in other banks
+    constexpr int VR = RK * 4, VL = NQ * RK * 32 + 8, NV = (32 * NQ * VR + 255) / 256;
+    constexpr int WB = RCONT ? 0 : RK * 32 * LD * 2, SB = 32 * LS * 4, STEP = SB + 32 * VL * 2;
+    __shared__ __attribute__((aligned(16))) char lds[WB > STEP ? WB : STEP];
     __shared__ int at[256];                     // the tile's rows, divided out once
     T* const wt = (T*)lds;                      // W, and when it is in registers
     float* const sums = (float*)lds;            // the products
+    T* const vt = (T*)(lds + SB);               // and V
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
     const int block = by_xcd();
     const Tile f = find_tile(rows, block / strips, shift);
     const int strip = block % strips * 256, m0 = strip + wave * 64;
+    const long LV = row_length(SCALED, R16);
     const bool mine = f.adapter >= 0;
     if (!mine && base == out) return;           // nothing to add in place
     const long jend = min(f.n, f.j0 + (1l << shift));
@@ -424,8 +489,8 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
     // a lane's share of base and out: eight columns of every eighth row
     const int m = strip + (tid & 31) * 8;
     const bool whole = m + 8 <= M;
-    F y[4];
-    f32x8 v[2][RK];
+    F y[4], v[NV];
+    int shifts[2], next_shifts[2];
     auto load_base = [&](long j0) {
         if (!base) return;
 #pragma unroll
@@ -436,19 +501,32 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
     };
     auto load_rows = [&](long j0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const long j = j0 + h * 16 + (lane & 15);
-            const long row = at[(j < jend ? j : jend - 1) - f.j0];
-#pragma unroll
-            for (int k = 0; k < RK; ++k) {          // a contraction of 32 is zeros behind 16
-                const bool there = RK > 1 || g * 8 < R16;
-                v[h][k] = *(const f32x8*)(V + row * R16 + (there ? k * 32 + g * 8 : 0));
-                if (!there) v[h][k] = 0.f;
-            }
+        for (int i = 0; i < NV; ++i) {
+            const int u = i * 256 + tid, n = u / VR % 32, c = u % VR * 8;
+            const long j = j0 + n, row = at[(j < jend ? j : jend - 1) - f.j0];
+            const bool there = RK > 1 || c < R16;       // zeros up to a contraction of 32
+            v[i] = *(const F*)(V + row * LV + min(u / VR / 32, NQ - 1) * R16 + (there ? c : 0));
+            if (!there) v[i] = F{};
         }
+        if (SCALED)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const long j = j0 + h * 16 + (lane & 15);
+                next_shifts[h] = row_shift(V + at[(j < jend ? j : jend - 1) - f.j0] * LV, R16);
+            }
     };
-    load_base(f.j0);
+    auto store_rows = [&]() {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int u = i * 256 + tid;
+            if (u < 32 * NQ * VR)
+                *(F*)(vt + u / VR % 32 * VL + u / VR / 32 * RK * 32 + u % VR * 8) = v[i];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) shifts[h] = next_shifts[h];
+    };
     if (mine) load_rows(f.j0);
+    load_base(f.j0);
     if (mine && !RCONT) {
 #pragma unroll
         for (int k = 0; k < RK; ++k)
@@ -456,32 +534,29 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
             for (int t = 0; t < 4; ++t)
                 w[k][t] = column_frag(wt, LD, k * 32, wave * 64 + t * 16 + own_columns());
     }
+    __syncthreads();                            // W is read
+    if (mine) {
+        store_rows();
+        load_rows(f.j0 + 32);
+    }
+    __syncthreads();
     auto multiply = [&](f32x4 (&acc)[2][4]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            int e = 0;
-            if (__is_same(T, f16_t)) {          // a row's lanes are 16 apart
-                float m = 0.f;
-#pragma unroll
-                for (int k = 0; k < RK; ++k)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_size(v[h][k][j]));
-                m = fmaxf(m, __shfl_xor(m, 16, 64));
-                e = shift_of(fmaxf(m, __shfl_xor(m, 32, 64)));
-            }
+            const T* row = vt + (h * 16 + (lane & 15)) * VL + g * 8;
 #pragma unroll
             for (int t = 0; t < 4; ++t) acc[h][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int k = 0; k < RK; ++k) {
-                const Split<T> s(__is_same(T, f16_t) ? v[h][k] * two_to(-e) : v[h][k]);
+            for (int i = 0; i < NQ; ++i)
 #pragma unroll
-                for (int i = 0; i < Split<T>::N; ++i)
+                for (int k = 0; k < RK; ++k) {
+                    const F p = *(const F*)(row + (i * RK + k) * 32);
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) acc[h][t] = mfma(w[k][t], s.p[i], acc[h][t]);
-            }
-            if (__is_same(T, f16_t))
+                    for (int t = 0; t < 4; ++t) acc[h][t] = mfma(w[k][t], p, acc[h][t]);
+                }
+            if (SCALED)                         // a lane's column of D is a row
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc[h][t] *= two_to(e);
+                for (int t = 0; t < 4; ++t) acc[h][t] *= two_to(shifts[h]);
         }
     };
     auto to_lds = [&](const f32x4 (&acc)[2][4]) {
@@ -499,9 +574,10 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
         for (; j0 + 32 <= jend; j0 += 32) {
             f32x4 acc[2][4];
             multiply(acc);
-            __syncthreads();                    // W, or the last step's products, are read
+            __syncthreads();                    // V and the last step's products are read
             to_lds(acc);
-            load_rows(j0 + 32);
+            store_rows();
+            load_rows(j0 + 64);
             __syncthreads();
             U8 o[4];
 #pragma unroll
@@ -523,7 +599,11 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
         f32x4 acc[2][4];
         if (mine) multiply(acc);
         __syncthreads();
-        if (mine) to_lds(acc);
+        if (mine) {
+            to_lds(acc);
+            store_rows();
+            load_rows(j0 + 64);
+        }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -550,10 +630,7 @@ __global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long bli
                             (T)((base ? (float)was[q] : 0.f) + (q < 4 ? lo[q & 3] : hi[q & 3]));
             }
         }
-        if (j0 + 32 < jend) {
-            load_base(j0 + 32);
-            if (mine) load_rows(j0 + 32);
-        }
+        if (j0 + 32 < jend) load_base(j0 + 32);
     }
 }
 
@@ -666,10 +743,8 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
 // CT columns and walks the tile's rows 64 at a time: they pass through LDS as they are, and both
 // operands are read from there with their columns' rows side by side.
 //
-// Q's numbers pass as their bf16 parts, split once on the way into LDS.  fp16's have to be scaled
-// first, by a power of two for each of Q's columns: such a column is the 16 lanes' own number in
-// B and in D, so every wave reads Q from LDS as it is, takes the largest of a column's 32 rows,
-// and, when that is larger than any before, brings the column's sums to the new scale.
+// fp16's rows of Q have shifts of their own, and a sum over rows has to have one: the largest so
+// far.  A row's parts are scaled to it on the way into LDS, and the sums when it grows.
 //
 // NS > 0: the rows meet W on the way too, partv[share][row][r] = sum over the workgroup's columns
 // of P[row][p] W_l[r][p] -- the backward pass's u, in shares of NS times as many columns.  dy is
@@ -678,7 +753,7 @@ __global__ __launch_bounds__(64) void k_expand_few(const T* base, long bs, T* ou
 // ---------------------------------------------------------------------------
 template <typename T, int RT, int CT, int NS>
 __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps, long plimit,
-                                               int NP, const float* __restrict__ Q,
+                                               int NP, const T* __restrict__ Q,
                                                float* __restrict__ part,
                                                const T* __restrict__ W, long wlimit, int R,
                                                float* __restrict__ partv, long N,
@@ -689,10 +764,11 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
     constexpr int C = DV ? NS : 1;                  // strips of PC columns
     constexpr bool SCALED = __is_same(T, f16_t);
     constexpr int PC = 64 * CT, S = PC / 32, LP = PC + 16, LQ = RT * 16 + (RT >= 4 ? 16 : 0);
-    constexpr int LW = C * PC + 8, LF = RT * 16 + 2, NQ = Split<T>::N;
+    constexpr int LW = C * PC + 8, NQ = parts_of(SCALED);
+    constexpr int R16 = RT * 16;
+    constexpr long LV = row_length(SCALED, R16);
     __shared__ __attribute__((aligned(16))) T pt[64 * LP];
-    __shared__ __attribute__((aligned(16))) T qt[SCALED ? 1 : NQ][SCALED ? 8 : 64 * LQ];
-    __shared__ __attribute__((aligned(16))) float qf[SCALED ? 64 * LF : 4];
+    __shared__ __attribute__((aligned(16))) T qt[NQ][64 * LQ];
     __shared__ __attribute__((aligned(16))) T wt[DV ? RT * 16 * LW : 8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
     const int block = by_xcd(), tile = block / shares, share = block % shares;
@@ -707,22 +783,23 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
             *(F*)(wt + r * LW + c) = trim(eight(W, e, wlimit), e, wlimit, r < R ? NP - p0 - c : 0);
         }
     }
-    f32x4 acc[C][CT][RT];
+    // A wave takes all of the ranks and a fourth of the columns; of many ranks a part and more of
+    // the columns, so that fewer operands are read from LDS (rank 128: 28 a step instead of 52).
+    constexpr int WR = RT == 8 ? 4 : RT == 4 ? 2 : 1, RW = RT / WR, CW = CT * WR;
+    const int ct0 = wave / WR * CW, rt0 = wave % WR * RW;
+    f32x4 acc[C][CW][RW];
 #pragma unroll
     for (int k = 0; k < C; ++k)
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+        for (int c = 0; c < CW; ++c)
 #pragma unroll
-            for (int t = 0; t < RT; ++t) acc[k][c][t] = f32x4{0, 0, 0, 0};
+            for (int t = 0; t < RW; ++t) acc[k][c][t] = f32x4{0, 0, 0, 0};
     const long jend = min(f.n, f.j0 + (1l << shift));
     constexpr int QV = (64 * RT * 2 + 255) / 256;       // vectors of Q a thread
     constexpr int PV = 64 * PC / 8 / 256, PW = PC / 8;  // of P; a row's
     constexpr int D = C > 1 ? 2 : 1;                    // strips of P ahead
-    F x[D][PV];
-    f32x8 q[QV];
-    int shift_q[RT];            // a column's sums are what they stand for over two to this
-#pragma unroll
-    for (int t = 0; t < RT; ++t) shift_q[t] = -120;
+    F x[D][PV], q[QV][NQ];
+    int shifts[QV], shift_of_lane = -120, shift_q = -120;   // of a vector's row; the sums'
     // Loads and stores end in the order they went out, and a wait for a load has to know how many
     // are younger: so nothing in the loop goes out on a condition (rows behind the last are the
     // last again), or the wait would drain all of them (8192 rows of 50000 in one group, a
@@ -756,8 +833,12 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
         for (int i = 0; i < QV; ++i) {
             const int u = i * 256 + tid, n = u / (RT * 2);
             if (n >= 64) continue;
-            q[i] = *(const f32x8*)(Q + (long)at[slot][n] * (RT * 16) + u % (RT * 2) * 8);
+            const T* row = Q + at[slot][n] * LV;
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) q[i][j] = *(const F*)(row + j * R16 + u % (RT * 2) * 8);
+            if (SCALED) shifts[i] = row_shift(row, R16);
         }
+        if (SCALED) shift_of_lane = row_shift(Q + at[slot][lane] * LV, R16);
     };
     // u of a step goes out in the next one, before its loads; rows behind the last, and the first
     // time all, to a row behind the shares that nobody reads.
@@ -802,22 +883,29 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
                 else if (p0 + (k + 1) * PC > NP) v = keep(v, mask);
                 *(F*)(pt + n * LP + tid % PW * 8) = v;
             }
+            if (SCALED && k == 0) {
+                const int e = wave_largest(shift_of_lane, -120);
+                if (e > shift_q) {
+                    const float f = ldexpf(1.f, shift_q - e);
+#pragma unroll
+                    for (int l = 0; l < C; ++l)
+#pragma unroll
+                        for (int c = 0; c < CW; ++c)
+#pragma unroll
+                            for (int t = 0; t < RW; ++t) acc[l][c][t] *= f;
+                    shift_q = e;
+                }
+            }
             if (k == 0)
 #pragma unroll
                 for (int i = 0; i < QV; ++i) {
                     const int u = i * 256 + tid, n = u / (RT * 2);
                     if (n >= 64) continue;
-                    const f32x8 v = j0 + n < jend ? q[i] : (f32x8)0.f;
-                    if (SCALED) {
-                        typedef float f32x2 __attribute__((ext_vector_type(2)));
-                        f32x2* to = (f32x2*)(qf + n * LF + u % (RT * 2) * 8);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) to[j] = f32x2{v[2 * j], v[2 * j + 1]};
-                    } else {
-                        const Split<T> s(v);
-#pragma unroll
-                        for (int j = 0; j < NQ; ++j)
-                            *(F*)(qt[SCALED ? 0 : j] + n * LQ + u % (RT * 2) * 8) = s.p[j];
+                    for (int j = 0; j < NQ; ++j) {
+                        F v = j0 + n < jend ? q[i][j] : F{};
+                        if (SCALED) v = shifted(v, shifts[i] - shift_q);
+                        *(F*)(qt[j] + n * LQ + u % (RT * 2) * 8) = v;
                     }
                 }
             __syncthreads();
@@ -840,47 +928,20 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                F a[CT];
+                F b[NQ][RW];
 #pragma unroll
-                for (int c = 0; c < CT; ++c)
-                    a[c] = column_frag(pt, LP, s * 32, (wave * CT + c) * 16 + own_columns());
+                for (int i = 0; i < NQ; ++i)
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    if (SCALED) {
-                        f32x8 v;
-                        float m = 0.f;
+                    for (int t = 0; t < RW; ++t)
+                        b[i][t] = column_frag(qt[i], LQ, s * 32, (rt0 + t) * 16 + own_columns());
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            v[j] = qf[(s * 32 + g * 8 + j) * LF + t * 16 + (lane & 15)];
-                            m = fmaxf(m, finite_size(v[j]));
-                        }
-                        m = fmaxf(m, __shfl_xor(m, 16, 64));
-                        const int e = shift_of(fmaxf(m, __shfl_xor(m, 32, 64)));
-                        if (__any(e > shift_q[t])) {
-                            const int to = max(e, shift_q[t]);
-                            const float f = ldexpf(1.f, shift_q[t] - to);
+                for (int c = 0; c < CW; ++c) {
+                    const F a = column_frag(pt, LP, s * 32, (ct0 + c) * 16 + own_columns());
 #pragma unroll
-                            for (int l = 0; l < C; ++l)
+                    for (int i = 0; i < NQ; ++i)
 #pragma unroll
-                                for (int c = 0; c < CT; ++c) acc[l][c][t] *= f;
-                            shift_q[t] = to;
-                        }
-                        const Split<T> b(v * two_to(-shift_q[t]));
-#pragma unroll
-                        for (int i = 0; i < NQ; ++i)
-#pragma unroll
-                            for (int c = 0; c < CT; ++c)
-                                acc[k][c][t] = mfma(a[c], b.p[i], acc[k][c][t]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < NQ; ++i) {
-                            const F b = column_frag(qt[SCALED ? 0 : i], LQ, s * 32,
-                                                    t * 16 + own_columns());
-#pragma unroll
-                            for (int c = 0; c < CT; ++c)
-                                acc[k][c][t] = mfma(a[c], b, acc[k][c][t]);
-                        }
-                    }
+                        for (int t = 0; t < RW; ++t)
+                            acc[k][c][t] = mfma(a, b[i][t], acc[k][c][t]);
                 }
             }
         }
@@ -897,22 +958,22 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
     if (DV) store_u();
     if (SCALED)
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+        for (int t = 0; t < RW; ++t)
 #pragma unroll
             for (int k = 0; k < C; ++k)
 #pragma unroll
-                for (int c = 0; c < CT; ++c) acc[k][c][t] *= two_to(shift_q[t]);
+                for (int c = 0; c < CW; ++c) acc[k][c][t] *= two_to(shift_q);
     if (whole) {                // the adapter's only tile: its gradient, rounded here
         T* o = whole + (long)f.adapter * NP * R;
 #pragma unroll
         for (int k = 0; k < C; ++k)
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
+            for (int c = 0; c < CW; ++c)
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
+                for (int t = 0; t < RW; ++t) {
                     typedef T out4 __attribute__((ext_vector_type(4), aligned(2)));
-                    const int p = p0 + k * PC + (wave * CT + c) * 16 + g * 4;
-                    const int r = t * 16 + (lane & 15);
+                    const int p = p0 + k * PC + (ct0 + c) * 16 + g * 4;
+                    const int r = (rt0 + t) * 16 + (lane & 15);
                     const f32x4 v = acc[k][c][t];
                     if (r >= R) continue;
                     if (!rcont && p + 4 <= NP) {
@@ -930,11 +991,11 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
 #pragma unroll
     for (int k = 0; k < C; ++k)
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+        for (int c = 0; c < CW; ++c)
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
-                *(f32x4*)(part + ((long)tile * RT * 16 + t * 16 + (lane & 15)) * LO + p0 + k * PC +
-                          (wave * CT + c) * 16 + g * 4) = acc[k][c][t];
+            for (int t = 0; t < RW; ++t)
+                *(f32x4*)(part + ((long)tile * RT * 16 + (rt0 + t) * 16 + (lane & 15)) * LO + p0 + k * PC +
+                          (ct0 + c) * 16 + g * 4) = acc[k][c][t];
 }
 
 // The weights' gradient: an adapter's tiles in a fixed order, rounded once.  An adapter without
@@ -996,11 +1057,11 @@ int r16_of(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 template <typename T, bool KCONT>
 void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int K, int R,
             const Rows& rows, int tiles,
-            const Scale& scale, float* V, float* part, long N, int splits, int kper,
+            const Scale& scale, void* V, float* part, long N, int splits, int kper,
             hipStream_t st) {
 #define GO(RT)                                                                                   \
     k_shrink<T, RT, KCONT><<<(unsigned)(tiles * splits), 256, 0, st>>>(                          \
-        (const T*)X, xs, xlimit, (const T*)W, wlimit, K, R, rows, scale, V, part, N,             \
+        (const T*)X, xs, xlimit, (const T*)W, wlimit, K, R, rows, scale, (T*)V, part, N,         \
         splits, kper)
     const int R16 = r16_of(R);
     if (R16 == 16) GO(1);
@@ -1011,13 +1072,13 @@ void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int
 }
 
 template <typename T, bool RCONT>
-void expand(const void* base, long bs, long blimit, void* out, long os, const float* V,
+void expand(const void* base, long bs, long blimit, void* out, long os, const void* V,
             const void* W, long wlimit, int M, int R, const Rows& rows, int tiles, int shift,
                 hipStream_t st) {
     const int strips = (M + 255) / 256, R16 = r16_of(R);
 #define GO(RK)                                                                                   \
     k_expand<T, RK, RCONT><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
-        (const T*)base, bs, blimit, (T*)out, os, V, R16, (const T*)W, wlimit, M, R,              \
+        (const T*)base, bs, blimit, (T*)out, os, (const T*)V, R16, (const T*)W, wlimit, M, R,    \
         rows, strips, shift)
     if (R16 <= 32) GO(1);
     else if (R16 == 64) GO(2);
@@ -1037,14 +1098,14 @@ int outer_columns(int R, int with_u, long row_tiles, int NP) {
 
 // `whole`: every adapter's rows are one tile, and out holds zeros for those without rows.
 template <typename T, bool RCONT>
-void outer(const void* P, long ps, long plimit, int NP, const float* Q, float* part,
+void outer(const void* P, long ps, long plimit, int NP, const void* Q, float* part,
            const void* W, long wlimit, float* partv, long N, const Rows& rows, int tiles,
                int shift, int columns, int whole,
            void* out, int R, int L, hipStream_t st) {
     const int PC = columns, strips = (NP + PC - 1) / PC, R16 = r16_of(R);
 #define GO(RT, CT, NS)                                                                           \
     k_outer<T, RT, CT, NS><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
-        (const T*)P, ps, plimit, NP, Q, part, (const T*)W, wlimit, R, partv, N,                  \
+        (const T*)P, ps, plimit, NP, (const T*)Q, part, (const T*)W, wlimit, R, partv, N,        \
         whole ? (T*)out : nullptr, RCONT, rows, strips, shift)
     if (tiles == 0) {           // no row has an adapter: the sum below writes zeros
     } else if (R16 == 16) {
@@ -1074,8 +1135,9 @@ void outer(const void* P, long ps, long plimit, int NP, const float* Q, float* p
 
 extern "C" {
 
-// Row length of v, u and their shares.
+// Numbers of a row of v's and u's shares, and 16-bit words of a row of v or u.
 int lowrank_width(int R) { return r16_of(R); }
+int lowrank_row(int type, int R) { return row_length(type == LM_F16, r16_of(R)); }
 
 // Workgroups that share a row tile's contraction: about two a CU, no share below a step.  Up to
 // `alone` steps stay with one: where the sum is a launch of its own, four do (8192 rows of 1024,
@@ -1090,7 +1152,7 @@ int lowrank_splits(const long* counts, int S, long T, int K, int alone) {
 void launch_shrink(int type, int kcont, const void* X, long xs, long xlimit, const void* W,
                    long wlimit, int K, int R, const int* order, const int* segs,
                    const int* adapter, const long* counts, int S, int Bn, long T,
-                   const float* scale, float scale_all, float* V, float* part, int splits,
+                   const float* scale, float scale_all, void* V, float* part, int splits,
                    hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const Scale sc{scale, scale_all};
@@ -1110,23 +1172,28 @@ void launch_shrink(int type, int kcont, const void* X, long xs, long xlimit, con
 #undef GO
 }
 
-void launch_shrink_sum(int R, const int* order, const int* segs, const int* adapter, int S, int Bn,
-                       long T, const float* scale, float scale_all, float* V, const float* part,
-                       int splits, hipStream_t st) {
+void launch_shrink_sum(int type, int R, const int* order, const int* segs, const int* adapter,
+                       int S, int Bn, long T, const float* scale, float scale_all, void* V,
+                       const float* part, int splits, hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
     const Scale sc{scale, scale_all};
     const int R16 = r16_of(R);
     const long N = T * Bn, threads = N * (R16 / 4);
-#define GO(GR)                                                                                   \
-    k_shrink_sum<GR><<<(unsigned)((threads + 256 / GR - 1) / (256 / GR)), 256, 0, st>>>(         \
-        part, N, R, R16, splits, rows, sc, V)
-    if (splits < 32) GO(1);
-    else GO(8);
+#define GO(T, GR)                                                                                \
+    k_shrink_sum<T, GR><<<(unsigned)((threads + 256 / GR - 1) / (256 / GR)), 256, 0, st>>>(      \
+        part, N, R, R16, splits, rows, sc, (T*)V)
+    if (type == LM_BF16) {
+        if (splits < 32) GO(bf16_t, 1);
+        else GO(bf16_t, 8);
+    } else {
+        if (splits < 32) GO(f16_t, 1);
+        else GO(f16_t, 8);
+    }
 #undef GO
 }
 
 void launch_expand(int type, int rcont, const void* base, long bs, long blimit, void* out,
-                   long os, const float* V, const void* W, long wlimit, int M, int R,
+                   long os, const void* V, const void* W, long wlimit, int M, int R,
                    const int* order, const int* segs, const int* adapter, const long* counts,
                    int S, int Bn, long T, hipStream_t st) {
     const Rows rows{order, (const int4*)segs, adapter, S, Bn, T};
@@ -1216,7 +1283,7 @@ int lowrank_outer_tiles(const long* counts, int S, long T, int shift) {
 int lowrank_one_reading(int R) { return R <= 32; }
 
 void launch_outer(int type, int rcont, const void* P, long ps, long plimit, int NP,
-                  const float* Q, float* part, const void* W, long wlimit, float* partv,
+                  const void* Q, float* part, const void* W, long wlimit, float* partv,
                   const int* order, const int* segs, const int* adapter, const long* counts, int S,
                   int Bn, long T, int shift, int columns, int whole, void* out, int R, int L,
                   hipStream_t st) {

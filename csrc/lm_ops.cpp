@@ -26,6 +26,7 @@ void launch_adjust(int, const void*, long, void*, const void*, long, int, int, c
                    float, const void*, long, int, const float*, long, int, const unsigned*, long,
                    long, int, hipStream_t);
 int lowrank_width(int R);
+int lowrank_row(int type, int R);
 int lowrank_splits(const long* counts, int S, long T, int K, int alone);
 int lowrank_outer_columns(const long* counts, int S, long T, int NP, int R, int with_u);
 int lowrank_outer_shift(const long* counts, int S, long T, int strips, int columns, int R);
@@ -38,13 +39,13 @@ int lowrank_outer_tiles(const long* counts, int S, long T, int shift);
 int lowrank_one_reading(int R);
 void launch_shrink(int, int, const void*, long, long, const void*, long, int, int, const int*,
                    const int*, const int*, const long*, int, int, long, const float*, float,
-                   float*, float*, int, hipStream_t);
-void launch_shrink_sum(int, const int*, const int*, const int*, int, int, long, const float*,
-                       float, float*, const float*, int, hipStream_t);
-void launch_expand(int, int, const void*, long, long, void*, long, const float*, const void*, long,
+                   void*, float*, int, hipStream_t);
+void launch_shrink_sum(int, int, const int*, const int*, const int*, int, int, long, const float*,
+                       float, void*, const float*, int, hipStream_t);
+void launch_expand(int, int, const void*, long, long, void*, long, const void*, const void*, long,
                    int, int, const int*, const int*, const int*, const long*, int, int, long,
                    hipStream_t);
-void launch_outer(int, int, const void*, long, long, int, const float*, float*, const void*, long,
+void launch_outer(int, int, const void*, long, long, int, const void*, float*, const void*, long,
                   float*, const int*, const int*, const int*, const long*, int, int, long, int,
                   int, int, void*, int, int, hipStream_t);
 }
@@ -410,24 +411,24 @@ struct Grouped {
     }
     const int* ip(const Tensor& t) const { return (const int*)t.data_ptr(); }
 
-    // v (N, width) = s x W in fp32, W (L, K, R) or, contraction contiguous, (L, R, K)
+    // v = s x W, N rows of fp32 numbers in parts (csrc/adapters.hip); W (L, K, R) or, contraction contiguous, (L, R, K)
     Tensor shrink(const Matrix& x, const Tensor& w_, bool kcont, hipStream_t st) const {
         const Tensor w = readable(w_);
         const int k = (int)x.cols, splits = lowrank_splits(counts.data(), S, T, k, 4);
-        const auto f32 = w.options().dtype(at::kFloat);
-        auto v = at::empty({N, (long)lowrank_width(R)}, f32);
+        auto v = at::empty({N, (long)lowrank_row(type, R)}, w.options());
         Tensor part;
-        if (splits > 1) part = at::empty({(long)splits * N * lowrank_width(R)}, f32);
+        if (splits > 1)
+            part = at::empty({(long)splits * N * lowrank_width(R)}, w.options().dtype(at::kFloat));
         launch_shrink(type, kcont, x.data(), x.stride, x.room, w.data_ptr(), room_of(w), k, R,
                       ip(order), ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale),
-                      scale_all, (float*)v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, splits, st);
+                      scale_all, v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, splits, st);
         if (splits > 1) sum(v, (const float*)part.data_ptr(), splits, st);
         check_launch("lowrank shrink");
         return v;
     }
     void sum(Tensor& v, const float* part, int splits, hipStream_t st) const {
-        launch_shrink_sum(R, ip(order), ip(segs), ip(adapter), S, Bn, T, float_ptr(scale),
-                          scale_all, (float*)v.data_ptr(), part, splits, st);
+        launch_shrink_sum(type, R, ip(order), ip(segs), ip(adapter), S, Bn, T, float_ptr(scale),
+                          scale_all, v.data_ptr(), part, splits, st);
     }
     // out = base + s x A B of a few rows an adapter, in two launches
     void few(const Matrix& base, const Matrix& out, const Matrix& x, const Tensor& a_,
@@ -449,12 +450,12 @@ struct Grouped {
                 bool rcont, hipStream_t st) const {
         const Tensor w = readable(w_);
         launch_expand(type, rcont, base.data(), base.stride, base.room, out.data(), out.stride,
-                      float_ptr(v), w.data_ptr(), room_of(w), (int)out.cols, R, ip(order),
+                      v.data_ptr(), w.data_ptr(), room_of(w), (int)out.cols, R, ip(order),
                       ip(segs), ip(adapter), counts.data(), S, Bn, T, st);
         check_launch("lowrank expand");
     }
     // sum over an adapter's rows of p^T q: (L, R, NP) or, rank contiguous, (L, NP, R).  With w
-    // (L, R, NP) also `u` (N, width) = s p w^T, from the same reading of p.
+    // (L, R, NP) also `u` = s p w^T, from the same reading of p.
     Tensor outer(const Matrix& p, const Tensor& q, bool rcont, hipStream_t st,
                  const Tensor& w_ = Tensor(), Tensor* u = nullptr) const {
         const Tensor w = readable(w_);
@@ -466,19 +467,20 @@ struct Grouped {
         const bool whole = lowrank_outer_whole(counts.data(), S, T, shift);
         // one workspace: the gradient's parts, u's shares and a row for what belongs to no row
         const long parts = whole ? 0 : tiles * width * strips * columns;
-        auto work = at::empty({parts + (u ? (strips * N + 1) * width : 0)}, q.options());
+        auto work = at::empty({parts + (u ? (strips * N + 1) * width : 0)},
+                              q.options().dtype(at::kFloat));
         float* part = (float*)work.data_ptr();
         const std::vector<int64_t> size = rcont ? std::vector<int64_t>{L, np, R}
                                                 : std::vector<int64_t>{L, R, np};
         // an adapter without rows has no tile to write its zeros
         auto out = whole && groups < L ? at::zeros(size, p.t.options())
                                        : at::empty(size, p.t.options());
-        launch_outer(type, rcont, p.data(), p.stride, p.room, np, float_ptr(q),
+        launch_outer(type, rcont, p.data(), p.stride, p.room, np, q.data_ptr(),
                      part, u ? w.data_ptr() : nullptr, u ? room_of(w) : 8,
                      u ? part + parts : nullptr, ip(order), ip(segs), ip(adapter),
                      counts.data(), S, Bn, T, shift, columns, whole, out.data_ptr(), R, L, st);
         if (u) {
-            *u = at::empty({N, (long)width}, q.options());
+            *u = at::empty({N, (long)lowrank_row(type, R)}, q.options());
             sum(*u, part + parts, strips, st);
         }
         check_launch("lowrank outer");
