@@ -429,10 +429,11 @@ __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ pa
 // 256 columns: read and written as 512 neighbouring bytes (in the operand's layout, 64 at a time,
 // rows of 50000 ran at 3.5 TB/s), loaded one step ahead.  V's parts pass through LDS too, a step
 // ahead and read once a workgroup: every wave needs all of them, and in registers they cost rank
-// 128 half of its waves (16384 rows of 4096: 137 us).
+// 128 half of its waves (16384 rows of 4096: 137 us, now 74).  dx, a stream of stores alone, runs
+// with a fourth workgroup a CU (65536 rows of 1024: 42 -> 36 us; with base 203 -> 205).
 // ---------------------------------------------------------------------------
 template <typename T, int RK, bool RCONT>
-__global__ __launch_bounds__(256) void k_expand(const T* base, long bs, long blimit, T* out,
+__global__ __launch_bounds__(256, RCONT && RK == 1 ? 4 : 1) void k_expand(const T* base, long bs, long blimit, T* out,
                                                 long os, const T* __restrict__ V, int R16,
                                                 const T* __restrict__ W, long wlimit, int M, int R,
                                                 Rows rows, int strips, int shift) {
