@@ -101,6 +101,13 @@ void check_launch(const char* name) {
     TORCH_CHECK(e == hipSuccess, name, ": ", hipGetErrorString(e));
 }
 
+// Forward-mode derivatives: a result without its tangent would make a wrong sum with others.
+void check_no_tangent(const char* name, std::initializer_list<OptTensor> inputs) {
+    for (const OptTensor& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.has_value() || !t->defined() || !t->_fw_grad(0).defined(),
+                                    name, " has no forward-mode derivative");
+}
+
 // Rows of any stride with neighbouring elements side by side; anything else is copied.
 Tensor rows_of(const Tensor& t) {
     return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous();
@@ -241,6 +248,7 @@ Tensor adjust(Tensor logits, OptTensor history, OptTensor lengths, OptTensor pro
     const long B = logits.size(0), V = logits.size(1);
     REQUIRE(V <= (1 << 30) && B * ((V + 2047) / 2048) < (1l << 24),
             "logits: V at most 2^30, and fewer than 2^24 parts of 2048 columns");
+    check_no_tangent("adjust_logits", {logits, repetition, presence, frequency, bias});
     const at::NoGradGuard off;
     const c10::DeviceGuard guard(logits.device());
     const int type = type_of(logits, "logits");
@@ -563,6 +571,7 @@ Tensor lowrank_add(Tensor y, Tensor x, Tensor a, Tensor b, Tensor order, Tensor 
                    double scale_all, bool inplace, int64_t adapters) {
     REQUIRE(a.dim() >= 1 && a.size(0) == adapters, "rows are of ", adapters, " adapters, a is ",
             a.sizes());
+    check_no_tangent("lowrank_add", {y, x, a, b, scale});
     if (!inplace && at::GradMode::is_enabled() &&
         (y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad()))
         return LowRankAdd::apply(y, x, a.contiguous(), b.contiguous(), order, segs, adapter,

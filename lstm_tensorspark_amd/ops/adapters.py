@@ -153,7 +153,8 @@ def lowrank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
                 b: torch.Tensor, rows: AdapterRows,
                 scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
     """y + scale * (x @ a[l]) @ b[l] with l the adapter of each row's column;
-    rows without an adapter are y's.  Differentiable in y, x, a and b.
+    rows without an adapter are y's.  Differentiable in y, x, a and b, once and
+    backward: the kernels refuse a tensor that carries a forward-mode tangent.
 
     y (..., B, M), x (..., B, K); a (L, K, R), b (L, R, M), R <= 128; rows of
     the B columns; scale a number or one for each adapter (L,), a constant.

@@ -146,7 +146,8 @@ def adjust_logits(logits: torch.Tensor,
     outside [0, V) is none, the same index twice adds both.
     allowed: (B, ceil(V / 32)) int32 as `pack_allowed` makes it.  A row that
     allows nothing comes back as -inf throughout; a masked NaN is -inf.
-    Not differentiable: this is the serving path.
+    Not differentiable: this is the serving path.  The kernel refuses tensors
+    that carry a forward-mode tangent.
     """
     if history is None:
         if not (lengths is prompt_lengths is repetition is presence

@@ -596,3 +596,35 @@ def test_kernel_infinite_weights_and_gradients(R, dtype):
             assert torch.equal(p.isnan(), q.isnan())
             assert torch.equal(p == inf, q == inf)
             assert torch.equal(p == -inf, q == -inf)
+
+
+def along(t, rows, scale, name, d, f):
+    """f's derivative along d of one of its tensors, forward mode."""
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        out = f(**{**t, name: fw.make_dual(t[name], d)}, rows=rows,
+                scale=scale)
+        return fw.unpack_dual(out).tangent
+
+
+@pytest.mark.parametrize("name", ["y", "x", "a", "b"])
+def test_reference_forward_mode(name):
+    t, rows, scale = make(2, 4, 3, 5, 2, 3, seed=1)
+    d = torch.randn_like(t[name])
+    got = along(t, rows, scale.double(), name, d, lowrank_add)
+    v = t[name].clone().requires_grad_()
+    w = torch.randn_like(t["y"])
+    g, = torch.autograd.grad(
+        lowrank_add(**{**t, name: v}, rows=rows, scale=scale.double()), v, w)
+    assert abs(float((got * w).sum() - (g * d).sum())) < 1e-12
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["y", "x", "a", "b"])
+def test_kernel_refuses_forward_mode(name):
+    t, rows, scale = make(2, 4, 30, 50, 2, 3, dtype=torch.bfloat16, dev="cuda")
+    for f in (lowrank_add, lowrank_add_):
+        with pytest.raises(NotImplementedError):
+            along(t, rows, scale, name, torch.randn_like(t[name]), f)
+    with torch.no_grad(), pytest.raises(NotImplementedError):
+        along(t, rows, scale, name, torch.randn_like(t[name]), lowrank_add)

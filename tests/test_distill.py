@@ -440,3 +440,13 @@ def test_kernel_teacher_gets_no_gradient():
     z.requires_grad_()
     distill_loss(z, i, t, y, alpha=0.5).backward()
     assert t.grad is None and z.grad is not None
+
+
+@pytest.mark.gpu
+def test_kernel_refuses_forward_mode():
+    fw = torch.autograd.forward_ad
+    z, i, t, y = make(4, 50, 3, dtype=torch.bfloat16, dev="cuda")
+    with fw.dual_level():
+        with pytest.raises(RuntimeError):
+            distill_loss(fw.make_dual(z, torch.ones_like(z)), i, t, y,
+                         alpha=0.5)

@@ -267,3 +267,17 @@ def test_kernel_refusals(monkeypatch):
     monkeypatch.setitem(globals(), "make", lambda *a: plain(
         *a, dtype=torch.bfloat16, dev="cuda"))
     test_refusals()
+
+
+@pytest.mark.gpu
+def test_kernel_refuses_forward_mode():
+    fw = torch.autograd.forward_ad
+    z, h, a = make(3, 50, 6, 4, dtype=torch.bfloat16, dev="cuda")
+    with fw.dual_level():
+        with pytest.raises(NotImplementedError):
+            adjust_logits(fw.make_dual(z, torch.ones_like(z)), h, **a)
+        for n in ("repetition", "presence", "frequency", "bias"):
+            with pytest.raises(NotImplementedError):
+                adjust_logits(z, h, **{**a, n: fw.make_dual(
+                    a[n], torch.ones_like(a[n]))})
+        adjust_logits(z, h, **a)
