@@ -218,9 +218,10 @@ class LogitRules:
         if (not isinstance(ok, torch.Tensor) or ok.dtype != torch.bool
                 or ok.shape != (vocab_size,)):
             raise ValueError(f"a grammar returns a ({vocab_size},) bool tensor")
+        # a copy: the grammar may fill the same tensor for the next row
+        ok = ok.clone()
         banned = [t for t, f in (self.bias or {}).items() if f == -math.inf]
         if banned:
-            ok = ok.clone()
             ok[banned] = False
         if not bool(ok.any()):
             raise ValueError(f"the grammar allows no token after {len(tokens)}")

@@ -223,6 +223,34 @@ def test_grammars_that_fail_end_their_request_only():
         solo(m, [1, 2], 6, LogitRules(grammar=later))
 
 
+class OneBuffer:
+    """A grammar that allows a request's first token alone, and answers with
+    one and the same tensor for every request."""
+
+    def __init__(self, dev="cpu"):
+        self.ok = torch.zeros(30, dtype=torch.bool, device=dev)
+
+    def __call__(self, tokens):
+        self.ok.fill_(False)
+        self.ok[tokens[0]] = True
+        return self.ok
+
+
+def grammars_with_one_buffer(m, dev):
+    rules = LogitRules(grammar=OneBuffer(dev))
+    out = m.generate(torch.tensor([[3, 9, 4]], device=dev), 5, rules=rules)
+    assert out.t().tolist() == [[3] * 6, [9] * 6, [4] * 6]
+    eng = ContinuousBatcher(m)
+    rids = [eng.submit([t], 5, rules=rules) for t in (3, 9, 4)]
+    eng.drain()
+    assert [eng.result(r, timeout=0) for r in rids] == [
+        [3] * 6, [9] * 6, [4] * 6]
+
+
+def test_grammars_may_answer_with_one_buffer():
+    grammars_with_one_buffer(LSTMModel(make_cfg()), "cpu")
+
+
 def test_grammar_is_not_asked_about_finished_columns():
     """Columns of one batch end at different steps."""
     m = LSTMModel(make_cfg())
@@ -428,6 +456,11 @@ def test_gpu_adapters_track_the_reference(head, bidi):
         off = (p.grad.float().cpu() - ref).norm() / ref.norm()
         assert off < 0.05, (n, float(off))
         assert (p.grad[0] == 0).all()
+
+
+@gpu
+def test_gpu_grammars_may_answer_with_one_buffer():
+    grammars_with_one_buffer(LSTMModel(make_cfg()).bfloat16().cuda(), "cuda")
 
 
 @gpu
