@@ -363,8 +363,6 @@ class LSTMModel(nn.Module):
         assert self.cfg.head == "lm", "generate() requires the LM head"
         assert not self.cfg.bidirectional, "decode is causal: fwd-only"
         assert prompt.dim() == 2 and prompt.dtype == torch.long
-        was_training = self.training
-        self.eval()
         if use_graph is None:
             use_graph = (temperature <= 0 and prompt.is_cuda and steps >= 16
                          and eos_token < 0 and rules is None
@@ -398,6 +396,9 @@ class LSTMModel(nn.Module):
                            for t, e in zip(past.tolist(), ended)]
             return every.apply(logits, past, None, allowed)
 
+        # behind every refusal: a refused call leaves the mode as it was
+        was_training = self.training
+        self.eval()
         try:
             out, state = self.forward(prompt, None, adapters)  # (Tp, B, V)
             cur = self._sample(ruled(out[-1], Tp), temperature, generator,

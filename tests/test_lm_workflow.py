@@ -311,6 +311,25 @@ def test_workflow_refusals():
         Trainer(Config(model=cfg), model=m, teacher=m)
 
 
+def test_a_refused_generate_keeps_the_training_mode():
+    m = LSTMModel(make_cfg())
+    prompt = torch.zeros(1, 1).long()
+    for training in (True, False):
+        m.train(training)
+        for kind, kw in ((ValueError, dict(rules=LogitRules(repetition=0.0))),
+                         (ValueError, dict(rules=LogitRules(bias={30: 1.0}))),
+                         (ValueError, dict(rules=LogitRules(
+                             grammar=lambda t: torch.zeros(30).bool()))),
+                         (AssertionError, dict(use_graph=True, eos_token=1)),
+                         (AssertionError, dict(use_graph=True,
+                                               temperature=1.0)),
+                         (AssertionError, dict(use_graph=True,
+                                               rules=LogitRules()))):
+            with pytest.raises(kind):
+                m.generate(prompt, 3, **kw)
+            assert m.training is training
+
+
 def distill_config(dtype="fp32", bptt=4):
     return Config(model=make_cfg(),
                   train=TrainConfig(batch_size=6, seq_len=8, bptt=bptt, lr=0.1,
