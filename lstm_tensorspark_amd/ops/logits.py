@@ -191,7 +191,8 @@ class LogitRules:
 
     def check(self, vocab_size: int):
         """Refuses what could leave a row without a finite logit to sample
-        from: the limits keep every adjusted logit of a bf16 model finite."""
+        from: the limits keep every adjusted logit finite in bf16 and fp32
+        (fp16's range ends at seven repeats; RowRules adjusts in fp32)."""
         if not 0.01 <= self.repetition <= 100.0:
             raise ValueError("repetition must be in [0.01, 100], got "
                              f"{self.repetition}")
@@ -259,9 +260,10 @@ class RowRules:
     def apply(self, logits: torch.Tensor, history: Optional[torch.Tensor],
               lengths: Optional[torch.Tensor],
               allowed: Sequence[Optional[torch.Tensor]] = ()) -> torch.Tensor:
-        """`adjust_logits` on the rows' (B, V) logits.  history (B, L) and
-        lengths (B,) are needed where a row penalizes; allowed: what the
-        grammars (LogitRules.allows) said for each row, None without one."""
+        """`adjust_logits` on the rows' (B, V) logits, fp16 ones as fp32.
+        history (B, L) and lengths (B,) are needed where a row penalizes;
+        allowed: what the grammars (LogitRules.allows) said for each row, None
+        without one."""
         args = dict(self.constant)
         if self.penalizes:
             args.update(history=history, lengths=lengths)
@@ -270,4 +272,8 @@ class RowRules:
             args["allowed"] = pack_allowed(torch.stack(
                 [(every if ok is None else ok).to(self.device)
                  for ok in allowed]))
-        return adjust_logits(logits, **args) if args else logits
+        if not args:
+            return logits
+        if logits.dtype == torch.float16:
+            logits = logits.float()
+        return adjust_logits(logits, **args)

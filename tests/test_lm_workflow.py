@@ -330,6 +330,36 @@ def test_a_refused_generate_keeps_the_training_mode():
             assert m.training is training
 
 
+def rules_at_their_limits(m, dev):
+    """Sampling in fp16 where the adjusted logits pass its range."""
+    torch.manual_seed(11)
+    for r in (LogitRules(frequency=-1e4), LogitRules(presence=-1e4),
+              LogitRules(frequency=1e4, presence=1e4),
+              LogitRules(repetition=100.0), LogitRules(repetition=0.01),
+              LogitRules(repetition=0.01, frequency=-1e4, presence=-1e4,
+                         bias={t: 1e4 for t in range(30)})):
+        prompt = torch.tensor([[1, 2]] * 9, device=dev)
+        prompt[:, 1] = torch.arange(9)
+        out = m.generate(prompt, 12, temperature=1.0, rules=r)
+        assert out.shape == (21, 2) and (out < 30).all()
+        if r == LogitRules(frequency=-1e4):     # what came first comes again
+            assert (out[9:, 0] == out[9, 0]).all()
+        eng = ContinuousBatcher(m)
+        rids = [eng.submit([1] * 9, 12, temperature=1.0, rules=r),
+                eng.submit([1] * 9, 12)]
+        eng.drain()
+        assert len(eng.result(rids[0], timeout=0)) == 21
+        assert eng.result(rids[1], timeout=0) == solo(m, [1] * 9, 12)
+
+
+def test_rules_at_their_limits_in_fp16():
+    torch.manual_seed(10)
+    m = LSTMModel(make_cfg()).half()
+    with torch.no_grad():
+        m.weight("head/b").mul_(0).add_(torch.linspace(-700, 700, 30))
+    rules_at_their_limits(m, "cpu")
+
+
 def distill_config(dtype="fp32", bptt=4):
     return Config(model=make_cfg(),
                   train=TrainConfig(batch_size=6, seq_len=8, bptt=bptt, lr=0.1,
@@ -480,6 +510,16 @@ def test_gpu_adapters_track_the_reference(head, bidi):
 @gpu
 def test_gpu_grammars_may_answer_with_one_buffer():
     grammars_with_one_buffer(LSTMModel(make_cfg()).bfloat16().cuda(), "cuda")
+
+
+@gpu
+def test_gpu_rules_at_their_limits_in_fp16():
+    torch.manual_seed(10)
+    m = LSTMModel(make_cfg(hidden=64)).half().cuda()
+    with torch.no_grad():
+        m.weight("head/b").mul_(0).add_(torch.linspace(
+            -700, 700, 30, device="cuda").half())
+    rules_at_their_limits(m, "cuda")
 
 
 @gpu
