@@ -200,8 +200,10 @@ class LogitRules:
             if not abs(x) <= 1e4:
                 raise ValueError(f"penalties must be in [-1e4, 1e4], got {x}")
         bias = self.bias or {}
-        if any(t < 0 or t >= vocab_size for t in bias):
-            raise ValueError(f"bias tokens must be in [0, {vocab_size})")
+        if any(not hasattr(t, "__index__") or t < 0 or t >= vocab_size
+               for t in bias):
+            raise ValueError("bias tokens must be whole numbers in "
+                             f"[0, {vocab_size})")
         if not all(f == -math.inf or abs(f) <= 1e4 for f in bias.values()):
             raise ValueError("a bias must be in [-1e4, 1e4] or -inf")
         if sum(f == -math.inf for f in bias.values()) == vocab_size:

@@ -223,6 +223,16 @@ def test_grammars_that_fail_end_their_request_only():
         solo(m, [1, 2], 6, LogitRules(grammar=later))
 
 
+def test_bias_tokens_are_whole_numbers():
+    m = LSTMModel(make_cfg())
+    eng = ContinuousBatcher(m)
+    for bad in (1.5, "3", None, 2.0):
+        with pytest.raises(ValueError):
+            eng.submit([1], 3, rules=LogitRules(bias={bad: 1.0}))
+        with pytest.raises(ValueError):
+            solo(m, [1], 3, LogitRules(bias={bad: 1.0}))
+
+
 class OneBuffer:
     """A grammar that allows a request's first token alone, and answers with
     one and the same tensor for every request."""
