@@ -29,6 +29,7 @@ serve); this is beyond-parity serving infrastructure.
 """
 from __future__ import annotations
 
+import dataclasses
 import itertools
 import threading
 from collections import deque
@@ -133,6 +134,9 @@ class ContinuousBatcher:
         if steps < 1 or steps > self.max_steps:
             raise ValueError(f"steps must be in [1, {self.max_steps}]")
         if rules is not None:
+            # as they are now: the caller may change the object for another
+            rules = dataclasses.replace(
+                rules, bias=dict(rules.bias) if rules.bias else None)
             rules.check(V)
         count = self.adapters.count if self.adapters is not None else 0
         if adapter < -1 or adapter >= count:

@@ -223,6 +223,22 @@ def test_grammars_that_fail_end_their_request_only():
         solo(m, [1, 2], 6, LogitRules(grammar=later))
 
 
+def test_a_request_keeps_the_rules_it_was_submitted_with():
+    torch.manual_seed(3)
+    m = LSTMModel(make_cfg())
+    eng = ContinuousBatcher(m)
+    rules = LogitRules(bias={11: 1e4})
+    first = eng.submit([1], 6, rules=rules)
+    eng.step()
+    rules.bias[11] = -1e4
+    rules.bias[12] = 2e4
+    rules.presence = 1e4
+    other = eng.submit([2], 6)          # a new batch reads its rules again
+    eng.drain()
+    assert eng.result(first, timeout=0)[1:] == [11] * 6
+    assert eng.result(other, timeout=0) == solo(m, [2], 6)
+
+
 def test_bias_tokens_are_whole_numbers():
     m = LSTMModel(make_cfg())
     eng = ContinuousBatcher(m)
