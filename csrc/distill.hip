@@ -56,7 +56,7 @@ struct Stats {
 
 template <int TH> DEVINL float block_max(float v, float* lds) {
     v = wave_max(v);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) lds[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)] = v;
     __syncthreads();
     v = lds[threadIdx.x & (TH / 64 - 1)];
 #pragma unroll
@@ -66,7 +66,7 @@ template <int TH> DEVINL float block_max(float v, float* lds) {
 }
 template <int TH> DEVINL float block_sum(float v, float* lds) {
     v = wave_sum(v);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) lds[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)] = v;
     __syncthreads();
     v = lds[threadIdx.x & (TH / 64 - 1)];
 #pragma unroll
@@ -220,42 +220,68 @@ template <int MODE> struct Grad {
 };
 
 // The listed columns and the label's in [lo, hi), written again after the stream (the caller has
-// synchronised): computed anew in 32 bits and rounded once.  An index that a row lists twice is
-// summed by its first entry.  `bits` holds hi - lo zero bits.
+// synchronised): computed anew in 32 bits and rounded once.  `bits` and `again` hold hi - lo zero
+// bits, whole windows of 256.  Of an index that a row lists twice the entries are summed in the
+// list's order: a wave walks the list once for a window of columns of its own, in `sums` (each
+// entry's own walk to find its like took four rows of 20000, one of them twice, 141 ms; now 0.4).
+constexpr int WINDOW = 256;
 template <typename T, int TH, int MODE>
 DEVINL void write_listed(const T* __restrict__ z, T* __restrict__ d, long row, int lo, int hi,
                          int V, const Lists& l, const Grad<MODE>& f, float rt, float lq,
-                         unsigned* bits, int* seen_label, int* twice) {
+                         unsigned* bits, unsigned* again, float* sums, int* seen_label,
+                         int* twice) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));       // nothing of this is worked out before the stream
     const long y = l.target ? l.target[row] : -1;
     if (f.soft) {
-        for (int k = threadIdx.x; k < l.K; k += TH) {
+        auto write = [&](long i, float q) {
+            d[i] = (T)(f((float)z[i]) - f.ak * q - (i == y ? f.ac : 0.f));
+        };
+        auto repeated = [&](long i) { return again[(i - lo) >> 5] >> ((i - lo) & 31) & 1; };
+        for (int k = tid; k < l.K; k += TH) {
             long i;
             float t;
             if (!entry(l, row, k, V, i, t) || i < lo || i >= hi) continue;
             const unsigned bit = 1u << ((i - lo) & 31);
-            if (atomicOr(&bits[(i - lo) >> 5], bit) & bit) *twice = 1;
+            if (atomicOr(&bits[(i - lo) >> 5], bit) & bit) {
+                atomicOr(&again[(i - lo) >> 5], bit);
+                *twice = 1;
+            }
             if (i == y) *seen_label = 1;
         }
         __syncthreads();
-        for (int k = threadIdx.x; k < l.K; k += TH) {
+        for (int k = tid; k < l.K; k += TH) {
             long i;
             float t;
             if (!entry(l, row, k, V, i, t) || i < lo || i >= hi) continue;
-            float q = exp2_((t - rt) * f.ct - lq);
-            bool first = true;
-            if (*twice) {
-                for (int j = 0; j < l.K; ++j) {
-                    long i2;
-                    float t2;
-                    if (j == k || !entry(l, row, j, V, i2, t2) || i2 != i) continue;
-                    if (j < k) first = false;
-                    else q += exp2_((t2 - rt) * f.ct - lq);
+            if (!repeated(i)) write(i, exp2_((t - rt) * f.ct - lq));
+        }
+        if (*twice) {
+            const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+            sums += wave * WINDOW;
+#pragma unroll 1
+            for (int w0 = lo + wave * WINDOW; w0 < hi; w0 += TH / 64 * WINDOW) {
+                if (!__any(again[((w0 - lo) >> 5) + (lane & 7)])) continue;
+                wave_fence();
+#pragma unroll 1
+                for (int i = 0; i < WINDOW / 64; ++i) sums[i * 64 + lane] = 0.f;
+                wave_fence();
+#pragma unroll 1
+                for (int k0 = 0; k0 < l.K; k0 += 64) {
+                    long i = 0;
+                    float t = 0.f;
+                    const bool mine = k0 + lane < l.K && entry(l, row, k0 + lane, V, i, t) &&
+                                      i >= w0 && i < min(w0 + WINDOW, hi) && repeated(i);
+                    add_in_order(mine, (int)i - w0, exp2_((t - rt) * f.ct - lq), sums);
                 }
+                wave_fence();
+#pragma unroll 1
+                for (int i = w0 + lane; i < min(w0 + WINDOW, hi); i += 64)
+                    if (repeated(i)) write(i, sums[i - w0]);
             }
-            if (first) d[i] = (T)(f((float)z[i]) - f.ak * q - (i == y ? f.ac : 0.f));
         }
     }
-    if (threadIdx.x == 0 && f.label && !*seen_label && y >= lo && y < hi)
+    if (tid == 0 && f.label && !*seen_label && y >= lo && y < hi)
         d[y] = (T)(f((float)z[y]) - f.ac);
 }
 
@@ -285,16 +311,21 @@ template <typename R> DEVINL void forget(R& v, float& a, float& b) {
 // A row in registers: TH threads hold NV vectors of eight each (50000 bf16 columns: 28 VGPRs of
 // 1024 threads, two workgroups a CU).  One read gives the maximum, the sums, the loss and, GRAD,
 // the gradient.
+// More than 80 scalar registers, as 96 with what the system keeps, would leave a CU one workgroup
+// of 1024 (1021 rows of 32001 fp32: 66 us instead of 56), a spilled one makes every wave wait for
+// its stores.
 // ---------------------------------------------------------------------------
 template <typename T, int MODE, int TH, int NV, bool GRAD>
-__global__ __launch_bounds__(TH, sizeof(T) * NV <= 14 ? 8 : 4) void k_distill_row(
+__global__ __launch_bounds__(TH, sizeof(T) * NV <= 14 ? 8 : 4)
+__attribute__((amdgpu_num_sgpr(80))) void k_distill_row(
     const T* __restrict__ logits, long zs, Lists l, Stats* __restrict__ stats,
     float* __restrict__ rows, const float* __restrict__ inv, T* __restrict__ dz, int V, float c1,
     float ct, float alpha, float tau) {
     typedef typename Raw<T>::type Vec;
     __shared__ float lds[TH / 64];
     __shared__ int seen_label, twice;
-    __shared__ unsigned bits[GRAD ? TH * NV / 4 : 1];
+    __shared__ unsigned bits[GRAD ? TH * NV / 4 : 1], again[GRAD ? TH * NV / 4 : 1];
+    __shared__ float sums[GRAD ? TH / 64 * WINDOW : 1];
     const int tid = threadIdx.x;
     const long row = blockIdx.x;
     const T* z = logits + row * zs;
@@ -309,7 +340,7 @@ __global__ __launch_bounds__(TH, sizeof(T) * NV <= 14 ? 8 : 4) void k_distill_ro
     const int last = (V & ~7) + tid;
     const float rest = last < V && tid < 8 ? (float)z[last] : neg_inf();
     if (GRAD) {
-        for (int i = tid; i < TH * NV / 4; i += TH) bits[i] = 0;
+        for (int i = tid; i < TH * NV / 4; i += TH) bits[i] = again[i] = 0;
         if (tid == 0) seen_label = twice = 0;
     }
     float m = rest, st = 0.f, s1 = 0.f;
@@ -361,8 +392,8 @@ __global__ __launch_bounds__(TH, sizeof(T) * NV <= 14 ? 8 : 4) void k_distill_ro
     // the row's registers are free from here on
     row_loss<T, TH>(z, row, V, l, m, l1, lt, ct, alpha, tau, stats, rows, lds);
     if (any)                                // row_loss has synchronised behind the stream
-        write_listed<T, TH, MODE>(z, d, row, 0, V, V, l, f, s.rt, s.lq, bits, &seen_label,
-                                  &twice);
+        write_listed<T, TH, MODE>(z, d, row, 0, V, V, l, f, s.rt, s.lq, bits, again, sums,
+                                  &seen_label, &twice);
 }
 
 // ---------------------------------------------------------------------------
@@ -432,7 +463,8 @@ __global__ __launch_bounds__(256) void k_distill_bwd(
     const float* __restrict__ inv, const float* __restrict__ grad, T* __restrict__ dz, int done,
     long N, int V, int chunks, int width, float c1, float ct, float alpha, float tau) {
     __shared__ int seen_label, twice;
-    __shared__ unsigned bits[512];      // width <= 16384 columns
+    __shared__ unsigned bits[512], again[512];      // width <= 16384 columns
+    __shared__ float sums[4 * WINDOW];
     if (done && *grad == 1.f) return;
     const float g = *grad * *inv;
     for (long b = blockIdx.x; b < N * chunks; b += gridDim.x) {
@@ -442,7 +474,7 @@ __global__ __launch_bounds__(256) void k_distill_bwd(
         T* d = dz + row * V;
         const Grad<MODE> f(stats[row], l, row, V, g, c1, ct, alpha, tau);
         const bool any = f.soft || f.label;
-        for (int i = threadIdx.x; i < 512; i += 256) bits[i] = 0;
+        for (int i = threadIdx.x; i < 512; i += 256) bits[i] = again[i] = 0;
         if (threadIdx.x == 0) seen_label = twice = 0;
         for (int v0 = lo + threadIdx.x * 8; v0 < hi; v0 += 256 * 8) {
             if (v0 + 8 <= hi) {
@@ -460,7 +492,7 @@ __global__ __launch_bounds__(256) void k_distill_bwd(
         __syncthreads();
         if (any)
             write_listed<T, 256, MODE>(z, d, row, lo, hi, V, l, f, stats[row].rt, stats[row].lq,
-                                       bits, &seen_label, &twice);
+                                       bits, again, sums, &seen_label, &twice);
         __syncthreads();                // bits and flags are used again by the next chunk
     }
 }

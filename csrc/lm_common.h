@@ -55,6 +55,27 @@ DEVINL float load_float(const void* p, long i, int type) {
     return ((const float*)p)[i];
 }
 
+// sums[at] += x of a wave's lanes that have one, lane by lane where `at` is the same: a list's
+// repeated indices are added in the list's order.  Every lane of the wave has to be there.
+DEVINL void add_in_order(bool has, int at, float x, float* sums) {
+    unsigned long long left = __ballot(has);
+    while (left) {
+        const int slot = __builtin_amdgcn_readlane(at, __ffsll(left) - 1);
+        unsigned long long same = __ballot(has && at == slot);
+        left &= ~same;
+        float s = sums[slot];
+        for (; same; same &= same - 1)
+            s += __int_as_float(
+                __builtin_amdgcn_readlane(__float_as_int(x), __ffsll(same) - 1));
+        sums[slot] = s;                 // the same from every lane
+    }
+}
+// LDS that one lane of the wave wrote and another reads, or the other way round.
+DEVINL void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+}
+
 DEVINL float wave_max(float v) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));

@@ -450,3 +450,63 @@ def test_kernel_refuses_forward_mode():
         with pytest.raises(RuntimeError):
             distill_loss(fw.make_dual(z, torch.ones_like(z)), i, t, y,
                          alpha=0.5)
+
+
+def seconds(f):
+    """The least of three runs on the GPU, after one."""
+    f()
+    times = []
+    for _ in range(3):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        torch.cuda.synchronize()
+        a.record()
+        f()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,K", [(300, 250), (9000, 4096), (40000, 5000),
+                                 (60000, 5000)])
+def test_kernel_long_lists_with_repeats(V, K, dtype):
+    """One index twice, and few indices a hundred times each: their entries
+    are summed in fp32, at most 128 of them, within the bound of
+    `check_on_gpu` (four times 192 roundings of q)."""
+    for few in (None, max(2, K // 40), 2 * WIDE):
+        z, i, t, y = make(3, V, K, seed=K, dtype=dtype, dev="cuda")
+        if few is None:
+            i[:, K // 3] = i[:, K - 1]
+        elif few >= V:
+            continue
+        else:
+            i = (torch.arange(K, device="cuda") * 7 % few * (V // few)) \
+                .repeat(3, 1)
+            i[1] = torch.where(i[1] < V // 2, i[1], -1)
+        y[0], y[1] = i[0, K - 1].clamp(0, V - 1), V - 1
+        a = check_on_gpu(z, i, t, y, 0.5, 2.0)
+        check_on_gpu(z, i, t, y, 1.0, 1.0, scale=0.5)
+        b = check_on_gpu(z, i, t, y, 0.5, 2.0)
+        assert torch.equal(a[1], b[1])
+
+
+WIDE = 256      # columns that one wave sums repeated entries of at once
+
+
+@pytest.mark.gpu
+def test_kernel_one_repeat_costs_no_walk_an_entry():
+    """Work is linear in the list's length, with repeats or without: a walk
+    through 20000 entries for each of them took five hundred times as long."""
+    z, i, t, _ = make(2, 50000, 20000, dtype=torch.bfloat16, dev="cuda",
+                      holes=False)
+    z.requires_grad_()
+    for scale in (1.0, 2.0):
+        def go():
+            (scale * distill_loss(z, i, t)).backward()
+        plain = seconds(go)
+        old = i[:, 777].clone()
+        i[:, 777] = i[:, 19000]
+        assert seconds(go) < 20 * plain
+        i[:, 777] = old

@@ -281,3 +281,49 @@ def test_kernel_refuses_forward_mode():
                 adjust_logits(z, h, **{**a, n: fw.make_dual(
                     a[n], torch.ones_like(a[n]))})
         adjust_logits(z, h, **a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,L,K", [(300, 5, 250), (9000, 50, 4000),
+                                   (20001, 4100, 4000)])
+def test_kernel_long_lists_of_biases_with_repeats(V, L, K, dtype):
+    for few in (None, 1, 30, 700):
+        z, h, a = make(3, V, L, K, seed=K, dtype=dtype, dev="cuda")
+        if few is None:         # one token twice
+            a["bias_index"] = torch.stack(
+                [torch.randperm(V, device="cuda")[:K] for _ in range(3)])
+            a["bias_index"][:, K // 3] = a["bias_index"][:, K - 1]
+        else:
+            a["bias_index"] = (torch.arange(K, device="cuda") * 7
+                               % min(few, V) * (V // min(few, V))).repeat(3, 1)
+            a["bias_index"][1, ::3] = -1
+        got = check_on_gpu(z, h, a)
+        assert torch.equal(got, adjust_logits(z, h, **a))
+
+
+@pytest.mark.gpu
+def test_kernel_one_repeat_costs_no_walk_an_entry():
+    """Work is linear in the list's length, with repeats or without: a walk
+    through 20000 biases for each of them took four thousand times as long."""
+    z = torch.randn(2, 50000, device="cuda")
+    i = torch.stack([torch.randperm(50000, device="cuda")[:20000]
+                     for _ in range(2)])
+    f = torch.randn(2, 20000, device="cuda")
+
+    def least():
+        times = []
+        for _ in range(4):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            torch.cuda.synchronize()
+            a.record()
+            for _ in range(5):
+                adjust_logits(z, bias_index=i, bias=f)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    plain = least()
+    i[:, 777] = i[:, 19000]
+    assert least() < 50 * plain
