@@ -149,7 +149,8 @@ void go(const void* z, long zs, void* out, const Adjust& a, long B, int V, hipSt
     // 2048 and of 8192, 64 rows of 50000: 16384 tokens 27 and 16 us, 4096 12.7 and 10.4, 1024 10.3
     // and 10.0; 1024 rows: 4096 tokens 105 and 97, 1024 75 and 92).
     const int small = (V + 2047) / 2048, large = (V + 8191) / 8192;
-    if (a.L >= 4096)
+    // A launch holds fewer than 2^32 threads: more rows than fit the large ones take the small.
+    if (a.L >= 4096 && B * large * 1024 < (1l << 32))
         k_adjust<T, 1024><<<(unsigned)(B * large), 1024, 0, stream>>>((const T*)z, zs, (T*)out, a,
                                                                       V, large);
     else

@@ -54,6 +54,17 @@ def test_adjust_far_rows():
         assert torch.equal(out[s], adjust_logits(z[s].clone(), h[s], **kw))
 
 
+def test_adjust_more_rows_than_large_workgroups_fit():
+    """2^22 rows with long histories: 1024 threads each are 2^32."""
+    n = 1 << 22
+    z = torch.randn(64, 3, device="cuda").bfloat16()
+    h = (torch.arange(4096, device="cuda") % 5)[None]
+    kw = dict(repetition=1.5, presence=0.5, frequency=0.25)
+    want = adjust_logits(z, h.expand(64, -1), **kw)
+    out = adjust_logits(z.repeat(n // 64, 1), h.expand(n, -1), **kw)
+    assert (out.view(-1, 64, 3) == want).all()
+
+
 def test_adapters_far_rows():
     y = big()
     x = torch.randn(N, 64, device="cuda").bfloat16()
