@@ -1121,8 +1121,9 @@ void outer(const void* P, long ps, long plimit, int NP, const void* Q, float* pa
     else GO(8, 2, 0);
 #undef GO
     if (whole) return;
-    if (tiles > 16 * L) {           // many tiles an adapter
-        const int blocks = (NP + 127) / 128 * R;
+    const long many = (NP + 127) / 128 * (long)R;
+    if (tiles > 16 * L && L * many * 256 < (1l << 32)) {    // many tiles an adapter
+        const int blocks = (int)many;
         k_outer_sum<T, RCONT, 8><<<(unsigned)L * blocks, 256, 0, st>>>(
             part, R16, strips * PC, rows, shift, (T*)out, NP, R, blocks);
     } else {

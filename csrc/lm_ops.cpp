@@ -414,8 +414,13 @@ struct Grouped {
         long sum = 0;
         for (long c : counts) sum += c;
         TORCH_CHECK(groups <= S && groups >= S - 1 && sum == Bn, "lowrank: groups");
-        REQUIRE(N < (1l << 31) && N / 64 * ((std::max(K, M) + 127) / 128) < (1l << 31),
-                "too many rows");
+        REQUIRE(N < (1l << 31), "too many rows");
+        check_grid(N / 64 + S, 256);                            // shrink
+        check_grid((N / 256 + S) * ((M + 255) / 256), 256);     // expand, also of few rows
+    }
+    // A launch holds fewer than 2^32 threads.
+    static void check_grid(long blocks, long threads) {
+        REQUIRE(blocks * threads < (1l << 32), "too many rows or adapters for one launch");
     }
     const int* ip(const Tensor& t) const { return (const int*)t.data_ptr(); }
 
@@ -457,6 +462,7 @@ struct Grouped {
     void expand(const Matrix& base, const Matrix& out, const Tensor& v, const Tensor& w_,
                 bool rcont, hipStream_t st) const {
         const Tensor w = readable(w_);
+        check_grid((N / 256 + S) * ((out.cols + 255) / 256), 256);
         launch_expand(type, rcont, base.data(), base.stride, base.room, out.data(), out.stride,
                       v.data_ptr(), w.data_ptr(), room_of(w), (int)out.cols, R, ip(order),
                       ip(segs), ip(adapter), counts.data(), S, Bn, T, st);
@@ -473,6 +479,9 @@ struct Grouped {
         const int shift = lowrank_outer_shift(counts.data(), S, T, strips, columns, R);
         const long tiles = lowrank_outer_tiles(counts.data(), S, T, shift);
         const bool whole = lowrank_outer_whole(counts.data(), S, T, shift);
+        check_grid(tiles * strips, 256);
+        check_grid((long)L * R * ((np + 1023) / 1024), 256);    // its sum
+        if (u) check_grid(N, width / 4);
         // one workspace: the gradient's parts, u's shares and a row for what belongs to no row
         const long parts = whole ? 0 : tiles * width * strips * columns;
         auto work = at::empty({parts + (u ? (strips * N + 1) * width : 0)},

@@ -95,6 +95,19 @@ def test_adapters_far_rows():
         assert ((dx[c].float() - want).abs() <= 2 ** -7 * size).all()
 
 
+def test_adapters_refuse_more_rows_than_a_launch_holds():
+    """Rows that are one and the same in memory: 2^30 / 64 workgroups of 256
+    threads are 2^32."""
+    one = torch.ones(1, 1, 1, device="cuda").bfloat16()
+    rows = AdapterRows([0], 1, device="cuda")
+    wide = one.expand(1 << 30, 1, 1)
+    with pytest.raises(ValueError, match="too many rows"):
+        lowrank_add(wide, wide, one, one, rows)
+    many = one.expand(1 << 22, 1, 1)
+    out = lowrank_add(many, many, one, one, rows)
+    assert (out == 2).all()
+
+
 def test_adapters_many_columns():
     """One group of every column of a wide batch, and an odd split of it."""
     n = 70001
