@@ -11,8 +11,8 @@ The engine is time-major, (T, B, .), and an adapter belongs to a sequence:
 and serves every projection of every step until the batch changes.
 
 bf16 and fp16 run the kernels of csrc/adapters.hip on the GPU (fp32
-accumulation; x @ A is rounded once to the type in between); the CPU, fp32
-and fp64 run the reference below, as the LSTM layers do.
+throughout, x @ A included; the result is rounded once); the CPU, fp32 and
+fp64 run the reference below, as the LSTM layers do.
 """
 from __future__ import annotations
 

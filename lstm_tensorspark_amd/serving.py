@@ -17,7 +17,8 @@ knobs (temperature/top-k/top-p with an OWN seeded generator, EOS
 early-stop) keep every request REPRODUCIBLE regardless of batch
 composition -- the test oracle is exact token-for-token parity with a
 solo `model.generate()` call, for greedy and seeded-sampled requests
-alike.
+alike.  Under an adapter on the GPU the logits are the same up to the
+order of fp32 sums, which depends on the rows that share it.
 
 This engine targets multi-tenant serving latency; the fixed-batch
 hipGraph decode (`model.generate(use_graph=True)`) remains the peak
@@ -123,9 +124,11 @@ class ContinuousBatcher:
         temperature > 0 samples with this request's OWN generator (seeded
         with `seed` when given), so a sampled request is reproducible and
         token-identical to a solo model.generate() with the same seed --
-        regardless of what else shares the batch.
+        regardless of what else shares the batch (with an adapter on the GPU:
+        up to the order of fp32 sums).
 
-        rules: this request's penalties, biases and grammar; a grammar that
+        rules: this request's penalties, biases and grammar, kept as they
+        are at this call; a grammar that
         raises or allows nothing ends the request, and result() raises what
         it raised.  adapter: one of the engine's AdapterSet, -1 for none."""
         V = self.model.cfg.vocab_size
