@@ -316,6 +316,8 @@ class LSTMModel(nn.Module):
         if teacher.shape != output.shape:
             raise ValueError(f"teacher's logits {tuple(teacher.shape)} and "
                              f"the model's {tuple(output.shape)} differ")
+        if top_k < 1:
+            raise ValueError(f"top_k must be positive, got {top_k}")
         C = output.shape[-1]
         top = teacher.detach().reshape(-1, C).topk(min(top_k, C), dim=1)
         return distill_loss(output.reshape(-1, C), top.indices, top.values,

@@ -337,6 +337,16 @@ def test_workflow_refusals():
         Trainer(Config(model=cfg), model=m, teacher=m)
 
 
+def test_a_teacher_without_entries_is_refused():
+    """top_k = 0 would leave (1 - alpha) of the label loss alone."""
+    m = LSTMModel(make_cfg())
+    z, y = torch.zeros(2, 3, 30), torch.zeros(2, 3).long()
+    for k in (0, -1):
+        with pytest.raises(ValueError):
+            m.distill_loss(z, z, y, top_k=k)
+    assert torch.isfinite(m.distill_loss(z, z, y, top_k=31))
+
+
 def test_a_refused_generate_keeps_the_training_mode():
     m = LSTMModel(make_cfg())
     prompt = torch.zeros(1, 1).long()
