@@ -11,8 +11,8 @@
 // them (y, dx), `outer` reads them again for the weights' gradients.  MFMA feeds on 32 of the
 // contraction at a time in the stream's own layout; accumulation, split sums, partial gradients,
 // v and u are fp32.  v and u meet the matrix instructions in parts of the type that add up to them
-// (`in_parts`): of 16-bit v the products would carry 2^-8 of error, and an fp16 v beyond 65504 is an
-// infinity where the result need not be.  Each result is rounded once.
+// (`in_parts`): of 16-bit v the products would carry 2^-8 of error, and an fp16 v beyond 65504 is
+// an infinity where the result need not be.  Each result is rounded once.
 //
 // Rows come grouped by adapter.  Sequences are time-major, row = t * Bn + column, and an adapter
 // belongs to a column, so only the Bn columns are grouped: segment s lists its columns in
@@ -433,10 +433,10 @@ __global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ pa
 // with a fourth workgroup a CU (65536 rows of 1024: 42 -> 36 us; with base 203 -> 205).
 // ---------------------------------------------------------------------------
 template <typename T, int RK, bool RCONT>
-__global__ __launch_bounds__(256, RCONT && RK == 1 ? 4 : 1) void k_expand(const T* base, long bs, long blimit, T* out,
-                                                long os, const T* __restrict__ V, int R16,
-                                                const T* __restrict__ W, long wlimit, int M, int R,
-                                                Rows rows, int strips, int shift) {
+__global__ __launch_bounds__(256, RCONT && RK == 1 ? 4 : 1)
+void k_expand(const T* base, long bs, long blimit, T* out, long os, const T* __restrict__ V,
+              int R16, const T* __restrict__ W, long wlimit, int M, int R, Rows rows, int strips,
+              int shift) {
     typedef typename Frag<T>::type F;
     typedef typename Vec8<T>::type U8;
     constexpr bool SCALED = __is_same(T, f16_t);
@@ -995,8 +995,8 @@ __global__ __launch_bounds__(256) void k_outer(const T* __restrict__ P, long ps,
         for (int c = 0; c < CW; ++c)
 #pragma unroll
             for (int t = 0; t < RW; ++t)
-                *(f32x4*)(part + ((long)tile * RT * 16 + (rt0 + t) * 16 + (lane & 15)) * LO + p0 + k * PC +
-                          (ct0 + c) * 16 + g * 4) = acc[k][c][t];
+                *(f32x4*)(part + ((long)tile * R16 + (rt0 + t) * 16 + (lane & 15)) * LO + p0 +
+                          k * PC + (ct0 + c) * 16 + g * 4) = acc[k][c][t];
 }
 
 // The weights' gradient: an adapter's tiles in a fixed order, rounded once.  An adapter without
@@ -1057,9 +1057,8 @@ int r16_of(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
 template <typename T, bool KCONT>
 void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int K, int R,
-            const Rows& rows, int tiles,
-            const Scale& scale, void* V, float* part, long N, int splits, int kper,
-            hipStream_t st) {
+            const Rows& rows, int tiles, const Scale& scale, void* V, float* part, long N,
+            int splits, int kper, hipStream_t st) {
 #define GO(RT)                                                                                   \
     k_shrink<T, RT, KCONT><<<(unsigned)(tiles * splits), 256, 0, st>>>(                          \
         (const T*)X, xs, xlimit, (const T*)W, wlimit, K, R, rows, scale, (T*)V, part, N,         \
@@ -1075,7 +1074,7 @@ void shrink(const void* X, long xs, long xlimit, const void* W, long wlimit, int
 template <typename T, bool RCONT>
 void expand(const void* base, long bs, long blimit, void* out, long os, const void* V,
             const void* W, long wlimit, int M, int R, const Rows& rows, int tiles, int shift,
-                hipStream_t st) {
+            hipStream_t st) {
     const int strips = (M + 255) / 256, R16 = r16_of(R);
 #define GO(RK)                                                                                   \
     k_expand<T, RK, RCONT><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \
@@ -1101,8 +1100,7 @@ int outer_columns(int R, int with_u, long row_tiles, int NP) {
 template <typename T, bool RCONT>
 void outer(const void* P, long ps, long plimit, int NP, const void* Q, float* part,
            const void* W, long wlimit, float* partv, long N, const Rows& rows, int tiles,
-               int shift, int columns, int whole,
-           void* out, int R, int L, hipStream_t st) {
+           int shift, int columns, int whole, void* out, int R, int L, hipStream_t st) {
     const int PC = columns, strips = (NP + PC - 1) / PC, R16 = r16_of(R);
 #define GO(RT, CT, NS)                                                                           \
     k_outer<T, RT, CT, NS><<<(unsigned)tiles * strips, 256, 0, st>>>(                            \

@@ -424,7 +424,8 @@ struct Grouped {
     }
     const int* ip(const Tensor& t) const { return (const int*)t.data_ptr(); }
 
-    // v = s x W, N rows of fp32 numbers in parts (csrc/adapters.hip); W (L, K, R) or, contraction contiguous, (L, R, K)
+    // v = s x W, N rows of fp32 numbers in parts (csrc/adapters.hip); W (L, K, R) or, contraction
+    // contiguous, (L, R, K)
     Tensor shrink(const Matrix& x, const Tensor& w_, bool kcont, hipStream_t st) const {
         const Tensor w = readable(w_);
         const int k = (int)x.cols, splits = lowrank_splits(counts.data(), S, T, k, 4);
@@ -434,7 +435,8 @@ struct Grouped {
             part = at::empty({(long)splits * N * lowrank_width(R)}, w.options().dtype(at::kFloat));
         launch_shrink(type, kcont, x.data(), x.stride, x.room, w.data_ptr(), room_of(w), k, R,
                       ip(order), ip(segs), ip(adapter), counts.data(), S, Bn, T, float_ptr(scale),
-                      scale_all, v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr, splits, st);
+                      scale_all, v.data_ptr(), splits > 1 ? (float*)part.data_ptr() : nullptr,
+                      splits, st);
         if (splits > 1) sum(v, (const float*)part.data_ptr(), splits, st);
         check_launch("lowrank shrink");
         return v;
