@@ -545,7 +545,8 @@ def test_gpu_adapters_track_the_reference(head, bidi):
 
 @gpu
 def test_gpu_grammars_may_answer_with_one_buffer():
-    grammars_with_one_buffer(LSTMModel(make_cfg()).bfloat16().cuda(), "cuda")
+    m = LSTMModel(make_cfg(hidden=64)).bfloat16().cuda()
+    grammars_with_one_buffer(m, "cuda")
 
 
 @gpu
